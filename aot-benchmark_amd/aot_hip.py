@@ -95,6 +95,13 @@ _SIGS = {
     'aot_bilinear_bwd_nhwc_f32': [_P, _P] + [_I] * 7 + [_P],
     'aot_window_gather_f32': [_P, _P] + [_I] * 4 + [_F, _P],
     'aot_window_scatter_f32': [_P, _P] + [_I] * 4 + [_F, _P],
+    'aot_rope': [_P] * 6 + [_I] * 9 + [_F, _P, _P],
+    'aot_rope_append': [_P] * 9 + [_I] * 7 + [_F, _I, _L, _P, _P],
+    'aot_attn_masked': [_P] * 10 + [_I] * 8 + [_F, _F, _P, _P],
+    'aot_attn_masked_bwd': [_P] * 15 + [_I] * 8 + [_F, _F, _P, _P],
+    'aot_paged_attn': [_P] * 10 + [_L] + [_I] * 7 + [_L, _F, _F, _P, _P],
+    'aot_paged_attn_work_floats': [_I] * 7 + [_P],
+    'aot_paged_evict': [_P] * 11 + [_I] * 8 + [_L] + [_I] * 3 + [_P, _P],
 }
 
 ACT_NONE, ACT_RELU, ACT_RELU6, ACT_GELU, ACT_SILU = 0, 1, 2, 3, 4
@@ -1023,3 +1030,289 @@ def sumsq_accum(x, out, stream=None):
         raise AotHipError('sumsq_accum: the accumulator must be float64')
     _chk(load().aot_sumsq_accum_f64(_dev(x), x.numel(), _dev(out), stream if stream is not None else stream_ptr()),
          'aot_sumsq_accum_f64')
+
+
+# ---- token sequences: rotary positions, masked attention, paged caches (csrc/rope.hip, masked_attn.hip, paged_attn.hip, paged_evict.hip)
+_DTYPE = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}
+_I32_MAX = 2 ** 31 - 1
+
+
+def _need(ok, what, *args):
+    if not ok:
+        raise AotHipError(what % args)
+
+
+class _OnDevice:
+    """The launch runs on the tensors' device, whichever is current, on that device's current stream."""
+
+    def __init__(self, *tensors):
+        dev = None
+        for t in tensors:
+            if t is None:
+                continue
+            if not t.is_cuda:
+                raise AotHipError('AOT HIP ops need ROCm device tensors (got %s); there is no CPU fallback' % t.device)
+            if dev is None:
+                dev = t.get_device()
+            elif t.get_device() != dev:
+                raise AotHipError('tensors on different devices: cuda:%d and cuda:%d' % (dev, t.get_device()))
+        self.dev = dev
+
+    def __enter__(self):
+        self.prev = torch.cuda.current_device()
+        if self.prev != self.dev:
+            torch.cuda.set_device(self.dev)
+        return torch._C._cuda_getCurrentRawStream(self.dev)
+
+    def __exit__(self, *exc):
+        if self.prev != self.dev:
+            torch.cuda.set_device(self.prev)
+        return False
+
+
+def _longs(*tensors):
+    """Host array of the leading dimensions' element strides (0 where a dimension has one place, whatever torch says there)."""
+    out = []
+    for t, n in tensors:
+        if t is None:
+            out += [0] * n
+        else:
+            sh, st = t.shape, t.stride()
+            out += [st[i] if sh[i] > 1 else 0 for i in range(n)]
+    return (_L * len(out))(*out)
+
+
+def _ptr(t):
+    return None if t is None else t.data_ptr()
+
+
+def _rows(t):
+    """t as the row kernels read it: last dimension dense, rows of 16-byte pieces at 16-byte addresses; a dense copy where it is not."""
+    n = 16 // t.element_size()
+    st = t.stride()
+    if t.numel() and ((st[-1] != 1 and t.shape[-1] > 1) or t.data_ptr() % 16 or any(s % n for s, d in zip(st[:-1], t.shape[:-1]) if d > 1)):
+        c = t.contiguous()
+        return c.clone(memory_format=torch.contiguous_format) if c.data_ptr() % 16 else c
+    return t
+
+
+def _dense_last(t):
+    return t if t is None or t.stride(-1) == 1 or t.shape[-1] <= 1 else t.contiguous()
+
+
+def _check_int32(name, t, shape):
+    _need(t.dtype == torch.int32 and tuple(t.shape) == tuple(shape), '%s must be int32 %s (got %s %s)', name, tuple(shape), t.dtype, tuple(t.shape))
+
+
+def _check_freqs(freqs, D):
+    _need(freqs.dtype == torch.float64 and freqs.dim() == 1 and freqs.is_contiguous() and 1 <= freqs.numel() <= D // 2,
+          'freqs must be a dense float64 vector of at most %d frequencies', D // 2)
+    return 2 * freqs.numel()
+
+
+def rope(q, k, pos, freqs, interleaved=False, mscale=1.0, inverse=False, stream=None):
+    """Rotary positions of q [B, S, H, D] and k [B, S, Hk, D] (or None) at pos [B, S] int32, freqs [rot / 2] float64 radians a position:
+    (q', k') (aot_rope; the first rot elements of a head turn, inverse: the gradient's direction)."""
+    _need(q.dim() == 4 and q.dtype in _DTYPE, 'rope: q must be [B, S, H, D] of float32 / float16 / bfloat16 (got %s %s)', tuple(q.shape), q.dtype)
+    B, S, H, D = q.shape
+    _need(k is None or (k.dim() == 4 and k.shape[:2] == q.shape[:2] and k.shape[3] == D and k.dtype == q.dtype),
+          'rope: k must be [B, S, Hk, D] like q')
+    _check_int32('rope: pos', pos, (B, S))
+    rot = _check_freqs(freqs, D)
+    _need(D <= 1024 and (not interleaved or D % 2 == 0), 'rope: head width %d not supported', D)
+    with _OnDevice(q, k, pos, freqs) as s:
+        q = _dense_last(q)
+        k = _dense_last(k)
+        if interleaved:
+            q, k = _rows(q), (None if k is None else _rows(k))
+        qo = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+        ko = torch.empty(k.shape, dtype=k.dtype, device=k.device) if k is not None else None
+        Hk = 0 if k is None else k.shape[2]
+        if H + Hk and B * S:
+            _chk(load().aot_rope(_ptr(q), _ptr(k), _ptr(qo), _ptr(ko), pos.data_ptr(), freqs.data_ptr(), _DTYPE[q.dtype], B, S, H, Hk, D,
+                                 rot, int(interleaved), int(inverse), mscale, _longs((q, 3), (k, 3), (qo, 3), (ko, 3), (pos, 2)),
+                                 stream if stream is not None else s), 'aot_rope')
+    return qo, ko
+
+
+def _check_pages(name, k_pages, v_pages, dtype, D=None, Hk=None):
+    _need(k_pages.dim() == 4 and k_pages.shape == v_pages.shape and k_pages.dtype == dtype and v_pages.dtype == dtype,
+          '%s: k_pages and v_pages must both be [pages, page, Hk, D] of %s', name, dtype)
+    P, page, h, d = k_pages.shape
+    _need((D is None or d == D) and (Hk is None or h == Hk), '%s: pages of %d heads of width %d do not fit the tokens', name, h, d)
+    _need(page >= 1 and page & (page - 1) == 0, '%s: the page size must be a power of two (got %d)', name, page)
+    _need(P * page <= _I32_MAX, '%s: a pool of %d places is too large', name, P * page)
+    for t in (k_pages, v_pages):
+        _need(t.stride(3) == 1 or d == 1, '%s: the last dimension of the pages must be dense', name)
+    return P, page, h, d
+
+
+def _check_page_rows(name, *pools):
+    for t in pools:
+        n = 16 // t.element_size()
+        _need(not t.numel() or (t.shape[3] % n == 0 and t.data_ptr() % 16 == 0 and all(x % n == 0 for x, d in zip(t.stride()[:3], t.shape[:3]) if d > 1)),
+              '%s: page rows must be whole 16-byte pieces at 16-byte addresses', name)
+
+
+def rope_append(q, k, v, pos, freqs, slots, k_pages, v_pages, interleaved=False, mscale=1.0, stream=None):
+    """New tokens q [N, H, D] (or None), k / v [N, Hk, D] at pos [N]: turns q and k, writes the turned keys and the values to the cache places
+    slots [N] int32 (page id * page + place; negative: not written) of k_pages / v_pages [pages, page, Hk, D], returns the turned q
+    (aot_rope_append)."""
+    _need(k.dim() == 3 and k.dtype in _DTYPE and v.shape == k.shape and v.dtype == k.dtype, 'rope_append: k and v must both be [N, Hk, D]')
+    N, Hk, D = k.shape
+    _need(q is None or (q.dim() == 3 and q.shape[0] == N and q.shape[2] == D and q.dtype == k.dtype), 'rope_append: q must be [N, H, D] like k')
+    _check_int32('rope_append: pos', pos, (N,))
+    _check_int32('rope_append: slots', slots, (N,))
+    rot = _check_freqs(freqs, D)
+    _need(D <= 1024 and (not interleaved or D % 2 == 0), 'rope_append: head width %d not supported', D)
+    P, page, _, _ = _check_pages('rope_append', k_pages, v_pages, k.dtype, D, Hk)
+    if interleaved:
+        for t in (k_pages, v_pages):
+            _need(t.data_ptr() % (2 * t.element_size()) == 0 and all(x % 2 == 0 for x, d in zip(t.stride()[:3], t.shape[:3]) if d > 1),
+                  'rope_append: interleaved pairs need pages aligned to pairs')
+    with _OnDevice(q, k, v, pos, freqs, slots, k_pages, v_pages) as s:
+        q, k, v = _dense_last(q), _dense_last(k), _dense_last(v)
+        pos, slots = pos.contiguous(), slots.contiguous()
+        if interleaved:
+            q, k, v = (None if q is None else _rows(q)), _rows(k), _rows(v)
+        qo = torch.empty(q.shape, dtype=q.dtype, device=q.device) if q is not None else None
+        if N and Hk:
+            _chk(load().aot_rope_append(_ptr(q), _ptr(k), _ptr(v), _ptr(qo), _ptr(k_pages), _ptr(v_pages), pos.data_ptr(), slots.data_ptr(),
+                                        freqs.data_ptr(), _DTYPE[k.dtype], N, 0 if q is None else q.shape[1], Hk, D, rot, int(interleaved),
+                                        mscale, page, P, _longs((q, 2), (k, 2), (v, 2), (qo, 2), (k_pages, 3), (v_pages, 3)),
+                                        stream if stream is not None else s), 'aot_rope_append')
+    return qo
+
+
+def _masked_args(name, q, k, v, scale, softcap, slopes, doc_q, doc_k, prefix):
+    _need(q.dim() == 4 and k.dim() == 4 and q.dtype in _DTYPE and k.dtype == q.dtype and v.dtype == q.dtype and v.shape == k.shape,
+          '%s: q must be [B, Sq, H, D], k and v [B, Sk, Hk, D], of one of float32 / float16 / bfloat16', name)
+    B, Sq, H, D = q.shape
+    Sk, Hk = k.shape[1:3]
+    _need(k.shape[0] == B and k.shape[3] == D and Hk >= 1 and H >= Hk and H % Hk == 0, '%s: q %s and k %s do not fit', name, tuple(q.shape), tuple(k.shape))
+    _need(1 <= D <= 128 and D * q.element_size() % 16 == 0, '%s: head width %d of %s not supported (whole 16-byte pieces, at most 128)', name, D, q.dtype)
+    _need(max(Sq, Sk) <= 1 << 22 and B <= 65535, '%s: sizes beyond 2^22 tokens or 65535 sequences', name)
+    _need(softcap >= 0, '%s: softcap must not be negative', name)
+    _need(slopes is None or (slopes.dtype == torch.float32 and tuple(slopes.shape) == (H,) and slopes.is_contiguous()), '%s: slopes must be dense float32 [H]', name)
+    _need((doc_q is None) == (doc_k is None), '%s: doc_q and doc_k go together', name)
+    if doc_q is not None:
+        _check_int32(name + ': doc_q', doc_q, (B, Sq))
+        _check_int32(name + ': doc_k', doc_k, (B, Sk))
+    if prefix is not None:
+        _check_int32(name + ': prefix', prefix, (B,))
+    return B, Sq, Sk, H, Hk, D, float(D ** -0.5 if scale is None else scale)
+
+
+def attn_masked(q, k, v, scale=None, causal=False, softcap=0.0, slopes=None, doc_q=None, doc_k=None, prefix=None, stream=None):
+    """Attention under masks (aot_attn_masked): q [B, Sq, H, D], k / v [B, Sk, Hk, D] -> (out [B, Sq, H, D], lse [B, H, Sq] in powers of two)."""
+    B, Sq, Sk, H, Hk, D, scale = _masked_args('attn_masked', q, k, v, scale, softcap, slopes, doc_q, doc_k, prefix)
+    with _OnDevice(q, k, v, slopes, doc_q, doc_k, prefix) as s:
+        q, k, v = _rows(q), _rows(k), _rows(v)
+        doc_q, doc_k = _dense_last(doc_q), _dense_last(doc_k)
+        prefix = None if prefix is None else prefix.contiguous()
+        out = torch.empty((B, Sq, H, D), dtype=q.dtype, device=q.device)
+        lse = torch.empty((B, H, Sq), dtype=torch.float32, device=q.device)
+        ranges = torch.empty(4 * B * (-(-Sq // 64) + -(-Sk // 64)), dtype=torch.int32, device=q.device) if doc_q is not None else None
+        if B and Sq:
+            _chk(load().aot_attn_masked(_ptr(q), _ptr(k), _ptr(v), _ptr(out), _ptr(lse), _ptr(slopes), _ptr(doc_q), _ptr(doc_k) or _ptr(doc_q),
+                                        _ptr(prefix), _ptr(ranges), _DTYPE[q.dtype], B, Sq, Sk, H, Hk, D, int(causal), scale, softcap,
+                                        _longs((q, 3), (k, 3), (v, 3), (out, 3), (doc_q, 1), (doc_k, 1)), stream if stream is not None else s),
+                 'aot_attn_masked')
+    return out, lse
+
+
+def attn_masked_bwd(dout, q, k, v, out, lse, scale=None, causal=False, softcap=0.0, slopes=None, doc_q=None, doc_k=None, prefix=None, stream=None):
+    """Gradients of attn_masked (aot_attn_masked_bwd): its inputs, results and the gradient of out -> (dq, dk, dv)."""
+    B, Sq, Sk, H, Hk, D, scale = _masked_args('attn_masked_bwd', q, k, v, scale, softcap, slopes, doc_q, doc_k, prefix)
+    _need(dout.shape == q.shape and out.shape == q.shape and dout.dtype == q.dtype and out.dtype == q.dtype, 'attn_masked_bwd: out and dout must be like q')
+    _need(lse.dtype == torch.float32 and tuple(lse.shape) == (B, H, Sq) and lse.is_contiguous(), 'attn_masked_bwd: lse must be dense float32 [B, H, Sq]')
+    with _OnDevice(q, k, v, out, dout, lse, slopes, doc_q, doc_k, prefix) as s:
+        q, k, v, out, dout = _rows(q), _rows(k), _rows(v), _rows(out), _rows(dout)
+        doc_q, doc_k = _dense_last(doc_q), _dense_last(doc_k)
+        prefix = None if prefix is None else prefix.contiguous()
+        dev = q.device
+        dq = torch.empty((B, Sq, H, D), dtype=q.dtype, device=dev)
+        dk = torch.empty((B, Sk, Hk, D), dtype=q.dtype, device=dev)
+        dv = torch.empty((B, Sk, Hk, D), dtype=q.dtype, device=dev)
+        delta = torch.empty(B * H * Sq, dtype=torch.float32, device=dev)
+        ranges = torch.empty(4 * B * (-(-Sq // 64) + -(-Sk // 64)), dtype=torch.int32, device=dev) if doc_q is not None else None
+        if B and (Sq or Sk):
+            _chk(load().aot_attn_masked_bwd(_ptr(q), _ptr(k), _ptr(v), _ptr(out), _ptr(lse), _ptr(dout), _ptr(dq), _ptr(dk), _ptr(dv), _ptr(slopes),
+                                            _ptr(doc_q) or _ptr(doc_k), _ptr(doc_k) or _ptr(doc_q), _ptr(prefix), _ptr(ranges), _ptr(delta), _DTYPE[q.dtype],
+                                            B, Sq, Sk, H, Hk, D, int(causal), scale, softcap,
+                                            _longs((q, 3), (k, 3), (v, 3), (out, 3), (dout, 3), (dq, 3), (dk, 3), (dv, 3), (doc_q, 1), (doc_k, 1)),
+                                            stream if stream is not None else s), 'aot_attn_masked_bwd')
+    return dq, dk, dv
+
+
+def paged_attn(q, k_pages, v_pages, table, lengths, scale=None, softcap=0.0, slopes=None, weights=None, key_pos=None, out=None, stream=None):
+    """One new token per sequence, q [B, H, D], over a paged cache (aot_paged_attn): table [B, max_pages] and lengths [B] int32, k_pages /
+    v_pages [pages, page, Hk, D]; weights [B, Hk, S] float32 is added to in place, key_pos [B, Hk, S] int32, S >= max_pages * page."""
+    _need(q.dim() == 3 and q.dtype in _DTYPE, 'paged_attn: q must be [B, H, D] of float32 / float16 / bfloat16')
+    B, H, D = q.shape
+    P, page, Hk, _ = _check_pages('paged_attn', k_pages, v_pages, q.dtype, D)
+    _need(Hk >= 1 and H >= Hk and H % Hk == 0, 'paged_attn: %d query heads on %d key heads', H, Hk)
+    _need(1 <= D <= 256 and D * q.element_size() % 16 == 0, 'paged_attn: head width %d of %s not supported (whole 16-byte pieces, at most 256)', D, q.dtype)
+    _check_page_rows('paged_attn', k_pages, v_pages)
+    _need(table.dim() == 2 and table.dtype == torch.int32 and table.shape[0] == B, 'paged_attn: table must be int32 [B, max_pages]')
+    mp = table.shape[1]
+    cap = mp * page
+    _need(cap <= _I32_MAX and B <= 65535, 'paged_attn: sizes beyond 2^31 entries or 65535 sequences')
+    _check_int32('paged_attn: lengths', lengths, (B,))
+    _need(softcap >= 0, 'paged_attn: softcap must not be negative')
+    _need(slopes is None or (slopes.dtype == torch.float32 and tuple(slopes.shape) == (H,) and slopes.is_contiguous()), 'paged_attn: slopes must be dense float32 [H]')
+    for name, t, dt in (('weights', weights, torch.float32), ('key_pos', key_pos, torch.int32)):
+        _need(t is None or (t.dtype == dt and t.dim() == 3 and t.shape[:2] == (B, Hk) and t.shape[2] >= cap and (t.stride(2) == 1 or t.shape[2] <= 1)),
+              'paged_attn: %s must be %s [B, Hk, at least %d], last dimension dense', name, dt, cap)
+    _need(out is None or (out.shape == q.shape and out.dtype == q.dtype and (out.stride(2) == 1 or D == 1)), 'paged_attn: out must be like q')
+    with _OnDevice(q, k_pages, v_pages, table, lengths, slopes, weights, key_pos, out) as s:
+        lib = load()
+        q = _rows(q)
+        table, lengths = _dense_last(table), lengths.contiguous()
+        if out is None:
+            out = torch.empty((B, H, D), dtype=q.dtype, device=q.device)
+        n = _L()
+        _chk(lib.aot_paged_attn_work_floats(B, H, Hk, D, page, mp, int(weights is not None), ctypes.addressof(n)), 'aot_paged_attn_work_floats')
+        work = torch.empty(n.value, dtype=torch.float32, device=q.device) if n.value else None
+        _chk(lib.aot_paged_attn(_ptr(q), _ptr(k_pages), _ptr(v_pages), _ptr(table), _ptr(lengths), _ptr(slopes), _ptr(key_pos), _ptr(weights), _ptr(out),
+                                _ptr(work), n.value, _DTYPE[q.dtype], B, H, Hk, D, page, mp, P, float(D ** -0.5 if scale is None else scale), softcap,
+                                _longs((q, 2), (out, 2), (k_pages, 3), (v_pages, 3), (table, 1), (weights, 2), (key_pos, 2)),
+                                stream if stream is not None else s), 'aot_paged_attn')
+    return out
+
+
+def paged_evict(k_pages, v_pages, table, lengths, weights, new_table, budget, sink=0, recent=0, key_pos=None, stream=None):
+    """Keeps `budget` entries of every cache row -- the first `sink`, the last `recent`, the heaviest by weights [B, Hk, S] -- and copies them into
+    the pages of new_table [B, new_pages] (aot_paged_evict): (kept [B, Hk, budget] old indices or -1, new lengths [B], new weights, new
+    key_pos or None)."""
+    _need(k_pages.dtype in _DTYPE, 'paged_evict: pages must be float32 / float16 / bfloat16')
+    P, page, Hk, D = _check_pages('paged_evict', k_pages, v_pages, k_pages.dtype)
+    _need(table.dim() == 2 and new_table.dim() == 2 and table.dtype == torch.int32 and new_table.dtype == torch.int32 and table.shape[0] == new_table.shape[0],
+          'paged_evict: table and new_table must be int32 [B, pages]')
+    B, mp = table.shape
+    npg = new_table.shape[1]
+    _check_int32('paged_evict: lengths', lengths, (B,))
+    _need(weights.dtype == torch.float32 and weights.dim() == 3 and weights.shape[:2] == (B, Hk) and weights.shape[2] >= mp * page,
+          'paged_evict: weights must be float32 [B, Hk, at least %d]', mp * page)
+    _need(key_pos is None or (key_pos.dtype == torch.int32 and key_pos.shape == weights.shape), 'paged_evict: key_pos must be int32, shaped like weights')
+    budget, sink, recent = int(budget), int(sink), int(recent)
+    _need(budget >= 1 and sink >= 0 and recent >= 0 and sink + recent <= budget, 'paged_evict: sink %d + recent %d must fit the budget %d', sink, recent, budget)
+    _need(npg * page >= budget, 'paged_evict: new_table holds %d entries, the budget is %d', npg * page, budget)
+    _need(mp * page <= _I32_MAX and B <= 65535 and Hk <= 65535, 'paged_evict: sizes beyond 2^31 entries or 65535 rows')
+    S = weights.shape[2]
+    with _OnDevice(k_pages, v_pages, table, lengths, weights, new_table, key_pos) as s:
+        dev = weights.device
+        _need(not (mp and npg) or table.data_ptr() != new_table.data_ptr(), 'paged_evict: new_table must not be table')
+        table, new_table, lengths = _dense_last(table), _dense_last(new_table), lengths.contiguous()
+        weights, key_pos = _dense_last(weights), _dense_last(key_pos)
+        kept = torch.empty((B, Hk, budget), dtype=torch.int32, device=dev)
+        new_lengths = torch.empty(B, dtype=torch.int32, device=dev)
+        new_weights = torch.empty((B, Hk, S), dtype=torch.float32, device=dev)
+        new_pos = torch.empty((B, Hk, S), dtype=torch.int32, device=dev) if key_pos is not None else None
+        if B and Hk:
+            _need(mp > 0, 'paged_evict: table has no pages')
+            _chk(load().aot_paged_evict(_ptr(k_pages), _ptr(v_pages), _ptr(table), _ptr(new_table), _ptr(lengths), _ptr(weights), _ptr(key_pos), _ptr(kept),
+                                        _ptr(new_lengths), _ptr(new_weights), _ptr(new_pos), _DTYPE[k_pages.dtype], B, Hk, D, S, page, mp, npg, P, budget,
+                                        sink, recent, _longs((k_pages, 3), (v_pages, 3), (table, 1), (new_table, 1), (weights, 2), (new_weights, 2),
+                                                             (key_pos, 2), (new_pos, 2)), stream if stream is not None else s), 'aot_paged_evict')
+    return kept, new_lengths, new_weights, new_pos

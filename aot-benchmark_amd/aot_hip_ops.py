@@ -44,6 +44,17 @@ _DEFS = {
     'preprocess': '(Tensor img, Tensor(a!) out, bool flip) -> ()',
     'fuse_probs': '(Tensor logits, int[] flips, Tensor? new_label) -> (Tensor, Tensor)',
     'label_resize': '(Tensor label, int out_h, int out_w, bool flip) -> Tensor',
+    'rope': '(Tensor q, Tensor? k, Tensor pos, Tensor freqs, bool interleaved, float mscale, bool inverse) -> (Tensor, Tensor?)',
+    'rope_append': '(Tensor? q, Tensor k, Tensor v, Tensor pos, Tensor freqs, Tensor slots, Tensor(a!) k_pages, Tensor(b!) v_pages, '
+                   'bool interleaved, float mscale) -> Tensor?',
+    'attn_masked': '(Tensor q, Tensor k, Tensor v, float? scale, bool causal, float softcap, Tensor? slopes, Tensor? doc_q, Tensor? doc_k, '
+                   'Tensor? prefix) -> (Tensor, Tensor)',
+    'attn_masked_bwd': '(Tensor dout, Tensor q, Tensor k, Tensor v, Tensor out, Tensor lse, float? scale, bool causal, float softcap, '
+                       'Tensor? slopes, Tensor? doc_q, Tensor? doc_k, Tensor? prefix) -> (Tensor, Tensor, Tensor)',
+    'paged_attn': '(Tensor q, Tensor k_pages, Tensor v_pages, Tensor table, Tensor lengths, float? scale, float softcap, Tensor? slopes, '
+                  'Tensor(a!)? weights, Tensor? key_pos) -> Tensor',
+    'paged_evict': '(Tensor(a!) k_pages, Tensor(b!) v_pages, Tensor table, Tensor lengths, Tensor weights, Tensor new_table, int budget, '
+                   'int sink, int recent, Tensor? key_pos) -> (Tensor, Tensor, Tensor, Tensor?)',
 }
 for _name, _schema in _DEFS.items():
     _lib.define(_name + _schema)
@@ -142,6 +153,10 @@ def _fuse_probs(logits, flips, new_label):
 @_impl('label_resize')
 def _label_resize(label, out_h, out_w, flip):
     return aot_hip.label_resize(label, out_h, out_w, flip)
+
+
+for _n in ('rope', 'rope_append', 'attn_masked', 'attn_masked_bwd', 'paged_attn', 'paged_evict'):     # (same names, same argument order)
+    _impl(_n)(getattr(aot_hip, _n))
 
 
 def op_names():

@@ -1,0 +1,814 @@
+// Attention under masks, forward and backward, for whole sequences of queries.  For query i of Sq (place i + off in the key sequence,
+// off = Sk - Sq) and key t of Sk:
+//   s = cap tanh(scale q_i.k_t / cap) - slope_h |i + off - t|          (cap = 0: no cap)
+//   seen(i, t): (not causal or t <= i + off or t < prefix_b) and (no documents or doc_q[i] == doc_k[t] >= 0)
+//   p = softmax of s over the seen keys, o = sum p v; a row that sees nothing is zero, with zero gradients.
+// Backward, with D_i = do_i.o_i:  dv_t = sum_i p do_i;  ds = p (do_i.v_t - D_i) (1 - tanh^2);  dq_i = scale sum_t ds k_t;
+// dk_t = scale sum_i ds q_i, both over the query heads that share the key head.
+//
+// Bound by the matrix cores and the exponentials: 4 D operations and one exponential a pair forward, 10 D backward.  Everything is
+// built on 32x32 tiles whose score registers are at once the second operand of the next product:
+//   a wave owns 32 columns (queries; in the key gradient's kernel: keys), one a lane; a score tile's registers run over rows
+//   8 (r / 4) + 4 (lane / 32) + r % 4 of the other side.  With exactly those rows as the reduction index of the following product the
+//   tile needs no exchange between lanes -- the first operand is read in the same order, transposed, from shared memory
+//   (ds_read_b64_tr_b16: four rows of one column a lane; fp32: one element).
+// Four waves share tiles of the other side, staged through registers into two buffers (one barrier a tile); 16-byte pieces are
+// xor-swizzled by their row, so both the row reads and the transposed reads spread over the banks.
+// The gradients of q and of k / v are separate kernels, each the only writer of its rows: no atomics, the result repeats bit for bit,
+// for 7 products instead of 5.  Tiles that no pair of is seen in are never visited: causal bounds, and per 64 tokens the smallest and
+// largest document id (doc_range_kernel), tested 64 tiles at a time by one ballot.
+//
+// Masked places may hold anything.  A masked score is replaced, never multiplied; where a masked row would enter a product with
+// weight zero (0 * inf is NaN), tiles with a mask are staged with infinities and NaN replaced by zero, and if there were any, the
+// seen ones among them are added element by element afterwards.
+//
+// Scores, statistics and sums are 32-bit.  p and ds are rounded to the inputs' type for the following product (nearest even: 2^-9 of
+// the value for bf16, 2^-12 for fp16, below which fp16 also loses what is under 6e-8), the sum that divides is not.
+#include "seq_common.h"
+
+static constexpr int RG = 64;                                  // tokens a document range covers
+
+struct MaskP {
+  const char *q, *k, *v, *o, *d_o;
+  char *out, *dq, *dk, *dv;
+  float *lse, *delta;
+  const float* slopes;
+  const int *doc_q, *doc_k, *prefix;
+  const int4 *rq, *rk;                                         // (smallest id >= 0, largest id, 1 if any is negative, 0) of RG tokens
+  long qs[3], ks[3], vs[3], os[3], dos[3], dqs[3], dks[3], dvs[3], dcs[2];
+  int B, Sq, Sk, H, Hk, G, D, causal, off;
+  float scale, softcap;
+};
+
+__global__ __launch_bounds__(256) void doc_range_kernel(const int* dq, const int* dk, int4* rq, int4* rk, int Sq, int Sk, long qs, long ks) {
+  const int nq = (Sq + RG - 1) / RG, nk = (Sk + RG - 1) / RG;
+  const int w = blockIdx.x * 4 + (threadIdx.x >> 6), lane = threadIdx.x & 63, b = blockIdx.y;
+  if (w >= nq + nk) return;
+  const bool isq = w < nq;
+  const int tile = isq ? w : w - nq, t = tile * RG + lane, n = isq ? Sq : Sk;
+  const int id = t < n ? (isq ? dq[b * qs + t] : dk[b * ks + t]) : -1;
+  int lo = id >= 0 ? id : 0x7fffffff, hi = id, neg = id < 0 && t < n;
+#pragma unroll
+  for (int d = 1; d < 64; d <<= 1) {
+    lo = min(lo, __shfl_xor(lo, d));
+    hi = max(hi, __shfl_xor(hi, d));
+    neg |= __shfl_xor(neg, d);
+  }
+  if (lane == 0) (isq ? rq + (long)b * nq : rk + (long)b * nk)[tile] = make_int4(lo, hi, neg, 0);
+}
+
+template <class T> __device__ __forceinline__ f32x16 mfma32(const u32x4& a, const u32x4& b, f32x16 c) {
+  if constexpr (std::is_same<T, f16>::value) return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
+  else if constexpr (std::is_same<T, bf16>::value) return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+  else {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) c = __builtin_amdgcn_mfma_f32_32x32x2f32(__uint_as_float(a[i]), __uint_as_float(b[i]), c, 0, 0, 0);
+    return c;
+  }
+}
+
+// A tile of R rows x DP columns in shared memory, 16-byte pieces xor-swizzled by row
+template <class T, int DP, int R> struct Tile {
+  static constexpr int CE = Elem<T>::CE, NCH = DP / CE, N = R * NCH / 256, ROWB = DP * (int)sizeof(T), BYTES = R * ROWB;
+  static constexpr int SH = NCH >= 16 ? 0 : NCH == 8 ? 1 : 2, MSK = NCH >= 16 ? 15 : NCH - 1;
+  static __device__ __forceinline__ int swz(int row) { return (row >> SH) & MSK; }
+  struct Regs { u32x4 r[N]; };
+  // rows row0 .. of x (element stride rs), zero past nrow rows and D columns
+  static __device__ __forceinline__ void load(Regs& g, const T* x, long rs, int row0, int nrow, int D) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      const int at = threadIdx.x + 256 * i, row = row0 + at / NCH, d = (at % NCH) * CE;
+      g.r[i] = row < nrow && d < D ? *(const u32x4*)(x + (long)row * rs + d) : u32x4{0, 0, 0, 0};
+    }
+  }
+  static __device__ __forceinline__ bool clean(Regs& g) {        // infinities and NaN to zero; whether there were any
+    bool bad = false;
+#pragma unroll
+    for (int i = 0; i < N; ++i)
+#pragma unroll
+      for (int w = 0; w < 4; ++w) {
+        bad |= word_nonfinite<T>(g.r[i][w]);
+        g.r[i][w] = word_finite<T>(g.r[i][w]);
+      }
+    return bad;
+  }
+  static __device__ __forceinline__ void store(char* lds, const Regs& g) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      const int at = threadIdx.x + 256 * i, row = at / NCH, c = at % NCH;
+      *(u32x4*)(lds + row * ROWB + ((c ^ swz(row)) << 4)) = g.r[i];
+    }
+  }
+  // first operand of a product over the columns: lane = row row0 + (lane & 31), piece 2 c + lane / 32
+  static __device__ __forceinline__ u32x4 rows(const char* lds, int row0, int c) {
+    const int lane = threadIdx.x & 63, row = row0 + (lane & 31);
+    return *(const u32x4*)(lds + row * ROWB + (((2 * c + (lane >> 5)) ^ swz(row)) << 4));
+  }
+  // acc[column 32 db + i][lane's own column] += sum over rows row0 .. row0 + 31 of tile[row][column] * p[row], p in score-tile order
+  static __device__ __forceinline__ f32x16 cols(const char* lds, int row0, int db, const u32x4 (&pk)[2], const f32x16& p, f32x16 acc) {
+    const int lane = threadIdx.x & 63;
+    if constexpr (sizeof(T) == 2) {
+      const int i = lane & 15, c = db * 4 + ((lane >> 4) & 1) * 2 + ((i & 3) >> 1), sub = (i & 1) * 8;
+#pragma unroll
+      for (int kb = 0; kb < 2; ++kb) {
+        u32x4 a;
+#pragma unroll
+        for (int s = 0; s < 2; ++s) {
+          const int row = row0 + 16 * kb + 8 * s + 4 * (lane >> 5) + (i >> 2);
+          typedef short s16x4 __attribute__((ext_vector_type(4)));
+          typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
+          const s16x4 x = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(lds + row * ROWB + ((c ^ swz(row)) << 4) + sub));
+          const u32x2 y = __builtin_bit_cast(u32x2, x);
+          a[2 * s] = y[0];
+          a[2 * s + 1] = y[1];
+        }
+        acc = mfma32<T>(a, pk[kb], acc);
+      }
+    } else {
+      const int d = db * 32 + (lane & 31), c = d / CE, e = d % CE;
+#pragma unroll
+      for (int r = 0; r < 16; ++r) {
+        const int row = row0 + mfma32_row(r, lane >> 5);
+        const float a = *(const float*)(lds + row * ROWB + ((c ^ swz(row)) << 4) + e * 4);
+        acc = __builtin_amdgcn_mfma_f32_32x32x2f32(a, p[r], acc, 0, 0, 0);
+      }
+    }
+    return acc;
+  }
+};
+
+template <class T> __device__ __forceinline__ void pack_tile(const f32x16& p, u32x4 (&pk)[2]) {
+  if constexpr (sizeof(T) == 2) {
+#pragma unroll
+    for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) pk[kb][i] = pack2<T>(p[8 * kb + 2 * i], p[8 * kb + 2 * i + 1]);
+  }
+}
+
+// the lane's own row (or none), in 16-byte pieces 2 c + lane / 32
+template <class T, int NP> __device__ __forceinline__ void own_row(u32x4 (&f)[NP], const T* x, bool ok, int D) {
+  const int h = (threadIdx.x & 63) >> 5;
+#pragma unroll
+  for (int c = 0; c < NP; ++c) {
+    const int d = (2 * c + h) * Elem<T>::CE;
+    f[c] = ok && d < D ? *(const u32x4*)(x + d) : u32x4{0, 0, 0, 0};
+  }
+}
+
+// Tiles of the other side that this workgroup visits: [first, last), of them those whose document range meets [lo, hi]
+template <int PER> struct Tiles {                                // PER tiles a document range
+  const int4* r;
+  int base, last, lo, hi;
+  unsigned long long mask;
+  __device__ __forceinline__ void init(const int4* ranges, int first, int last_, int lo_, int hi_) {
+    r = ranges; base = first; last = last_; lo = lo_; hi = hi_;
+    if (r && hi < 0) last = first;                               // every id of ours is negative: nothing is seen
+    fill();
+  }
+  __device__ __forceinline__ void fill() {
+    const int t = base + (threadIdx.x & 63);
+    bool on = t < last;
+    if (on && r) {
+      const int4 x = r[t / PER];
+      on = x.y >= 0 && x.y >= lo && x.x <= hi;
+    }
+    mask = __ballot(on);
+  }
+  __device__ __forceinline__ int next() {                        // -1: none left
+    while (mask == 0) {
+      base += 64;
+      if (base >= last) return -1;
+      fill();
+    }
+    const int i = __builtin_ctzll(mask);
+    mask &= mask - 1;
+    return base + i;
+  }
+};
+
+__device__ __forceinline__ bool any_flag(const int* f) { return (f[0] | f[1] | f[2] | f[3]) != 0; }
+
+struct Head { int b, h, hk; };
+// consecutive workgroups walk the (sequence, key head) pairs, so those that read the same keys land on the same of the 8 XCDs
+__device__ __forceinline__ Head head_of(int x, const MaskP& p) {
+  const int n = p.B * p.Hk, g = x / n, y = x - g * n;
+  Head r;
+  r.b = y / p.Hk;
+  r.hk = y - r.b * p.Hk;
+  r.h = r.hk * p.G + g;
+  return r;
+}
+
+struct Score {
+  float mul, cap2, slope;
+  bool capped;
+  __device__ __forceinline__ Score(const MaskP& p, int h) {
+    capped = p.softcap > 0.f;
+    mul = capped ? p.scale * 2.f * LOG2E / p.softcap : p.scale * LOG2E;
+    cap2 = p.softcap * LOG2E;
+    slope = p.slopes ? p.slopes[h] * LOG2E : 0.f;
+  }
+};
+
+// ---- forward -------------------------------------------------------------------------------------------------------------------
+template <class T, int DP, int KT>
+__global__ __launch_bounds__(256) void attn_masked_fwd_kernel(MaskP p) {
+  using TL = Tile<T, DP, KT>;
+  constexpr int NP = TL::NCH / 2, ND = DP / 32, NS = KT / 32;
+  __shared__ __align__(16) char smem[4 * TL::BYTES + 2 * KT * 4 + 32];      // K, V of two tiles; ids; flags of the waves
+  auto sk = [&](int buf) { return smem + buf * TL::BYTES; };
+  auto sv = [&](int buf) { return smem + (2 + buf) * TL::BYTES; };
+  int* const sid = (int*)(smem + 4 * TL::BYTES);                // [2][KT]
+  int* const sbad = sid + 2 * KT;                               // [2][4]
+  const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, half = lane >> 5;
+  const Head hd = head_of(blockIdx.x, p);
+  const int q0 = (p.causal ? gridDim.y - 1 - blockIdx.y : blockIdx.y) * 128;      // the long rows of a causal mask first
+  const int i = q0 + wave * 32 + (lane & 31);
+  const bool iok = i < p.Sq;
+  const T* K = (const T*)p.k + hd.b * p.ks[0] + hd.hk * p.ks[2];
+  const T* V = (const T*)p.v + hd.b * p.vs[0] + hd.hk * p.vs[2];
+  u32x4 qf[NP];
+  own_row<T, NP>(qf, (const T*)p.q + hd.b * p.qs[0] + (long)i * p.qs[1] + hd.h * p.qs[2], iok, p.D);
+  const Score sc(p, hd.h);
+  const int prefix = p.prefix ? p.prefix[hd.b] : 0;
+  const int myid = p.doc_q ? (iok ? p.doc_q[hd.b * p.dcs[0] + i] : -1) : 0;
+  const int qlast = min(q0 + 127, p.Sq - 1);
+  const int4 *rk = nullptr;
+  int4 qr = make_int4(0, 0, 0, 0);
+  if (p.doc_q) {
+    const int nq = (p.Sq + RG - 1) / RG;
+    const int4* rq = p.rq + (long)hd.b * nq + q0 / RG;
+    qr = rq[0];
+    if (q0 / RG + 1 < nq) {
+      const int4 x = rq[1];
+      qr = make_int4(min(qr.x, x.x), max(qr.y, x.y), qr.z | x.z, 0);
+    }
+    rk = p.rk + (long)hd.b * ((p.Sk + RG - 1) / RG);
+  }
+  const int tend = p.causal ? min(p.Sk, max(qlast + p.off + 1, prefix)) : p.Sk;
+  Tiles<RG / KT> it;
+  it.init(rk, 0, (max(tend, 0) + KT - 1) / KT, qr.x, qr.y);
+
+  auto whole = [&](int t) {                                      // every pair of the tile is seen
+    const int a = t * KT, z = a + KT - 1;
+    if (z >= p.Sk) return false;
+    if (p.causal && z > q0 + p.off && z >= prefix) return false;
+    if (rk) {
+      const int4 x = rk[a / RG];
+      if (x.x != x.y || x.z || qr.z || qr.x != qr.y || x.x != qr.x) return false;
+    }
+    return true;
+  };
+  auto seen = [&](int t, int id) {
+    return t < p.Sk && (!p.causal || t <= i + p.off || t < prefix) && id == myid && id >= 0;
+  };
+
+  typename TL::Regs gk, gv;
+  int gid = 0;
+  auto fetch = [&](int t) {
+    TL::load(gk, K, p.ks[1], t * KT, p.Sk, p.D);
+    TL::load(gv, V, p.vs[1], t * KT, p.Sk, p.D);
+    if (p.doc_k && threadIdx.x < KT) gid = t * KT + (int)threadIdx.x < p.Sk ? p.doc_k[hd.b * p.dcs[1] + t * KT + threadIdx.x] : -1;
+  };
+  auto put = [&](int buf, bool full) {
+    if (!full) {
+      const bool bad = __any(TL::clean(gv));
+      if (lane == 0) sbad[buf * 4 + wave] = bad;
+    }
+    TL::store(sk(buf), gk);
+    TL::store(sv(buf), gv);
+    if (threadIdx.x < KT) sid[buf * KT + threadIdx.x] = gid;
+  };
+
+  f32x16 o[ND];
+#pragma unroll
+  for (int d = 0; d < ND; ++d)
+#pragma unroll
+    for (int r = 0; r < 16; ++r) o[d][r] = 0.f;
+  float m = NEG_INF, l = 0.f;
+  int t = it.next(), buf = 0;
+  bool full = t >= 0 && whole(t);
+  if (t >= 0) fetch(t);
+  __syncthreads();
+  if (t >= 0) put(0, full);
+  __syncthreads();
+  while (t >= 0) {
+    const int tn = it.next();
+    const bool fulln = tn >= 0 && whole(tn);
+    if (tn >= 0) fetch(tn);
+    f32x16 s[NS];
+#pragma unroll
+    for (int n = 0; n < NS; ++n) {
+#pragma unroll
+      for (int r = 0; r < 16; ++r) s[n][r] = 0.f;
+#pragma unroll
+      for (int c = 0; c < NP; ++c) s[n] = mfma32<T>(TL::rows(sk(buf), n * 32, c), qf[c], s[n]);
+    }
+    float mx = NEG_INF;
+#pragma unroll
+    for (int n = 0; n < NS; ++n)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) {
+        float x = s[n][r] * sc.mul;
+        if (sc.capped) x = sc.cap2 * tanh_from_exp2(x);
+        s[n][r] = x;
+      }
+    if (p.slopes)
+#pragma unroll
+      for (int n = 0; n < NS; ++n)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) s[n][r] -= sc.slope * fabsf((float)(i + p.off - (t * KT + n * 32 + mfma32_row(r, half))));
+    if (!full)
+#pragma unroll
+      for (int n = 0; n < NS; ++n)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+          const int j = n * 32 + mfma32_row(r, half);
+          if (!seen(t * KT + j, sid[buf * KT + j])) s[n][r] = NEG_INF;
+        }
+#pragma unroll
+    for (int n = 0; n < NS; ++n)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) mx = fmaxf(mx, s[n][r]);
+    mx = fmaxf(mx, __shfl_xor(mx, 32));
+    const float m2 = fmaxf(m, mx), base = m2 == NEG_INF ? 0.f : m2;
+    const float f = exp2_hw(m - base);
+    m = m2;
+    l *= f;
+    if (__any(f != 1.f))
+#pragma unroll
+      for (int d = 0; d < ND; ++d) o[d] *= f;
+#pragma unroll
+    for (int n = 0; n < NS; ++n) {
+#pragma unroll
+      for (int r = 0; r < 16; ++r) { s[n][r] = exp2_hw(s[n][r] - base); l += s[n][r]; }
+      u32x4 pk[2];
+      pack_tile<T>(s[n], pk);
+#pragma unroll
+      for (int d = 0; d < ND; ++d) o[d] = TL::cols(sv(buf), n * 32, d, pk, s[n], o[d]);
+    }
+    if (!full && any_flag(sbad + buf * 4)) {                                    // the seen infinities and NaN that staging left out
+      for (int j = 0; j < KT; ++j) {
+        if (!seen(t * KT + j, sid[buf * KT + j])) continue;
+        const T* row = V + (long)(t * KT + j) * p.vs[1];
+#pragma unroll
+        for (int d = 0; d < ND; ++d)
+#pragma unroll
+          for (int r = 0; r < 16; ++r) {
+            const int e = d * 32 + mfma32_row(r, half);
+            if (e < p.D) {
+              const float x = (float)row[e];
+              if (!(fabsf(x) < __builtin_inff())) o[d][r] += x;
+            }
+          }
+      }
+    }
+    if (tn >= 0) put(buf ^ 1, fulln);
+    __syncthreads();
+    buf ^= 1;
+    t = tn;
+    full = fulln;
+  }
+  l += __shfl_xor(l, 32);
+  if (!iok) return;
+  const float inv = l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l);
+  T* out = (T*)p.out + hd.b * p.os[0] + (long)i * p.os[1] + hd.h * p.os[2];
+#pragma unroll
+  for (int d = 0; d < ND; ++d)
+#pragma unroll
+    for (int r = 0; r < 16; ++r) {
+      const int e = d * 32 + mfma32_row(r, half);
+      if (e < p.D) out[e] = (T)(o[d][r] * inv);
+    }
+  if (half == 0) p.lse[((long)hd.b * p.H + hd.h) * p.Sq + i] = l == 0.f ? NEG_INF : m + log2f(l);
+}
+
+// ---- gradient of the queries -----------------------------------------------------------------------------------------------------
+template <class T, int DP, int KT>
+__global__ __launch_bounds__(256) void attn_masked_dq_kernel(MaskP p) {
+  using TL = Tile<T, DP, KT>;
+  constexpr int NP = TL::NCH / 2, ND = DP / 32, NS = KT / 32;
+  __shared__ __align__(16) char smem[4 * TL::BYTES + 2 * KT * 4 + 32];
+  auto sk = [&](int buf) { return smem + buf * TL::BYTES; };
+  auto sv = [&](int buf) { return smem + (2 + buf) * TL::BYTES; };
+  int* const sid = (int*)(smem + 4 * TL::BYTES);
+  int* const sbad = sid + 2 * KT;
+  const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, half = lane >> 5;
+  const Head hd = head_of(blockIdx.x, p);
+  const int q0 = (p.causal ? gridDim.y - 1 - blockIdx.y : blockIdx.y) * 128;
+  const int i = q0 + wave * 32 + (lane & 31);
+  const bool iok = i < p.Sq;
+  const T* K = (const T*)p.k + hd.b * p.ks[0] + hd.hk * p.ks[2];
+  const T* V = (const T*)p.v + hd.b * p.vs[0] + hd.hk * p.vs[2];
+  u32x4 qf[NP], df[NP];
+  own_row<T, NP>(qf, (const T*)p.q + hd.b * p.qs[0] + (long)i * p.qs[1] + hd.h * p.qs[2], iok, p.D);
+  own_row<T, NP>(df, (const T*)p.d_o + hd.b * p.dos[0] + (long)i * p.dos[1] + hd.h * p.dos[2], iok, p.D);
+  const long at = ((long)hd.b * p.H + hd.h) * p.Sq + i;
+  float delta = 0.f;
+  {
+    u32x4 of[NP];
+    own_row<T, NP>(of, (const T*)p.o + hd.b * p.os[0] + (long)i * p.os[1] + hd.h * p.os[2], iok, p.D);
+#pragma unroll
+    for (int c = 0; c < NP; ++c)
+#pragma unroll
+      for (int w = 0; w < 4; ++w) {
+        if constexpr (sizeof(T) == 4) delta += __uint_as_float(of[c][w]) * __uint_as_float(df[c][w]);
+        else {
+          delta += half_to_float<T>((u16)of[c][w]) * half_to_float<T>((u16)df[c][w]);
+          delta += half_to_float<T>((u16)(of[c][w] >> 16)) * half_to_float<T>((u16)(df[c][w] >> 16));
+        }
+      }
+    delta += __shfl_xor(delta, 32);
+  }
+  float lse = iok ? p.lse[at] : __builtin_inff();
+  if (lse == NEG_INF) { lse = __builtin_inff(); delta = 0.f; }   // sees nothing: every probability is zero
+  if (iok && half == 0) p.delta[at] = delta;
+  const Score sc(p, hd.h);
+  const int prefix = p.prefix ? p.prefix[hd.b] : 0;
+  const int myid = p.doc_q ? (iok ? p.doc_q[hd.b * p.dcs[0] + i] : -1) : 0;
+  const int qlast = min(q0 + 127, p.Sq - 1);
+  const int4 *rk = nullptr;
+  int4 qr = make_int4(0, 0, 0, 0);
+  if (p.doc_q) {
+    const int nq = (p.Sq + RG - 1) / RG;
+    const int4* rq = p.rq + (long)hd.b * nq + q0 / RG;
+    qr = rq[0];
+    if (q0 / RG + 1 < nq) {
+      const int4 x = rq[1];
+      qr = make_int4(min(qr.x, x.x), max(qr.y, x.y), qr.z | x.z, 0);
+    }
+    rk = p.rk + (long)hd.b * ((p.Sk + RG - 1) / RG);
+  }
+  const int tend = p.causal ? min(p.Sk, max(qlast + p.off + 1, prefix)) : p.Sk;
+  Tiles<RG / KT> it;
+  it.init(rk, 0, (max(tend, 0) + KT - 1) / KT, qr.x, qr.y);
+  auto whole = [&](int t) {
+    const int a = t * KT, z = a + KT - 1;
+    if (z >= p.Sk) return false;
+    if (p.causal && z > q0 + p.off && z >= prefix) return false;
+    if (rk) {
+      const int4 x = rk[a / RG];
+      if (x.x != x.y || x.z || qr.z || qr.x != qr.y || x.x != qr.x) return false;
+    }
+    return true;
+  };
+  auto seen = [&](int t, int id) {
+    return t < p.Sk && (!p.causal || t <= i + p.off || t < prefix) && id == myid && id >= 0;
+  };
+  typename TL::Regs gk, gv;
+  int gid = 0;
+  auto fetch = [&](int t) {
+    TL::load(gk, K, p.ks[1], t * KT, p.Sk, p.D);
+    TL::load(gv, V, p.vs[1], t * KT, p.Sk, p.D);
+    if (p.doc_k && threadIdx.x < KT) gid = t * KT + (int)threadIdx.x < p.Sk ? p.doc_k[hd.b * p.dcs[1] + t * KT + threadIdx.x] : -1;
+  };
+  auto put = [&](int buf, bool full) {
+    if (!full) {
+      const bool bad = __any(TL::clean(gk));
+      if (lane == 0) sbad[buf * 4 + wave] = bad;
+    }
+    TL::store(sk(buf), gk);
+    TL::store(sv(buf), gv);
+    if (threadIdx.x < KT) sid[buf * KT + threadIdx.x] = gid;
+  };
+  f32x16 dq[ND];
+#pragma unroll
+  for (int d = 0; d < ND; ++d)
+#pragma unroll
+    for (int r = 0; r < 16; ++r) dq[d][r] = 0.f;
+  int t = it.next(), buf = 0;
+  bool full = t >= 0 && whole(t);
+  if (t >= 0) fetch(t);
+  __syncthreads();
+  if (t >= 0) put(0, full);
+  __syncthreads();
+  while (t >= 0) {
+    const int tn = it.next();
+    const bool fulln = tn >= 0 && whole(tn);
+    if (tn >= 0) fetch(tn);
+#pragma unroll
+    for (int n = 0; n < NS; ++n) {
+      f32x16 s, dp;
+#pragma unroll
+      for (int r = 0; r < 16; ++r) { s[r] = 0.f; dp[r] = 0.f; }
+#pragma unroll
+      for (int c = 0; c < NP; ++c) s = mfma32<T>(TL::rows(sk(buf), n * 32, c), qf[c], s);
+#pragma unroll
+      for (int c = 0; c < NP; ++c) dp = mfma32<T>(TL::rows(sv(buf), n * 32, c), df[c], dp);
+#pragma unroll
+      for (int r = 0; r < 16; ++r) {
+        const int j = n * 32 + mfma32_row(r, half);
+        float x = s[r] * sc.mul, g = dp[r] - delta;
+        if (sc.capped) {
+          const float th = tanh_from_exp2(x);
+          x = sc.cap2 * th;
+          g *= 1.f - th * th;
+        }
+        if (p.slopes) x -= sc.slope * fabsf((float)(i + p.off - (t * KT + j)));
+        g *= exp2_hw(x - lse);
+        if (!full && !seen(t * KT + j, sid[buf * KT + j])) g = 0.f;
+        s[r] = g;
+      }
+      u32x4 pk[2];
+      pack_tile<T>(s, pk);
+#pragma unroll
+      for (int d = 0; d < ND; ++d) dq[d] = TL::cols(sk(buf), n * 32, d, pk, s, dq[d]);
+    }
+    if (!full && any_flag(sbad + buf * 4)) {
+      for (int j = 0; j < KT; ++j) {
+        if (!seen(t * KT + j, sid[buf * KT + j])) continue;
+        const T* row = K + (long)(t * KT + j) * p.ks[1];
+#pragma unroll
+        for (int d = 0; d < ND; ++d)
+#pragma unroll
+          for (int r = 0; r < 16; ++r) {
+            const int e = d * 32 + mfma32_row(r, half);
+            if (e < p.D) {
+              const float x = (float)row[e];
+              if (!(fabsf(x) < __builtin_inff())) dq[d][r] += x;
+            }
+          }
+      }
+    }
+    if (tn >= 0) put(buf ^ 1, fulln);
+    __syncthreads();
+    buf ^= 1;
+    t = tn;
+    full = fulln;
+  }
+  if (!iok) return;
+  T* out = (T*)p.dq + hd.b * p.dqs[0] + (long)i * p.dqs[1] + hd.h * p.dqs[2];
+#pragma unroll
+  for (int d = 0; d < ND; ++d)
+#pragma unroll
+    for (int r = 0; r < 16; ++r) {
+      const int e = d * 32 + mfma32_row(r, half);
+      if (e < p.D) out[e] = (T)(dq[d][r] * p.scale);
+    }
+}
+
+// ---- gradients of the keys and values ----------------------------------------------------------------------------------------------
+template <class T, int DP, int QT>
+__global__ __launch_bounds__(256) void attn_masked_dkv_kernel(MaskP p) {
+  using TL = Tile<T, DP, QT>;
+  constexpr int NP = TL::NCH / 2, ND = DP / 32, NS = QT / 32;
+  __shared__ __align__(16) char smem[4 * TL::BYTES + 6 * QT * 4 + 32];      // Q, dO of two tiles; lse, delta, ids; flags of the waves
+  auto sq = [&](int buf) { return smem + buf * TL::BYTES; };
+  auto sd = [&](int buf) { return smem + (2 + buf) * TL::BYTES; };
+  float* const slse = (float*)(smem + 4 * TL::BYTES);           // [2][QT]
+  float* const sdel = slse + 2 * QT;
+  int* const sid = (int*)(sdel + 2 * QT);
+  int* const sbad = sid + 2 * QT;
+  const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, half = lane >> 5;
+  const int b = blockIdx.x / p.Hk, hk = blockIdx.x - b * p.Hk;
+  const int k0 = blockIdx.y * 128;                               // (causal: the first keys are seen by most queries)
+  const int t = k0 + wave * 32 + (lane & 31);
+  const bool tok = t < p.Sk;
+  u32x4 kf[NP], vf[NP];
+  own_row<T, NP>(kf, (const T*)p.k + b * p.ks[0] + (long)t * p.ks[1] + hk * p.ks[2], tok, p.D);
+  own_row<T, NP>(vf, (const T*)p.v + b * p.vs[0] + (long)t * p.vs[1] + hk * p.vs[2], tok, p.D);
+  const int prefix = p.prefix ? p.prefix[b] : 0;
+  const int myid = p.doc_k ? (tok ? p.doc_k[b * p.dcs[1] + t] : -1) : 0;
+  const int klast = min(k0 + 127, p.Sk - 1);
+  const int4 *rq = nullptr;
+  int4 kr = make_int4(0, 0, 0, 0);
+  if (p.doc_q) {
+    const int nk = (p.Sk + RG - 1) / RG;
+    const int4* rk = p.rk + (long)b * nk + k0 / RG;
+    kr = rk[0];
+    if (k0 / RG + 1 < nk) {
+      const int4 x = rk[1];
+      kr = make_int4(min(kr.x, x.x), max(kr.y, x.y), kr.z | x.z, 0);
+    }
+    rq = p.rq + (long)b * ((p.Sq + RG - 1) / RG);
+  }
+  const int first = p.causal && k0 >= prefix ? max(0, k0 - p.off) / QT : 0;
+  auto whole = [&](int tq) {                                     // every pair of the tile is seen (rows past Sq have probability zero)
+    const int a = tq * QT;
+    if (p.causal && klast > a + p.off && klast >= prefix) return false;
+    if (rq) {
+      const int4 x = rq[a / RG];
+      if (x.x != x.y || x.z || kr.z || kr.x != kr.y || x.x != kr.x) return false;
+    }
+    return true;
+  };
+  auto seen = [&](int i, int id) {
+    return i < p.Sq && (!p.causal || t <= i + p.off || t < prefix) && id == myid && id >= 0;
+  };
+  f32x16 dk[ND], dv[ND];
+#pragma unroll
+  for (int d = 0; d < ND; ++d)
+#pragma unroll
+    for (int r = 0; r < 16; ++r) { dk[d][r] = 0.f; dv[d][r] = 0.f; }
+  typename TL::Regs gq, gd;
+  float glse = 0.f, gdel = 0.f;
+  int gid = 0;
+  for (int g = 0; g < p.G; ++g) {
+    const int h = hk * p.G + g;
+    const T* Q = (const T*)p.q + b * p.qs[0] + h * p.qs[2];
+    const T* DO = (const T*)p.d_o + b * p.dos[0] + h * p.dos[2];
+    const float* lse = p.lse + ((long)b * p.H + h) * p.Sq;
+    const float* del = p.delta + ((long)b * p.H + h) * p.Sq;
+    const Score sc(p, h);
+    Tiles<RG / QT> it;
+    it.init(rq, first, (p.Sq + QT - 1) / QT, kr.x, kr.y);
+    auto fetch = [&](int tq) {
+      TL::load(gq, Q, p.qs[1], tq * QT, p.Sq, p.D);
+      TL::load(gd, DO, p.dos[1], tq * QT, p.Sq, p.D);
+      if (threadIdx.x < QT) {
+        const int i = tq * QT + threadIdx.x;
+        glse = i < p.Sq ? lse[i] : __builtin_inff();
+        if (glse == NEG_INF) glse = __builtin_inff();
+        gdel = i < p.Sq ? del[i] : 0.f;
+        gid = p.doc_q ? (i < p.Sq ? p.doc_q[b * p.dcs[0] + i] : -1) : 0;
+      }
+    };
+    auto put = [&](int buf, bool full) {
+      if (!full) {
+        const bool x = TL::clean(gq), y = TL::clean(gd), bad = __any(x || y);
+        if (lane == 0) sbad[buf * 4 + wave] = bad;
+      }
+      TL::store(sq(buf), gq);
+      TL::store(sd(buf), gd);
+      if (threadIdx.x < QT) {
+        slse[buf * QT + threadIdx.x] = glse;
+        sdel[buf * QT + threadIdx.x] = gdel;
+        sid[buf * QT + threadIdx.x] = gid;
+      }
+    };
+    __syncthreads();
+    int tq = it.next(), buf = 0;
+    bool full = tq >= 0 && whole(tq);
+    if (tq >= 0) fetch(tq);
+    __syncthreads();
+    if (tq >= 0) put(0, full);
+    __syncthreads();
+    while (tq >= 0) {
+      const int tn = it.next();
+      const bool fulln = tn >= 0 && whole(tn);
+      if (tn >= 0) fetch(tn);
+#pragma unroll
+      for (int n = 0; n < NS; ++n) {
+        f32x16 s, dp;
+#pragma unroll
+        for (int r = 0; r < 16; ++r) { s[r] = 0.f; dp[r] = 0.f; }
+#pragma unroll
+        for (int c = 0; c < NP; ++c) s = mfma32<T>(TL::rows(sq(buf), n * 32, c), kf[c], s);
+#pragma unroll
+        for (int c = 0; c < NP; ++c) dp = mfma32<T>(TL::rows(sd(buf), n * 32, c), vf[c], dp);
+#pragma unroll
+        for (int r4 = 0; r4 < 4; ++r4) {
+          const int j0 = n * 32 + 8 * r4 + 4 * half;
+          const f32x4 ls = *(const f32x4*)(slse + buf * QT + j0), de = *(const f32x4*)(sdel + buf * QT + j0);
+          const i32x4 id = *(const i32x4*)(sid + buf * QT + j0);
+#pragma unroll
+          for (int w = 0; w < 4; ++w) {
+            const int r = 4 * r4 + w, i = tq * QT + j0 + w;
+            float x = s[r] * sc.mul, gg = dp[r] - de[w];
+            if (sc.capped) {
+              const float th = tanh_from_exp2(x);
+              x = sc.cap2 * th;
+              gg *= 1.f - th * th;
+            }
+            if (p.slopes) x -= sc.slope * fabsf((float)(i + p.off - t));
+            float pr = exp2_hw(x - ls[w]);
+            gg *= pr;
+            if (!full && !seen(i, id[w])) { pr = 0.f; gg = 0.f; }
+            s[r] = pr;
+            dp[r] = gg;
+          }
+        }
+        u32x4 pk[2];
+        pack_tile<T>(s, pk);
+#pragma unroll
+        for (int d = 0; d < ND; ++d) dv[d] = TL::cols(sd(buf), n * 32, d, pk, s, dv[d]);
+        pack_tile<T>(dp, pk);
+#pragma unroll
+        for (int d = 0; d < ND; ++d) dk[d] = TL::cols(sq(buf), n * 32, d, pk, dp, dk[d]);
+      }
+      if (!full && any_flag(sbad + buf * 4)) {
+        for (int j = 0; j < QT; ++j) {
+          const int i = tq * QT + j;
+          if (!seen(i, sid[buf * QT + j])) continue;
+          const T *r1 = DO + (long)i * p.dos[1], *r2 = Q + (long)i * p.qs[1];
+#pragma unroll
+          for (int d = 0; d < ND; ++d)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) {
+              const int e = d * 32 + mfma32_row(r, half);
+              if (e < p.D) {
+                const float x = (float)r1[e], y = (float)r2[e];
+                if (!(fabsf(x) < __builtin_inff())) dv[d][r] += x;
+                if (!(fabsf(y) < __builtin_inff())) dk[d][r] += y;
+              }
+            }
+        }
+      }
+      if (tn >= 0) put(buf ^ 1, fulln);
+      __syncthreads();
+      buf ^= 1;
+      tq = tn;
+      full = fulln;
+    }
+  }
+  if (!tok) return;
+  T* ok = (T*)p.dk + b * p.dks[0] + (long)t * p.dks[1] + hk * p.dks[2];
+  T* ov = (T*)p.dv + b * p.dvs[0] + (long)t * p.dvs[1] + hk * p.dvs[2];
+#pragma unroll
+  for (int d = 0; d < ND; ++d)
+#pragma unroll
+    for (int r = 0; r < 16; ++r) {
+      const int e = d * 32 + mfma32_row(r, half);
+      if (e < p.D) {
+        ok[e] = (T)(dk[d][r] * p.scale);
+        ov[e] = (T)dv[d][r];
+      }
+    }
+}
+
+// ---- C entries -----------------------------------------------------------------------------------------------------------------------
+static int mask_args(int dtype, int B, int Sq, int Sk, int H, int Hk, int D, float softcap, const int* doc_q, const int* doc_k, const void* ranges,
+                     const long* strides) {
+  const int es = dtype_size(dtype);
+  if (!es || B < 0 || Sq < 0 || Sk < 0 || Hk < 1 || H < Hk || H % Hk || D < 1 || !strides || !(softcap >= 0.f)) return AOT_ERR_BADARG;
+  if ((doc_q == nullptr) != (doc_k == nullptr) || (doc_q && !ranges)) return AOT_ERR_BADARG;
+  if (D > 128 || D * es % 16 || Sq > (1 << 22) || Sk > (1 << 22) || (long)B * H > 0x7fffffffL || B > 65535) return AOT_ERR_UNSUPPORTED;
+  return AOT_OK;
+}
+static bool rows_aligned(const void* x, const long* st, int es) {
+  for (int i = 0; i < 3; ++i) if (st[i] * es % 16) return false;
+  return aligned16(x);
+}
+static void mask_common(MaskP& p, int B, int Sq, int Sk, int H, int Hk, int D, int causal, float scale, float softcap, const float* slopes,
+                        const int* doc_q, const int* doc_k, const int* prefix, void* ranges) {
+  p.B = B; p.Sq = Sq; p.Sk = Sk; p.H = H; p.Hk = Hk; p.G = H / Hk; p.D = D; p.causal = causal != 0; p.off = Sk - Sq;
+  p.scale = scale; p.softcap = softcap; p.slopes = slopes; p.doc_q = doc_q; p.doc_k = doc_k; p.prefix = causal ? prefix : nullptr;
+  p.rq = (const int4*)ranges;
+  p.rk = p.rq + (long)B * ((Sq + RG - 1) / RG);
+}
+static void range_launch(const MaskP& p, hipStream_t st) {
+  const int n = (p.Sq + RG - 1) / RG + (p.Sk + RG - 1) / RG;
+  hipLaunchKernelGGL(doc_range_kernel, dim3((n + 3) / 4, p.B), dim3(256), 0, st, p.doc_q, p.doc_k, (int4*)p.rq, (int4*)p.rk, p.Sq, p.Sk, p.dcs[0], p.dcs[1]);
+}
+// f(element type, padded head width, rows of a shared-memory tile): 64 rows a tile where four of them fit 64 KB, else 32
+template <class F> static void with_tile(int dtype, int D, F&& f) {
+  with_dtype(dtype, [&](auto t) {
+    using T = decltype(t);
+    if (D <= 32) f(t, std::integral_constant<int, 32>{}, std::integral_constant<int, 64>{});
+    else if (D <= 64) f(t, std::integral_constant<int, 64>{}, std::integral_constant<int, 64>{});
+    else f(t, std::integral_constant<int, 128>{}, std::integral_constant<int, sizeof(T) == 4 ? 32 : 64>{});
+  });
+}
+
+extern "C" int aot_attn_masked(const void* q, const void* k, const void* v, void* out, float* lse, const float* slopes, const int* doc_q,
+                               const int* doc_k, const int* prefix, void* ranges, int dtype, int B, int Sq, int Sk, int H, int Hk, int D,
+                               int causal, float scale, float softcap, const long* strides, void* stream) {
+  int rc = mask_args(dtype, B, Sq, Sk, H, Hk, D, softcap, doc_q, doc_k, ranges, strides);
+  if (rc) return rc;
+  if (B == 0 || Sq == 0) return AOT_OK;
+  if (!q || !out || !lse || (Sk && (!k || !v))) return AOT_ERR_BADARG;
+  MaskP p{};
+  p.q = (const char*)q; p.k = (const char*)k; p.v = (const char*)v; p.out = (char*)out; p.lse = lse;
+  for (int i = 0; i < 3; ++i) { p.qs[i] = strides[i]; p.ks[i] = strides[3 + i]; p.vs[i] = strides[6 + i]; p.os[i] = strides[9 + i]; }
+  p.dcs[0] = strides[12]; p.dcs[1] = strides[13];
+  const int es = dtype_size(dtype);
+  if (!rows_aligned(q, p.qs, es) || !rows_aligned(k, p.ks, es) || !rows_aligned(v, p.vs, es)) return AOT_ERR_BADARG;
+  mask_common(p, B, Sq, Sk, H, Hk, D, causal, scale, softcap, slopes, doc_q, doc_k, prefix, ranges);
+  hipStream_t st = (hipStream_t)stream;
+  if (doc_q) range_launch(p, st);
+  const dim3 grid(B * H, cdiv(Sq, 128));
+  with_tile(dtype, D, [&](auto t, auto dp, auto kt) {
+    hipLaunchKernelGGL((attn_masked_fwd_kernel<decltype(t), decltype(dp)::value, decltype(kt)::value>), grid, dim3(256), 0, st, p);
+  });
+  AOT_LAUNCH_CHECK();
+}
+
+extern "C" int aot_attn_masked_bwd(const void* q, const void* k, const void* v, const void* out, const float* lse, const void* dout, void* dq, void* dk,
+                                   void* dv, const float* slopes, const int* doc_q, const int* doc_k, const int* prefix, void* ranges, float* delta,
+                                   int dtype, int B, int Sq, int Sk, int H, int Hk, int D, int causal, float scale, float softcap, const long* strides,
+                                   void* stream) {
+  int rc = mask_args(dtype, B, Sq, Sk, H, Hk, D, softcap, doc_q, doc_k, ranges, strides);
+  if (rc) return rc;
+  if (B == 0 || (Sq == 0 && Sk == 0)) return AOT_OK;
+  if ((Sq && (!q || !out || !lse || !dout || !dq || !delta)) || (Sk && (!k || !v || !dk || !dv))) return AOT_ERR_BADARG;
+  MaskP p{};
+  p.q = (const char*)q; p.k = (const char*)k; p.v = (const char*)v; p.o = (const char*)out; p.d_o = (const char*)dout;
+  p.lse = (float*)lse; p.delta = delta; p.dq = (char*)dq; p.dk = (char*)dk; p.dv = (char*)dv;
+  for (int i = 0; i < 3; ++i) {
+    p.qs[i] = strides[i]; p.ks[i] = strides[3 + i]; p.vs[i] = strides[6 + i]; p.os[i] = strides[9 + i]; p.dos[i] = strides[12 + i];
+    p.dqs[i] = strides[15 + i]; p.dks[i] = strides[18 + i]; p.dvs[i] = strides[21 + i];
+  }
+  p.dcs[0] = strides[24]; p.dcs[1] = strides[25];
+  const int es = dtype_size(dtype);
+  if (!rows_aligned(q, p.qs, es) || !rows_aligned(k, p.ks, es) || !rows_aligned(v, p.vs, es) || !rows_aligned(out, p.os, es) ||
+      !rows_aligned(dout, p.dos, es)) return AOT_ERR_BADARG;
+  mask_common(p, B, Sq, Sk, H, Hk, D, causal, scale, softcap, slopes, doc_q, doc_k, prefix, ranges);
+  hipStream_t st = (hipStream_t)stream;
+  if (doc_q) range_launch(p, st);
+  with_tile(dtype, D, [&](auto t, auto dp, auto kt) {
+    if (Sq) hipLaunchKernelGGL((attn_masked_dq_kernel<decltype(t), decltype(dp)::value, decltype(kt)::value>), dim3(B * H, cdiv(Sq, 128)), dim3(256), 0, st, p);
+    if (Sk) hipLaunchKernelGGL((attn_masked_dkv_kernel<decltype(t), decltype(dp)::value, decltype(kt)::value>), dim3(B * Hk, cdiv(Sk, 128)), dim3(256), 0, st, p);
+  });
+  AOT_LAUNCH_CHECK();
+}

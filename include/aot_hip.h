@@ -511,6 +511,77 @@ int aot_bilinear_bwd_nhwc_f32(const float* dy, float* dx, int B, int IH, int IW,
 int aot_window_gather_f32(const float* dense, float* win, int G, int h, int w, int max_dis, float fill, void* stream);
 int aot_window_scatter_f32(const float* win, float* dense, int G, int h, int w, int max_dis, float fill, void* stream);
 
+/* ---- token sequences: 16-bit and 32-bit element types, paged caches -----------------------------------------------------------
+ * These entries take strided tensors of one element type (`dtype`: AOT_F32 / AOT_F16 / AOT_BF16; queries, keys, values, outputs and
+ * pages alike).  `strides` is a HOST array of longs read during the call: element strides, in the order each entry names; the last
+ * (head) dimension has stride 1.  H query heads share Hk key heads, H % Hk == 0: query head h reads key head h / (H / Hk).  Sums,
+ * softmax statistics, scores and collected weights are 32-bit whatever the type.  None of these calls keeps anything between calls. */
+#define AOT_F32 0
+#define AOT_F16 1
+#define AOT_BF16 2
+
+/* Rotary positions: qo / ko = q / k [B, S, H | Hk, D] with the first `rot` (even, <= D <= 1024) elements of every head turned in pairs by
+ * pos[b, s] * freqs[j], j < rot / 2 (radians, 64-bit: exact for positions of millions), times mscale; interleaved: pairs (2j, 2j + 1),
+ * else (j, j + rot / 2); the rest of the head is copied.  inverse: the negated angle -- with the same mscale the gradient of the forward
+ * turn.  H or Hk may be 0 (its pointers NULL); qo == q / ko == k (same strides) turns in place.  Any strides and alignment for
+ * half-split pairs; interleaved ones need D even, pairs aligned to their size and even strides.
+ * strides: q b s h, k b s h, qo b s h, ko b s h, pos b s (14).  Beside the sine positions of networks/layers/position.py:33-74. */
+int aot_rope(const void* q, const void* k, void* qo, void* ko, const int* pos, const double* freqs, int dtype, int B, int S,
+             int H, int Hk, int D, int rot, int interleaved, int inverse, float mscale, const long* strides, void* stream);
+/* The same turn for N new tokens q [N, H, D], k [N, Hk, D] at pos [N], the turned keys and the values v [N, Hk, D] written to the cache
+ * slots slots[n] = page_id * page + place of k_pages / v_pages (num_pages pages of `page` places, a power of two).  A negative slot, or one
+ * outside the pool, writes nothing (padded tokens); two tokens with one slot leave either.  H = 0: keys and values only.
+ * strides: q n h, k n h, v n h, qo n h, k_pages page place h, v_pages page place h (14). */
+int aot_rope_append(const void* q, const void* k, const void* v, void* qo, void* k_pages, void* v_pages, const int* pos,
+                    const int* slots, const double* freqs, int dtype, int N, int H, int Hk, int D, int rot, int interleaved,
+                    float mscale, int page, long num_pages, const long* strides, void* stream);
+
+/* Attention under masks, q [B, Sq, H, D], k / v [B, Sk, Hk, D] -> out [B, Sq, H, D] and lse [B, H, Sq] (log2 of the sum of exponentials;
+ * -inf for a row that sees nothing, whose output is zero).  Query i stands at place i + Sk - Sq of the key sequence.
+ *   s = softcap tanh(scale q.k / softcap) - slopes[h] |i + Sk - Sq - t|      (softcap = 0: no cap; slopes [H] or NULL)
+ * Key t is seen if (not causal, or t <= i + Sk - Sq, or t < prefix[b]) and (no documents, or doc_q[b, i] == doc_k[b, t] >= 0).  A negative
+ * document id marks padding.  What masked places hold (NaN, infinities) does not reach the result.  prefix [B] or NULL (read with causal
+ * only); doc_q [B, Sq] / doc_k [B, Sk] both or neither, then `ranges` is scratch of 16 * B * (ceil(Sq / 64) + ceil(Sk / 64)) bytes, 16-byte
+ * aligned.  D <= 128, rows of whole 16-byte pieces, 16-byte aligned.  Sq, Sk <= 2^22.
+ * strides: q b s h, k b s h, v b s h, out b s h, doc_q b, doc_k b (14).  Beside aot_attn_f32 (attention.py:82-117). */
+int aot_attn_masked(const void* q, const void* k, const void* v, void* out, float* lse, const float* slopes, const int* doc_q,
+                    const int* doc_k, const int* prefix, void* ranges, int dtype, int B, int Sq, int Sk, int H, int Hk, int D,
+                    int causal, float scale, float softcap, const long* strides, void* stream);
+/* Its gradients: out and lse from the forward call on the same arguments, dout -> dq, dk, dv (key heads: summed over the query heads
+ * that share them); delta: scratch of B * H * Sq floats.  Probabilities and score gradients are rounded to `dtype` for the products they
+ * enter (fp16: what is below 6e-8 is lost, as in any fp16 gradient -- scale the loss).  No atomics: results repeat bit for bit.
+ * strides: q k v out dout dq dk dv (b s h each), doc_q b, doc_k b (26). */
+int aot_attn_masked_bwd(const void* q, const void* k, const void* v, const void* out, const float* lse, const void* dout, void* dq, void* dk,
+                        void* dv, const float* slopes, const int* doc_q, const int* doc_k, const int* prefix, void* ranges, float* delta,
+                        int dtype, int B, int Sq, int Sk, int H, int Hk, int D, int causal, float scale, float softcap, const long* strides,
+                        void* stream);
+
+/* Attention of ONE new token per sequence over a paged cache: q / out [B, H, D]; entry t < lengths[b] of sequence b lies at place t % page
+ * of page table[b, t / page] (max_pages a row) of k_pages / v_pages.  The new token's own key and value are already in the cache (entry
+ * lengths[b] - 1).  Scores as in aot_attn_masked, the distance being key_pos[b, hk, len - 1] - key_pos[b, hk, t] where key_pos is given
+ * (a cache that entries were evicted from), else len - 1 - t.  weights (optional): weights[b, hk, t] += the sum of the group's
+ * probabilities, one writer per entry.  lengths are read on the device: 0 gives a zero row, more than max_pages * page counts as
+ * that.  A page id outside the pool hides its entries.  Places past the length are not read.  D <= 256, rows of whole 16-byte pieces,
+ * 16-byte aligned.  work: scratch of aot_paged_attn_work_floats floats (0: may be NULL); two calls in flight at once need two.
+ * strides: q b h, out b h, k_pages page place h, v_pages page place h, table b, weights b h, key_pos b h (15). */
+int aot_paged_attn(const void* q, const void* k_pages, const void* v_pages, const int* table, const int* lengths, const float* slopes,
+                   const int* key_pos, float* weights, void* out, float* work, long work_floats, int dtype, int B, int H, int Hk,
+                   int D, int page, int max_pages, long num_pages, float scale, float softcap, const long* strides, void* stream);
+int aot_paged_attn_work_floats(int B, int H, int Hk, int D, int page, int max_pages, int with_weights, long* floats);
+
+/* Eviction by collected weight: of the lengths[b] entries of every (sequence, key head) the first `sink`, the last `recent` and the
+ * heaviest others stay, `budget` in all (all of them if there are no more), ties to the lower index, NaN lightest.  The kept entries' K / V
+ * rows are copied in order to the pages of new_table [B, new_pages] (new_pages * page >= budget; pages of the pool that no live sequence
+ * reads -- the old pages are left as they are and may be shared).  kept [B, Hk, budget]: their old indices, -1 behind the last;
+ * new_lengths [B]; new_weights / new_key_pos [B, Hk, S]: moved along, zero behind the last (key_pos optional, both or neither).  A page id
+ * outside the pool moves nothing; a negative id in new_table keeps a sequence where it is (its indices are still reported).
+ * strides: k_pages page place h, v_pages page place h, table b, new_table b, weights b h, new_weights b h, key_pos b h,
+ * new_key_pos b h (16).  Beside the first-and-latest rule of the bounded memory bank (aot_engine.py:307-338). */
+int aot_paged_evict(void* k_pages, void* v_pages, const int* table, const int* new_table, const int* lengths, const float* weights,
+                    const int* key_pos, int* kept, int* new_lengths, float* new_weights, int* new_key_pos, int dtype, int B, int Hk,
+                    int D, int S, int page, int max_pages, int new_pages, long num_pages, int budget, int sink, int recent,
+                    const long* strides, void* stream);
+
 #ifdef __cplusplus
 }
 #endif
