@@ -213,7 +213,7 @@ struct Score {
 
 // ---- forward -------------------------------------------------------------------------------------------------------------------
 template <class T, int DP, int KT>
-__global__ __launch_bounds__(256) void attn_masked_fwd_kernel(MaskP p) {
+__global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void attn_masked_fwd_kernel(MaskP p) {
   using TL = Tile<T, DP, KT>;
   constexpr int NP = TL::NCH / 2, ND = DP / 32, NS = KT / 32;
   __shared__ __align__(16) char smem[4 * TL::BYTES + 2 * KT * 4 + 32];      // K, V of two tiles; ids; flags of the waves
@@ -305,33 +305,41 @@ __global__ __launch_bounds__(256) void attn_masked_fwd_kernel(MaskP p) {
 #pragma unroll
       for (int c = 0; c < NP; ++c) s[n] = mfma32<T>(TL::rows(sk(buf), n * 32, c), qf[c], s[n]);
     }
+    // in powers of two: s * m0 (plain scores are left as they are, the scale goes into the exponential's argument)
+    float m0 = sc.mul;
+    if (sc.capped) {
+      m0 = 1.f;
+#pragma unroll
+      for (int n = 0; n < NS; ++n)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) s[n][r] = sc.cap2 * tanh_from_exp2(s[n][r] * sc.mul);
+    }
+    if (p.slopes) {
+      const float far = (float)(i + p.off - t * KT - 4 * half);
+#pragma unroll
+      for (int n = 0; n < NS; ++n)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) s[n][r] = s[n][r] * m0 - sc.slope * fabsf(far - (float)(n * 32 + mfma32_row(r, 0)));
+      m0 = 1.f;
+    }
+    if (!full) {
+#pragma unroll
+      for (int n = 0; n < NS; ++n)
+#pragma unroll
+        for (int r4 = 0; r4 < 4; ++r4) {
+          const int j0 = n * 32 + 8 * r4 + 4 * half;
+          const i32x4 id = *(const i32x4*)(sid + buf * KT + j0);
+#pragma unroll
+          for (int w = 0; w < 4; ++w)
+            if (!seen(t * KT + j0 + w, id[w])) s[n][4 * r4 + w] = NEG_INF;
+        }
+    }
     float mx = NEG_INF;
 #pragma unroll
     for (int n = 0; n < NS; ++n)
 #pragma unroll
-      for (int r = 0; r < 16; ++r) {
-        float x = s[n][r] * sc.mul;
-        if (sc.capped) x = sc.cap2 * tanh_from_exp2(x);
-        s[n][r] = x;
-      }
-    if (p.slopes)
-#pragma unroll
-      for (int n = 0; n < NS; ++n)
-#pragma unroll
-        for (int r = 0; r < 16; ++r) s[n][r] -= sc.slope * fabsf((float)(i + p.off - (t * KT + n * 32 + mfma32_row(r, half))));
-    if (!full)
-#pragma unroll
-      for (int n = 0; n < NS; ++n)
-#pragma unroll
-        for (int r = 0; r < 16; ++r) {
-          const int j = n * 32 + mfma32_row(r, half);
-          if (!seen(t * KT + j, sid[buf * KT + j])) s[n][r] = NEG_INF;
-        }
-#pragma unroll
-    for (int n = 0; n < NS; ++n)
-#pragma unroll
       for (int r = 0; r < 16; ++r) mx = fmaxf(mx, s[n][r]);
-    mx = fmaxf(mx, __shfl_xor(mx, 32));
+    mx = fmaxf(mx, __shfl_xor(mx, 32)) * m0;
     const float m2 = fmaxf(m, mx), base = m2 == NEG_INF ? 0.f : m2;
     const float f = exp2_hw(m - base);
     m = m2;
@@ -342,7 +350,7 @@ __global__ __launch_bounds__(256) void attn_masked_fwd_kernel(MaskP p) {
 #pragma unroll
     for (int n = 0; n < NS; ++n) {
 #pragma unroll
-      for (int r = 0; r < 16; ++r) { s[n][r] = exp2_hw(s[n][r] - base); l += s[n][r]; }
+      for (int r = 0; r < 16; ++r) { s[n][r] = exp2_hw(__builtin_fmaf(s[n][r], m0, -base)); l += s[n][r]; }
       u32x4 pk[2];
       pack_tile<T>(s[n], pk);
 #pragma unroll
@@ -386,7 +394,7 @@ __global__ __launch_bounds__(256) void attn_masked_fwd_kernel(MaskP p) {
 
 // ---- gradient of the queries -----------------------------------------------------------------------------------------------------
 template <class T, int DP, int KT>
-__global__ __launch_bounds__(256) void attn_masked_dq_kernel(MaskP p) {
+__global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void attn_masked_dq_kernel(MaskP p) {
   using TL = Tile<T, DP, KT>;
   constexpr int NP = TL::NCH / 2, ND = DP / 32, NS = KT / 32;
   __shared__ __align__(16) char smem[4 * TL::BYTES + 2 * KT * 4 + 32];
@@ -497,18 +505,34 @@ __global__ __launch_bounds__(256) void attn_masked_dq_kernel(MaskP p) {
 #pragma unroll
       for (int c = 0; c < NP; ++c) dp = mfma32<T>(TL::rows(sv(buf), n * 32, c), df[c], dp);
 #pragma unroll
-      for (int r = 0; r < 16; ++r) {
-        const int j = n * 32 + mfma32_row(r, half);
-        float x = s[r] * sc.mul, g = dp[r] - delta;
-        if (sc.capped) {
-          const float th = tanh_from_exp2(x);
-          x = sc.cap2 * th;
-          g *= 1.f - th * th;
+      for (int r = 0; r < 16; ++r) dp[r] -= delta;
+      float m0 = sc.mul;
+      if (sc.capped) {
+        m0 = 1.f;
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+          const float th = tanh_from_exp2(s[r] * sc.mul);
+          s[r] = sc.cap2 * th;
+          dp[r] *= 1.f - th * th;
         }
-        if (p.slopes) x -= sc.slope * fabsf((float)(i + p.off - (t * KT + j)));
-        g *= exp2_hw(x - lse);
-        if (!full && !seen(t * KT + j, sid[buf * KT + j])) g = 0.f;
-        s[r] = g;
+      }
+      if (p.slopes) {
+        const float far = (float)(i + p.off - t * KT - n * 32 - 4 * half);
+#pragma unroll
+        for (int r = 0; r < 16; ++r) s[r] = s[r] * m0 - sc.slope * fabsf(far - (float)mfma32_row(r, 0));
+        m0 = 1.f;
+      }
+#pragma unroll
+      for (int r = 0; r < 16; ++r) s[r] = exp2_hw(__builtin_fmaf(s[r], m0, -lse)) * dp[r];
+      if (!full) {
+#pragma unroll
+        for (int r4 = 0; r4 < 4; ++r4) {
+          const int j0 = n * 32 + 8 * r4 + 4 * half;
+          const i32x4 id = *(const i32x4*)(sid + buf * KT + j0);
+#pragma unroll
+          for (int w = 0; w < 4; ++w)
+            if (!seen(t * KT + j0 + w, id[w])) s[4 * r4 + w] = 0.f;
+        }
       }
       u32x4 pk[2];
       pack_tile<T>(s, pk);
@@ -659,24 +683,44 @@ __global__ __launch_bounds__(256) void attn_masked_dkv_kernel(MaskP p) {
         for (int c = 0; c < NP; ++c) dp = mfma32<T>(TL::rows(sd(buf), n * 32, c), vf[c], dp);
 #pragma unroll
         for (int r4 = 0; r4 < 4; ++r4) {
-          const int j0 = n * 32 + 8 * r4 + 4 * half;
-          const f32x4 ls = *(const f32x4*)(slse + buf * QT + j0), de = *(const f32x4*)(sdel + buf * QT + j0);
-          const i32x4 id = *(const i32x4*)(sid + buf * QT + j0);
+          const f32x4 de = *(const f32x4*)(sdel + buf * QT + n * 32 + 8 * r4 + 4 * half);
+#pragma unroll
+          for (int w = 0; w < 4; ++w) dp[4 * r4 + w] -= de[w];
+        }
+        float m0 = sc.mul;
+        if (sc.capped) {
+          m0 = 1.f;
+#pragma unroll
+          for (int r = 0; r < 16; ++r) {
+            const float th = tanh_from_exp2(s[r] * sc.mul);
+            s[r] = sc.cap2 * th;
+            dp[r] *= 1.f - th * th;
+          }
+        }
+        if (p.slopes) {
+          const float far = (float)(tq * QT + n * 32 + 4 * half + p.off - t);
+#pragma unroll
+          for (int r = 0; r < 16; ++r) s[r] = s[r] * m0 - sc.slope * fabsf(far + (float)mfma32_row(r, 0));
+          m0 = 1.f;
+        }
+#pragma unroll
+        for (int r4 = 0; r4 < 4; ++r4) {
+          const f32x4 ls = *(const f32x4*)(slse + buf * QT + n * 32 + 8 * r4 + 4 * half);
 #pragma unroll
           for (int w = 0; w < 4; ++w) {
-            const int r = 4 * r4 + w, i = tq * QT + j0 + w;
-            float x = s[r] * sc.mul, gg = dp[r] - de[w];
-            if (sc.capped) {
-              const float th = tanh_from_exp2(x);
-              x = sc.cap2 * th;
-              gg *= 1.f - th * th;
-            }
-            if (p.slopes) x -= sc.slope * fabsf((float)(i + p.off - t));
-            float pr = exp2_hw(x - ls[w]);
-            gg *= pr;
-            if (!full && !seen(i, id[w])) { pr = 0.f; gg = 0.f; }
-            s[r] = pr;
-            dp[r] = gg;
+            const int r = 4 * r4 + w;
+            s[r] = exp2_hw(__builtin_fmaf(s[r], m0, -ls[w]));
+            dp[r] *= s[r];
+          }
+        }
+        if (!full) {
+#pragma unroll
+          for (int r4 = 0; r4 < 4; ++r4) {
+            const int j0 = n * 32 + 8 * r4 + 4 * half;
+            const i32x4 id = *(const i32x4*)(sid + buf * QT + j0);
+#pragma unroll
+            for (int w = 0; w < 4; ++w)
+              if (!seen(tq * QT + j0 + w, id[w])) { s[4 * r4 + w] = 0.f; dp[4 * r4 + w] = 0.f; }
           }
         }
         u32x4 pk[2];
