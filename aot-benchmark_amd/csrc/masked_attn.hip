@@ -67,42 +67,58 @@ template <class T> __device__ __forceinline__ f32x16 mfma32(const u32x4& a, cons
   }
 }
 
-// A tile of R rows x DP columns in shared memory, 16-byte pieces xor-swizzled by row
+// A tile of R rows x DP columns in shared memory, in lines of 256 bytes (all 64 banks): a row is one line, a part of one, or (fp32, 128
+// columns) two; the 16-byte pieces of a line are xor-swizzled by the line.  The xor is chosen for the two ways a tile is read.  Sixteen
+// lanes read one column of pieces of 16 rows: the xor must differ in all of them.  A transposed read takes 4 rows x 64 bytes (fp32: 2
+// rows four apart x 128 bytes): its low row bits (bit 2 of the row) must move whole 64-byte (128-byte) groups.  With the plain xor by
+// row half of the time in shared memory was bank conflicts.
 template <class T, int DP, int R> struct Tile {
   static constexpr int CE = Elem<T>::CE, NCH = DP / CE, N = R * NCH / 256, ROWB = DP * (int)sizeof(T), BYTES = R * ROWB;
-  static constexpr int SH = NCH >= 16 ? 0 : NCH == 8 ? 1 : 2, MSK = NCH >= 16 ? 15 : NCH - 1;
-  static __device__ __forceinline__ int swz(int row) { return (row >> SH) & MSK; }
+  static __device__ __forceinline__ int at(int row, int c) {      // byte offset of piece c of a row
+    if constexpr (NCH >= 16) {
+      const int f = sizeof(T) == 2 ? ((row & 3) << 2) | ((row >> 2) & 3) : ((row & 4) << 1) | ((row & 8) >> 1) | (row & 3);
+      return row * ROWB + ((c ^ f) << 4);
+    } else if constexpr (NCH == 8) {
+      const int l = row >> 1, f = sizeof(T) == 2 ? ((l & 1) << 2) | ((l >> 1) & 3) : (l & 7) | ((l & 2) << 2);
+      return l * 256 + ((((row & 1) * 8 + c) ^ f) << 4);
+    } else {
+      const int l = row >> 2;
+      return l * 256 + ((((row & 3) * 4 + c) ^ (l & 3)) << 4);
+    }
+  }
   struct Regs { u32x4 r[N]; };
   // rows row0 .. of x (element stride rs), zero past nrow rows and D columns
   static __device__ __forceinline__ void load(Regs& g, const T* x, long rs, int row0, int nrow, int D) {
 #pragma unroll
     for (int i = 0; i < N; ++i) {
-      const int at = threadIdx.x + 256 * i, row = row0 + at / NCH, d = (at % NCH) * CE;
+      const int n = threadIdx.x + 256 * i, row = row0 + n / NCH, d = (n % NCH) * CE;
       g.r[i] = row < nrow && d < D ? *(const u32x4*)(x + (long)row * rs + d) : u32x4{0, 0, 0, 0};
     }
   }
-  static __device__ __forceinline__ bool clean(Regs& g) {        // infinities and NaN to zero; whether there were any
+  static __device__ __forceinline__ bool clean(Regs& g) {        // infinities and NaN to zero; whether the wave had any
     bool bad = false;
 #pragma unroll
     for (int i = 0; i < N; ++i)
 #pragma unroll
-      for (int w = 0; w < 4; ++w) {
-        bad |= word_nonfinite<T>(g.r[i][w]);
-        g.r[i][w] = word_finite<T>(g.r[i][w]);
-      }
-    return bad;
+      for (int w = 0; w < 4; ++w) bad |= word_nonfinite<T>(g.r[i][w]);
+    if (!__any(bad)) return false;
+#pragma unroll
+    for (int i = 0; i < N; ++i)
+#pragma unroll
+      for (int w = 0; w < 4; ++w) g.r[i][w] = word_finite<T>(g.r[i][w]);
+    return true;
   }
   static __device__ __forceinline__ void store(char* lds, const Regs& g) {
 #pragma unroll
     for (int i = 0; i < N; ++i) {
-      const int at = threadIdx.x + 256 * i, row = at / NCH, c = at % NCH;
-      *(u32x4*)(lds + row * ROWB + ((c ^ swz(row)) << 4)) = g.r[i];
+      const int n = threadIdx.x + 256 * i;
+      *(u32x4*)(lds + at(n / NCH, n % NCH)) = g.r[i];
     }
   }
   // first operand of a product over the columns: lane = row row0 + (lane & 31), piece 2 c + lane / 32
   static __device__ __forceinline__ u32x4 rows(const char* lds, int row0, int c) {
-    const int lane = threadIdx.x & 63, row = row0 + (lane & 31);
-    return *(const u32x4*)(lds + row * ROWB + (((2 * c + (lane >> 5)) ^ swz(row)) << 4));
+    const int lane = threadIdx.x & 63;
+    return *(const u32x4*)(lds + row0 * ROWB + at(lane & 31, 2 * c + (lane >> 5)));
   }
   // acc[column 32 db + i][lane's own column] += sum over rows row0 .. row0 + 31 of tile[row][column] * p[row], p in score-tile order
   static __device__ __forceinline__ f32x16 cols(const char* lds, int row0, int db, const u32x4 (&pk)[2], const f32x16& p, f32x16 acc) {
@@ -114,10 +130,10 @@ template <class T, int DP, int R> struct Tile {
         u32x4 a;
 #pragma unroll
         for (int s = 0; s < 2; ++s) {
-          const int row = row0 + 16 * kb + 8 * s + 4 * (lane >> 5) + (i >> 2);
+          const int row = 8 * s + 4 * (lane >> 5) + (i >> 2);
           typedef short s16x4 __attribute__((ext_vector_type(4)));
           typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
-          const s16x4 x = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(lds + row * ROWB + ((c ^ swz(row)) << 4) + sub));
+          const s16x4 x = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(lds + (row0 + 16 * kb) * ROWB + at(row, c) + sub));
           const u32x2 y = __builtin_bit_cast(u32x2, x);
           a[2 * s] = y[0];
           a[2 * s + 1] = y[1];
@@ -128,8 +144,8 @@ template <class T, int DP, int R> struct Tile {
       const int d = db * 32 + (lane & 31), c = d / CE, e = d % CE;
 #pragma unroll
       for (int r = 0; r < 16; ++r) {
-        const int row = row0 + mfma32_row(r, lane >> 5);
-        const float a = *(const float*)(lds + row * ROWB + ((c ^ swz(row)) << 4) + e * 4);
+        const int row = mfma32_row(r & 7, lane >> 5);
+        const float a = *(const float*)(lds + (row0 + 16 * (r >> 3)) * ROWB + at(row, c) + e * 4);
         acc = __builtin_amdgcn_mfma_f32_32x32x2f32(a, p[r], acc, 0, 0, 0);
       }
     }
@@ -260,9 +276,9 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void attn_masked_fwd_k
     }
     return true;
   };
-  auto seen = [&](int t, int id) {
-    return t < p.Sk && (!p.causal || t <= i + p.off || t < prefix) && id == myid && id >= 0;
-  };
+  // the last key this lane's query sees, documents aside (none: -1)
+  const int lim = myid < 0 || !iok ? -1 : p.causal ? min(p.Sk - 1, max(i + p.off, prefix - 1)) : p.Sk - 1;
+  auto seen = [&](int t, int id) { return t <= lim && id == myid; };
 
   typename TL::Regs gk, gv;
   int gid = 0;
@@ -273,7 +289,7 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void attn_masked_fwd_k
   };
   auto put = [&](int buf, bool full) {
     if (!full) {
-      const bool bad = __any(TL::clean(gv));
+      const bool bad = TL::clean(gv);
       if (lane == 0) sbad[buf * 4 + wave] = bad;
     }
     TL::store(sk(buf), gk);
@@ -328,10 +344,15 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void attn_masked_fwd_k
 #pragma unroll
         for (int r4 = 0; r4 < 4; ++r4) {
           const int j0 = n * 32 + 8 * r4 + 4 * half;
-          const i32x4 id = *(const i32x4*)(sid + buf * KT + j0);
 #pragma unroll
           for (int w = 0; w < 4; ++w)
-            if (!seen(t * KT + j0 + w, id[w])) s[n][4 * r4 + w] = NEG_INF;
+            if (j0 + w > lim - t * KT) s[n][4 * r4 + w] = NEG_INF;
+          if (p.doc_k) {
+            const i32x4 id = *(const i32x4*)(sid + buf * KT + j0);
+#pragma unroll
+            for (int w = 0; w < 4; ++w)
+              if (id[w] != myid) s[n][4 * r4 + w] = NEG_INF;
+          }
         }
     }
     float mx = NEG_INF;
@@ -461,9 +482,9 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void attn_masked_dq_ke
     }
     return true;
   };
-  auto seen = [&](int t, int id) {
-    return t < p.Sk && (!p.causal || t <= i + p.off || t < prefix) && id == myid && id >= 0;
-  };
+  // the last key this lane's query sees, documents aside (none: -1)
+  const int lim = myid < 0 || !iok ? -1 : p.causal ? min(p.Sk - 1, max(i + p.off, prefix - 1)) : p.Sk - 1;
+  auto seen = [&](int t, int id) { return t <= lim && id == myid; };
   typename TL::Regs gk, gv;
   int gid = 0;
   auto fetch = [&](int t) {
@@ -473,7 +494,7 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void attn_masked_dq_ke
   };
   auto put = [&](int buf, bool full) {
     if (!full) {
-      const bool bad = __any(TL::clean(gk));
+      const bool bad = TL::clean(gk);
       if (lane == 0) sbad[buf * 4 + wave] = bad;
     }
     TL::store(sk(buf), gk);
@@ -528,10 +549,15 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void attn_masked_dq_ke
 #pragma unroll
         for (int r4 = 0; r4 < 4; ++r4) {
           const int j0 = n * 32 + 8 * r4 + 4 * half;
-          const i32x4 id = *(const i32x4*)(sid + buf * KT + j0);
 #pragma unroll
           for (int w = 0; w < 4; ++w)
-            if (!seen(t * KT + j0 + w, id[w])) s[4 * r4 + w] = 0.f;
+            if (j0 + w > lim - t * KT) s[4 * r4 + w] = 0.f;
+          if (p.doc_k) {
+            const i32x4 id = *(const i32x4*)(sid + buf * KT + j0);
+#pragma unroll
+            for (int w = 0; w < 4; ++w)
+              if (id[w] != myid) s[4 * r4 + w] = 0.f;
+          }
         }
       }
       u32x4 pk[2];
@@ -617,9 +643,9 @@ __global__ __launch_bounds__(256) void attn_masked_dkv_kernel(MaskP p) {
     }
     return true;
   };
-  auto seen = [&](int i, int id) {
-    return i < p.Sq && (!p.causal || t <= i + p.off || t < prefix) && id == myid && id >= 0;
-  };
+  // the first query that sees this lane's key, documents aside
+  const int lim = myid < 0 || !tok ? 0x7fffffff : p.causal && t >= prefix ? t - p.off : 0;
+  auto seen = [&](int i, int id) { return i >= lim && i < p.Sq && id == myid; };
   f32x16 dk[ND], dv[ND];
 #pragma unroll
   for (int d = 0; d < ND; ++d)
@@ -650,7 +676,7 @@ __global__ __launch_bounds__(256) void attn_masked_dkv_kernel(MaskP p) {
     };
     auto put = [&](int buf, bool full) {
       if (!full) {
-        const bool x = TL::clean(gq), y = TL::clean(gd), bad = __any(x || y);
+        const bool x = TL::clean(gq), y = TL::clean(gd), bad = x || y;
         if (lane == 0) sbad[buf * 4 + wave] = bad;
       }
       TL::store(sq(buf), gq);
@@ -720,7 +746,7 @@ __global__ __launch_bounds__(256) void attn_masked_dkv_kernel(MaskP p) {
             const i32x4 id = *(const i32x4*)(sid + buf * QT + j0);
 #pragma unroll
             for (int w = 0; w < 4; ++w)
-              if (!seen(tq * QT + j0 + w, id[w])) { s[4 * r4 + w] = 0.f; dp[4 * r4 + w] = 0.f; }
+              if (j0 + w < lim - tq * QT || id[w] != myid) { s[4 * r4 + w] = 0.f; dp[4 * r4 + w] = 0.f; }
           }
         }
         u32x4 pk[2];
