@@ -203,6 +203,12 @@ template <int PER> struct Tiles {                                // PER tiles a 
   }
 };
 
+// the head width, read where it is needed: as a loop invariant its 64 comparisons would sit in scalar registers throughout the loop
+__device__ __forceinline__ int width_here(const MaskP& p) {
+  int d = p.D;
+  asm volatile("" : "+s"(d));
+  return d;
+}
 __device__ __forceinline__ bool any_flag(const int* f) { return (f[0] | f[1] | f[2] | f[3]) != 0; }
 
 struct Head { int b, h, hk; };
@@ -378,6 +384,7 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void attn_masked_fwd_k
       for (int d = 0; d < ND; ++d) o[d] = TL::cols(sv(buf), n * 32, d, pk, s[n], o[d]);
     }
     if (!full && any_flag(sbad + buf * 4)) {                                    // the seen infinities and NaN that staging left out
+      const int width = width_here(p);
       for (int j = 0; j < KT; ++j) {
         if (!seen(t * KT + j, sid[buf * KT + j])) continue;
         const T* row = V + (long)(t * KT + j) * p.vs[1];
@@ -386,7 +393,7 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void attn_masked_fwd_k
 #pragma unroll
           for (int r = 0; r < 16; ++r) {
             const int e = d * 32 + mfma32_row(r, half);
-            if (e < p.D) {
+            if (e < width) {
               const float x = (float)row[e];
               if (!(fabsf(x) < __builtin_inff())) o[d][r] += x;
             }
@@ -402,13 +409,14 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void attn_masked_fwd_k
   l += __shfl_xor(l, 32);
   if (!iok) return;
   const float inv = l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l);
+  const int width = width_here(p);
   T* out = (T*)p.out + hd.b * p.os[0] + (long)i * p.os[1] + hd.h * p.os[2];
 #pragma unroll
   for (int d = 0; d < ND; ++d)
 #pragma unroll
     for (int r = 0; r < 16; ++r) {
       const int e = d * 32 + mfma32_row(r, half);
-      if (e < p.D) out[e] = (T)(o[d][r] * inv);
+      if (e < width) out[e] = (T)(o[d][r] * inv);
     }
   if (half == 0) p.lse[((long)hd.b * p.H + hd.h) * p.Sq + i] = l == 0.f ? NEG_INF : m + log2f(l);
 }
@@ -566,6 +574,7 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void attn_masked_dq_ke
       for (int d = 0; d < ND; ++d) dq[d] = TL::cols(sk(buf), n * 32, d, pk, s, dq[d]);
     }
     if (!full && any_flag(sbad + buf * 4)) {
+      const int width = width_here(p);
       for (int j = 0; j < KT; ++j) {
         if (!seen(t * KT + j, sid[buf * KT + j])) continue;
         const T* row = K + (long)(t * KT + j) * p.ks[1];
@@ -574,7 +583,7 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void attn_masked_dq_ke
 #pragma unroll
           for (int r = 0; r < 16; ++r) {
             const int e = d * 32 + mfma32_row(r, half);
-            if (e < p.D) {
+            if (e < width) {
               const float x = (float)row[e];
               if (!(fabsf(x) < __builtin_inff())) dq[d][r] += x;
             }
@@ -588,13 +597,14 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void attn_masked_dq_ke
     full = fulln;
   }
   if (!iok) return;
+  const int width = width_here(p);
   T* out = (T*)p.dq + hd.b * p.dqs[0] + (long)i * p.dqs[1] + hd.h * p.dqs[2];
 #pragma unroll
   for (int d = 0; d < ND; ++d)
 #pragma unroll
     for (int r = 0; r < 16; ++r) {
       const int e = d * 32 + mfma32_row(r, half);
-      if (e < p.D) out[e] = (T)(dq[d][r] * p.scale);
+      if (e < width) out[e] = (T)(dq[d][r] * p.scale);
     }
 }
 
@@ -758,6 +768,7 @@ __global__ __launch_bounds__(256) void attn_masked_dkv_kernel(MaskP p) {
         for (int d = 0; d < ND; ++d) dk[d] = TL::cols(sq(buf), n * 32, d, pk, dp, dk[d]);
       }
       if (!full && any_flag(sbad + buf * 4)) {
+        const int width = width_here(p);
         for (int j = 0; j < QT; ++j) {
           const int i = tq * QT + j;
           if (!seen(i, sid[buf * QT + j])) continue;
@@ -767,7 +778,7 @@ __global__ __launch_bounds__(256) void attn_masked_dkv_kernel(MaskP p) {
 #pragma unroll
             for (int r = 0; r < 16; ++r) {
               const int e = d * 32 + mfma32_row(r, half);
-              if (e < p.D) {
+              if (e < width) {
                 const float x = (float)r1[e], y = (float)r2[e];
                 if (!(fabsf(x) < __builtin_inff())) dv[d][r] += x;
                 if (!(fabsf(y) < __builtin_inff())) dk[d][r] += y;
@@ -783,6 +794,7 @@ __global__ __launch_bounds__(256) void attn_masked_dkv_kernel(MaskP p) {
     }
   }
   if (!tok) return;
+  const int width = width_here(p);
   T* ok = (T*)p.dk + b * p.dks[0] + (long)t * p.dks[1] + hk * p.dks[2];
   T* ov = (T*)p.dv + b * p.dvs[0] + (long)t * p.dvs[1] + hk * p.dvs[2];
 #pragma unroll
@@ -790,7 +802,7 @@ __global__ __launch_bounds__(256) void attn_masked_dkv_kernel(MaskP p) {
 #pragma unroll
     for (int r = 0; r < 16; ++r) {
       const int e = d * 32 + mfma32_row(r, half);
-      if (e < p.D) {
+      if (e < width) {
         ok[e] = (T)(dk[d][r] * p.scale);
         ov[e] = (T)dv[d][r];
       }

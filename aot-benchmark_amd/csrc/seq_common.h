@@ -22,12 +22,11 @@ template <> struct Elem<bf16> { static constexpr int CE = 8; };
 __device__ __forceinline__ float exp2_hw(float x) { return __builtin_amdgcn_exp2f(x); }
 __device__ __forceinline__ float rcp_hw(float x) { return __builtin_amdgcn_rcpf(x); }
 
-// two floats rounded to nearest even into one dword (low half first)
+// two floats rounded to nearest even into one dword, low half first (one packed conversion)
 template <class T> __device__ __forceinline__ unsigned pack2(float a, float b) {
-  union { T h[2]; unsigned u; } r;
-  r.h[0] = (T)a;
-  r.h[1] = (T)b;
-  return r.u;
+  typedef float f2 __attribute__((ext_vector_type(2)));
+  typedef T t2 __attribute__((ext_vector_type(2)));
+  return __builtin_bit_cast(unsigned, __builtin_convertvector((f2{a, b}), t2));
 }
 template <class T> __device__ __forceinline__ float half_to_float(u16 x) {
   union { u16 u; T h; } r;
