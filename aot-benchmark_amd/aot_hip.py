@@ -98,7 +98,8 @@ _SIGS = {
     'aot_rope': [_P] * 6 + [_I] * 9 + [_F, _P, _P],
     'aot_rope_append': [_P] * 9 + [_I] * 7 + [_F, _I, _L, _P, _P],
     'aot_attn_masked': [_P] * 10 + [_I] * 8 + [_F, _F, _P, _P],
-    'aot_attn_masked_bwd': [_P] * 15 + [_I] * 8 + [_F, _F, _P, _P],
+    'aot_attn_masked_bwd': [_P] * 15 + [_L] + [_I] * 8 + [_F, _F, _P, _P],
+    'aot_attn_masked_bwd_floats': [_I] * 6 + [_P],
     'aot_paged_attn': [_P] * 10 + [_L] + [_I] * 7 + [_L, _F, _F, _P, _P],
     'aot_paged_attn_work_floats': [_I] * 7 + [_P],
     'aot_paged_evict': [_P] * 11 + [_I] * 8 + [_L] + [_I] * 3 + [_P, _P],
@@ -1234,11 +1235,13 @@ def attn_masked_bwd(dout, q, k, v, out, lse, scale=None, causal=False, softcap=0
         dq = torch.empty((B, Sq, H, D), dtype=q.dtype, device=dev)
         dk = torch.empty((B, Sk, Hk, D), dtype=q.dtype, device=dev)
         dv = torch.empty((B, Sk, Hk, D), dtype=q.dtype, device=dev)
-        delta = torch.empty(B * H * Sq, dtype=torch.float32, device=dev)
+        n = _L()
+        _chk(load().aot_attn_masked_bwd_floats(B, Sq, Sk, H, Hk, D, ctypes.addressof(n)), 'aot_attn_masked_bwd_floats')
+        work = torch.empty(max(n.value, 1), dtype=torch.float32, device=dev)
         ranges = torch.empty(4 * B * (-(-Sq // 64) + -(-Sk // 64)), dtype=torch.int32, device=dev) if doc_q is not None else None
         if B and (Sq or Sk):
             _chk(load().aot_attn_masked_bwd(_ptr(q), _ptr(k), _ptr(v), _ptr(out), _ptr(lse), _ptr(dout), _ptr(dq), _ptr(dk), _ptr(dv), _ptr(slopes),
-                                            _ptr(doc_q) or _ptr(doc_k), _ptr(doc_k) or _ptr(doc_q), _ptr(prefix), _ptr(ranges), _ptr(delta), _DTYPE[q.dtype],
+                                            _ptr(doc_q) or _ptr(doc_k), _ptr(doc_k) or _ptr(doc_q), _ptr(prefix), _ptr(ranges), _ptr(work), n.value, _DTYPE[q.dtype],
                                             B, Sq, Sk, H, Hk, D, int(causal), scale, softcap,
                                             _longs((q, 3), (k, 3), (v, 3), (out, 3), (dout, 3), (dq, 3), (dk, 3), (dv, 3), (doc_q, 1), (doc_k, 1)),
                                             stream if stream is not None else s), 'aot_attn_masked_bwd')

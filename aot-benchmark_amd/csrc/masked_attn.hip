@@ -19,8 +19,8 @@
 // largest document id (doc_range_kernel), tested 64 tiles at a time by one ballot.
 //
 // Masked places may hold anything.  A masked score is replaced, never multiplied; where a masked row would enter a product with
-// weight zero (0 * inf is NaN), tiles with a mask are staged with infinities and NaN replaced by zero, and if there were any, the
-// seen ones among them are added element by element afterwards.
+// weight zero (0 * inf is NaN), tiles with a mask are staged with infinities and NaN replaced by zero; if there were any, a second walk
+// over those tiles counts the seen ones (the same product, of 0 / 1 weights and small codes) and adds what they make of the sums.
 //
 // Scores, statistics and sums are 32-bit.  p and ds are rounded to the inputs' type for the following product (nearest even: 2^-9 of
 // the value for bf16, 2^-12 for fp16, below which fp16 also loses what is under 6e-8), the sum that divides is not.
@@ -36,7 +36,8 @@ struct MaskP {
   const int *doc_q, *doc_k, *prefix;
   const int4 *rq, *rk;                                         // (smallest id >= 0, largest id, 1 if any is negative, 0) of RG tokens
   long qs[3], ks[3], vs[3], os[3], dos[3], dqs[3], dks[3], dvs[3], dcs[2];
-  int B, Sq, Sk, H, Hk, G, D, causal, off;
+  float* part;                                                 // split key blocks: [nsplit][dv, dk][B][Sk][Hk][D]
+  int B, Sq, Sk, H, Hk, G, D, causal, off, nsplit;
   float scale, softcap;
 };
 
@@ -67,13 +68,23 @@ template <class T> __device__ __forceinline__ f32x16 mfma32(const u32x4& a, cons
   }
 }
 
+template <class T> __device__ __forceinline__ void pack_tile(const f32x16& p, u32x4 (&pk)[2]) {
+  if constexpr (sizeof(T) == 2) {
+#pragma unroll
+    for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) pk[kb][i] = pack2<T>(p[8 * kb + 2 * i], p[8 * kb + 2 * i + 1]);
+  }
+}
+
 // A tile of R rows x DP columns in shared memory, in lines of 256 bytes (all 64 banks): a row is one line, a part of one, or (fp32, 128
 // columns) two; the 16-byte pieces of a line are xor-swizzled by the line.  The xor is chosen for the two ways a tile is read.  Sixteen
 // lanes read one column of pieces of 16 rows: the xor must differ in all of them.  A transposed read takes 4 rows x 64 bytes (fp32: 2
 // rows four apart x 128 bytes): its low row bits (bit 2 of the row) must move whole 64-byte (128-byte) groups.  With the plain xor by
 // row half of the time in shared memory was bank conflicts.
-template <class T, int DP, int R> struct Tile {
-  static constexpr int CE = Elem<T>::CE, NCH = DP / CE, N = R * NCH / 256, ROWB = DP * (int)sizeof(T), BYTES = R * ROWB;
+template <class T, int DP, int R, int NT> struct Tile {           // NT threads stage it
+  static constexpr int CE = Elem<T>::CE, NCH = DP / CE, N = (R * NCH + NT - 1) / NT, ROWB = DP * (int)sizeof(T), BYTES = R * ROWB;
+  static constexpr bool EVEN = R * NCH % NT == 0;                 // (else some threads have nothing to stage)
   static __device__ __forceinline__ int at(int row, int c) {      // byte offset of piece c of a row
     if constexpr (NCH >= 16) {
       const int f = sizeof(T) == 2 ? ((row & 3) << 2) | ((row >> 2) & 3) : ((row & 4) << 1) | ((row & 8) >> 1) | (row & 3);
@@ -86,13 +97,14 @@ template <class T, int DP, int R> struct Tile {
       return l * 256 + ((((row & 3) * 4 + c) ^ (l & 3)) << 4);
     }
   }
+  static __device__ __forceinline__ void pack(const f32x16& p, u32x4 (&pk)[2]) { pack_tile<T>(p, pk); }
   struct Regs { u32x4 r[N]; };
   // rows row0 .. of x (element stride rs), zero past nrow rows and D columns
   static __device__ __forceinline__ void load(Regs& g, const T* x, long rs, int row0, int nrow, int D) {
 #pragma unroll
     for (int i = 0; i < N; ++i) {
-      const int n = threadIdx.x + 256 * i, row = row0 + n / NCH, d = (n % NCH) * CE;
-      g.r[i] = row < nrow && d < D ? *(const u32x4*)(x + (long)row * rs + d) : u32x4{0, 0, 0, 0};
+      const int n = threadIdx.x + NT * i, row = row0 + n / NCH, d = (n % NCH) * CE;
+      g.r[i] = row < nrow && d < D && (EVEN || n < R * NCH) ? *(const u32x4*)(x + (long)row * rs + d) : u32x4{0, 0, 0, 0};
     }
   }
   static __device__ __forceinline__ bool clean(Regs& g) {        // infinities and NaN to zero; whether the wave had any
@@ -108,11 +120,35 @@ template <class T, int DP, int R> struct Tile {
       for (int w = 0; w < 4; ++w) g.r[i][w] = word_finite<T>(g.r[i][w]);
     return true;
   }
+  // finite elements to 0, +inf to 1, -inf to 2^8, NaN to 2^15: sums of up to 64 of each stay apart
+  // Written over the tile, one piece at a time: the rare path must not cost the common one registers.
+  static __device__ __forceinline__ void encode(char* lds, const T* x, long rs, int row0, int nrow, int D) {
+#pragma unroll 1
+    for (int n = threadIdx.x; n < R * NCH; n += NT) {
+      const int row = row0 + n / NCH, d = (n % NCH) * CE;
+      u32x4 v = row < nrow && d < D ? *(const u32x4*)(x + (long)row * rs + d) : u32x4{0, 0, 0, 0};
+#pragma unroll
+      for (int w = 0; w < 4; ++w) {
+        if constexpr (sizeof(T) == 4) v[w] = __float_as_uint(code(__uint_as_float(v[w])));
+        else v[w] = pack2<T>(code(half_to_float<T>((u16)v[w])), code(half_to_float<T>((u16)(v[w] >> 16))));
+      }
+      *(u32x4*)(lds + at(n / NCH, n % NCH)) = v;
+    }
+  }
+  static __device__ __forceinline__ float code(float x) {
+    return fabsf(x) < __builtin_inff() ? 0.f : x != x ? 32768.f : x > 0.f ? 1.f : 256.f;
+  }
+  static __device__ __forceinline__ float decode(float sum) {    // what such a sum adds to a result
+    const int n = (int)sum;
+    if (n == 0) return 0.f;
+    const bool pos = n & 255, neg = n & 0x7f00;
+    return n >= 32768 || (pos && neg) ? __builtin_nanf("") : pos ? __builtin_inff() : -__builtin_inff();
+  }
   static __device__ __forceinline__ void store(char* lds, const Regs& g) {
 #pragma unroll
     for (int i = 0; i < N; ++i) {
-      const int n = threadIdx.x + 256 * i;
-      *(u32x4*)(lds + at(n / NCH, n % NCH)) = g.r[i];
+      const int n = threadIdx.x + NT * i;
+      if (EVEN || n < R * NCH) *(u32x4*)(lds + at(n / NCH, n % NCH)) = g.r[i];
     }
   }
   // first operand of a product over the columns: lane = row row0 + (lane & 31), piece 2 c + lane / 32
@@ -120,26 +156,28 @@ template <class T, int DP, int R> struct Tile {
     const int lane = threadIdx.x & 63;
     return *(const u32x4*)(lds + row0 * ROWB + at(lane & 31, 2 * c + (lane >> 5)));
   }
+  // 16-bit: first operand of a product over 16 rows (row0 + 16 kb ..) of the tile, in score-tile order: lane = column 32 db + (lane & 31)
+  static __device__ __forceinline__ u32x4 col16(const char* lds, int row0, int db, int kb) {
+    const int lane = threadIdx.x & 63, i = lane & 15, c = db * 4 + ((lane >> 4) & 1) * 2 + ((i & 3) >> 1), sub = (i & 1) * 8;
+    u32x4 a;
+#pragma unroll
+    for (int s = 0; s < 2; ++s) {
+      const int row = 8 * s + 4 * (lane >> 5) + (i >> 2);
+      typedef short s16x4 __attribute__((ext_vector_type(4)));
+      typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
+      const s16x4 x = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(lds + (row0 + 16 * kb) * ROWB + at(row, c) + sub));
+      const u32x2 y = __builtin_bit_cast(u32x2, x);
+      a[2 * s] = y[0];
+      a[2 * s + 1] = y[1];
+    }
+    return a;
+  }
   // acc[column 32 db + i][lane's own column] += sum over rows row0 .. row0 + 31 of tile[row][column] * p[row], p in score-tile order
   static __device__ __forceinline__ f32x16 cols(const char* lds, int row0, int db, const u32x4 (&pk)[2], const f32x16& p, f32x16 acc) {
     const int lane = threadIdx.x & 63;
     if constexpr (sizeof(T) == 2) {
-      const int i = lane & 15, c = db * 4 + ((lane >> 4) & 1) * 2 + ((i & 3) >> 1), sub = (i & 1) * 8;
 #pragma unroll
-      for (int kb = 0; kb < 2; ++kb) {
-        u32x4 a;
-#pragma unroll
-        for (int s = 0; s < 2; ++s) {
-          const int row = 8 * s + 4 * (lane >> 5) + (i >> 2);
-          typedef short s16x4 __attribute__((ext_vector_type(4)));
-          typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
-          const s16x4 x = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(lds + (row0 + 16 * kb) * ROWB + at(row, c) + sub));
-          const u32x2 y = __builtin_bit_cast(u32x2, x);
-          a[2 * s] = y[0];
-          a[2 * s + 1] = y[1];
-        }
-        acc = mfma32<T>(a, pk[kb], acc);
-      }
+      for (int kb = 0; kb < 2; ++kb) acc = mfma32<T>(col16(lds, row0, db, kb), pk[kb], acc);
     } else {
       const int d = db * 32 + (lane & 31), c = d / CE, e = d % CE;
 #pragma unroll
@@ -152,15 +190,6 @@ template <class T, int DP, int R> struct Tile {
     return acc;
   }
 };
-
-template <class T> __device__ __forceinline__ void pack_tile(const f32x16& p, u32x4 (&pk)[2]) {
-  if constexpr (sizeof(T) == 2) {
-#pragma unroll
-    for (int kb = 0; kb < 2; ++kb)
-#pragma unroll
-      for (int i = 0; i < 4; ++i) pk[kb][i] = pack2<T>(p[8 * kb + 2 * i], p[8 * kb + 2 * i + 1]);
-  }
-}
 
 // the lane's own row (or none), in 16-byte pieces 2 c + lane / 32
 template <class T, int NP> __device__ __forceinline__ void own_row(u32x4 (&f)[NP], const T* x, bool ok, int D) {
@@ -175,16 +204,17 @@ template <class T, int NP> __device__ __forceinline__ void own_row(u32x4 (&f)[NP
 // Tiles of the other side that this workgroup visits: [first, last), of them those whose document range meets [lo, hi]
 template <int PER> struct Tiles {                                // PER tiles a document range
   const int4* r;
-  int base, last, lo, hi;
+  int base, last, lo, hi, step, mine;
   unsigned long long mask;
-  __device__ __forceinline__ void init(const int4* ranges, int first, int last_, int lo_, int hi_) {
-    r = ranges; base = first; last = last_; lo = lo_; hi = hi_;
+  // of the tiles those with index = mine_ modulo step_
+  __device__ __forceinline__ void init(const int4* ranges, int first, int last_, int lo_, int hi_, int step_ = 1, int mine_ = 0) {
+    r = ranges; base = first; last = last_; lo = lo_; hi = hi_; step = step_; mine = mine_;
     if (r && hi < 0) last = first;                               // every id of ours is negative: nothing is seen
     fill();
   }
   __device__ __forceinline__ void fill() {
     const int t = base + (threadIdx.x & 63);
-    bool on = t < last;
+    bool on = t < last && (step == 1 || t % step == mine);
     if (on && r) {
       const int4 x = r[t / PER];
       on = x.y >= 0 && x.y >= lo && x.x <= hi;
@@ -203,13 +233,17 @@ template <int PER> struct Tiles {                                // PER tiles a 
   }
 };
 
-// the head width, read where it is needed: as a loop invariant its 64 comparisons would sit in scalar registers throughout the loop
-__device__ __forceinline__ int width_here(const MaskP& p) {
-  int d = p.D;
-  asm volatile("" : "+s"(d));
-  return d;
+// four consecutive results of a row
+template <class T> __device__ __forceinline__ void store4(T* x, float a, float b, float c, float d) {
+  if constexpr (sizeof(T) == 4) *(f32x4*)x = f32x4{a, b, c, d};
+  else *(u32x2*)x = u32x2{pack2<T>(a, b), pack2<T>(c, d)};
 }
-__device__ __forceinline__ bool any_flag(const int* f) { return (f[0] | f[1] | f[2] | f[3]) != 0; }
+template <int N> __device__ __forceinline__ bool any_flag(const int* f) {
+  int x = 0;
+#pragma unroll
+  for (int i = 0; i < N; ++i) x |= f[i];
+  return x != 0;
+}
 
 struct Head { int b, h, hk; };
 // consecutive workgroups walk the (sequence, key head) pairs, so those that read the same keys land on the same of the 8 XCDs
@@ -233,16 +267,39 @@ struct Score {
   }
 };
 
+// acc += what the encoded tile's rows that `seen` admits add to each column
+template <class TL, int R, int ND, class F> __device__ __forceinline__ void add_seen(f32x16 (&acc)[ND], const char* lds, F&& seen) {
+  const int half = (threadIdx.x & 63) >> 5;
+#pragma unroll 1
+  for (int n = 0; n < R / 32; ++n) {
+    f32x16 one;
+#pragma unroll
+    for (int r = 0; r < 16; ++r) one[r] = seen(n * 32 + mfma32_row(r, half)) ? 1.f : 0.f;
+    u32x4 pk[2];
+    TL::pack(one, pk);
+#pragma unroll
+    for (int d = 0; d < ND; ++d) {
+      __builtin_amdgcn_sched_barrier(0);
+      f32x16 z;
+#pragma unroll
+      for (int r = 0; r < 16; ++r) z[r] = 0.f;
+      z = TL::cols(lds, n * 32, d, pk, one, z);
+#pragma unroll
+      for (int r = 0; r < 16; ++r) acc[d][r] += TL::decode(z[r]);
+    }
+  }
+}
+
 // ---- forward -------------------------------------------------------------------------------------------------------------------
 template <class T, int DP, int KT>
 __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void attn_masked_fwd_kernel(MaskP p) {
-  using TL = Tile<T, DP, KT>;
+  using TL = Tile<T, DP, KT, 256>;
   constexpr int NP = TL::NCH / 2, ND = DP / 32, NS = KT / 32;
   __shared__ __align__(16) char smem[4 * TL::BYTES + 2 * KT * 4 + 32];      // K, V of two tiles; ids; flags of the waves
   auto sk = [&](int buf) { return smem + buf * TL::BYTES; };
   auto sv = [&](int buf) { return smem + (2 + buf) * TL::BYTES; };
   int* const sid = (int*)(smem + 4 * TL::BYTES);                // [2][KT]
-  int* const sbad = sid + 2 * KT;                               // [2][4]
+  int* const sbad = sid + 2 * KT;                               // [4]
   const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, half = lane >> 5;
   const Head hd = head_of(blockIdx.x, p);
   const int q0 = (p.causal ? gridDim.y - 1 - blockIdx.y : blockIdx.y) * 128;      // the long rows of a causal mask first
@@ -288,16 +345,14 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void attn_masked_fwd_k
 
   typename TL::Regs gk, gv;
   int gid = 0;
+  bool dirty = false;
   auto fetch = [&](int t) {
     TL::load(gk, K, p.ks[1], t * KT, p.Sk, p.D);
     TL::load(gv, V, p.vs[1], t * KT, p.Sk, p.D);
     if (p.doc_k && threadIdx.x < KT) gid = t * KT + (int)threadIdx.x < p.Sk ? p.doc_k[hd.b * p.dcs[1] + t * KT + threadIdx.x] : -1;
   };
   auto put = [&](int buf, bool full) {
-    if (!full) {
-      const bool bad = TL::clean(gv);
-      if (lane == 0) sbad[buf * 4 + wave] = bad;
-    }
+    if (!full) dirty |= TL::clean(gv);
     TL::store(sk(buf), gk);
     TL::store(sv(buf), gv);
     if (threadIdx.x < KT) sid[buf * KT + threadIdx.x] = gid;
@@ -383,40 +438,36 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void attn_masked_fwd_k
 #pragma unroll
       for (int d = 0; d < ND; ++d) o[d] = TL::cols(sv(buf), n * 32, d, pk, s[n], o[d]);
     }
-    if (!full && any_flag(sbad + buf * 4)) {                                    // the seen infinities and NaN that staging left out
-      const int width = width_here(p);
-      for (int j = 0; j < KT; ++j) {
-        if (!seen(t * KT + j, sid[buf * KT + j])) continue;
-        const T* row = V + (long)(t * KT + j) * p.vs[1];
-#pragma unroll
-        for (int d = 0; d < ND; ++d)
-#pragma unroll
-          for (int r = 0; r < 16; ++r) {
-            const int e = d * 32 + mfma32_row(r, half);
-            if (e < width) {
-              const float x = (float)row[e];
-              if (!(fabsf(x) < __builtin_inff())) o[d][r] += x;
-            }
-          }
-      }
-    }
     if (tn >= 0) put(buf ^ 1, fulln);
     __syncthreads();
     buf ^= 1;
     t = tn;
     full = fulln;
   }
+  // The seen infinities and NaN that staging left out, if it met any (in a masked tile): once more over the masked tiles
+  if (lane == 0) sbad[wave] = dirty;
+  __syncthreads();
+  if (any_flag<4>(sbad)) {
+    it.init(rk, 0, (max(tend, 0) + KT - 1) / KT, qr.x, qr.y);
+    for (t = it.next(); t >= 0; t = it.next()) {
+      if (whole(t)) continue;
+      __syncthreads();
+      TL::encode(smem, V, p.vs[1], t * KT, p.Sk, p.D);
+      if (threadIdx.x < KT) sid[threadIdx.x] = t * KT + (int)threadIdx.x < p.Sk && p.doc_k ? p.doc_k[hd.b * p.dcs[1] + t * KT + threadIdx.x] : 0;
+      __syncthreads();
+      add_seen<TL, KT>(o, smem, [&](int j) { return seen(t * KT + j, sid[j]); });
+    }
+  }
   l += __shfl_xor(l, 32);
   if (!iok) return;
   const float inv = l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l);
-  const int width = width_here(p);
   T* out = (T*)p.out + hd.b * p.os[0] + (long)i * p.os[1] + hd.h * p.os[2];
 #pragma unroll
   for (int d = 0; d < ND; ++d)
 #pragma unroll
-    for (int r = 0; r < 16; ++r) {
+    for (int r = 0; r < 16; r += 4) {
       const int e = d * 32 + mfma32_row(r, half);
-      if (e < width) out[e] = (T)(o[d][r] * inv);
+      if (e < p.D) store4(out + e, o[d][r] * inv, o[d][r + 1] * inv, o[d][r + 2] * inv, o[d][r + 3] * inv);
     }
   if (half == 0) p.lse[((long)hd.b * p.H + hd.h) * p.Sq + i] = l == 0.f ? NEG_INF : m + log2f(l);
 }
@@ -424,7 +475,7 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void attn_masked_fwd_k
 // ---- gradient of the queries -----------------------------------------------------------------------------------------------------
 template <class T, int DP, int KT>
 __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void attn_masked_dq_kernel(MaskP p) {
-  using TL = Tile<T, DP, KT>;
+  using TL = Tile<T, DP, KT, 256>;
   constexpr int NP = TL::NCH / 2, ND = DP / 32, NS = KT / 32;
   __shared__ __align__(16) char smem[4 * TL::BYTES + 2 * KT * 4 + 32];
   auto sk = [&](int buf) { return smem + buf * TL::BYTES; };
@@ -495,16 +546,14 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void attn_masked_dq_ke
   auto seen = [&](int t, int id) { return t <= lim && id == myid; };
   typename TL::Regs gk, gv;
   int gid = 0;
+  bool dirty = false;
   auto fetch = [&](int t) {
     TL::load(gk, K, p.ks[1], t * KT, p.Sk, p.D);
     TL::load(gv, V, p.vs[1], t * KT, p.Sk, p.D);
     if (p.doc_k && threadIdx.x < KT) gid = t * KT + (int)threadIdx.x < p.Sk ? p.doc_k[hd.b * p.dcs[1] + t * KT + threadIdx.x] : -1;
   };
   auto put = [&](int buf, bool full) {
-    if (!full) {
-      const bool bad = TL::clean(gk);
-      if (lane == 0) sbad[buf * 4 + wave] = bad;
-    }
+    if (!full) dirty |= TL::clean(gk);
     TL::store(sk(buf), gk);
     TL::store(sv(buf), gv);
     if (threadIdx.x < KT) sid[buf * KT + threadIdx.x] = gid;
@@ -573,71 +622,74 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void attn_masked_dq_ke
 #pragma unroll
       for (int d = 0; d < ND; ++d) dq[d] = TL::cols(sk(buf), n * 32, d, pk, s, dq[d]);
     }
-    if (!full && any_flag(sbad + buf * 4)) {
-      const int width = width_here(p);
-      for (int j = 0; j < KT; ++j) {
-        if (!seen(t * KT + j, sid[buf * KT + j])) continue;
-        const T* row = K + (long)(t * KT + j) * p.ks[1];
-#pragma unroll
-        for (int d = 0; d < ND; ++d)
-#pragma unroll
-          for (int r = 0; r < 16; ++r) {
-            const int e = d * 32 + mfma32_row(r, half);
-            if (e < width) {
-              const float x = (float)row[e];
-              if (!(fabsf(x) < __builtin_inff())) dq[d][r] += x;
-            }
-          }
-      }
-    }
     if (tn >= 0) put(buf ^ 1, fulln);
     __syncthreads();
     buf ^= 1;
     t = tn;
     full = fulln;
   }
+  // The seen infinities and NaN that staging left out, if it met any (in a masked tile): once more over the masked tiles
+  if (lane == 0) sbad[wave] = dirty;
+  __syncthreads();
+  if (any_flag<4>(sbad)) {
+    it.init(rk, 0, (max(tend, 0) + KT - 1) / KT, qr.x, qr.y);
+    for (t = it.next(); t >= 0; t = it.next()) {
+      if (whole(t)) continue;
+      __syncthreads();
+      TL::encode(smem, K, p.ks[1], t * KT, p.Sk, p.D);
+      if (threadIdx.x < KT) sid[threadIdx.x] = t * KT + (int)threadIdx.x < p.Sk && p.doc_k ? p.doc_k[hd.b * p.dcs[1] + t * KT + threadIdx.x] : 0;
+      __syncthreads();
+      add_seen<TL, KT>(dq, smem, [&](int j) { return seen(t * KT + j, sid[j]); });
+    }
+  }
   if (!iok) return;
-  const int width = width_here(p);
   T* out = (T*)p.dq + hd.b * p.dqs[0] + (long)i * p.dqs[1] + hd.h * p.dqs[2];
 #pragma unroll
   for (int d = 0; d < ND; ++d)
 #pragma unroll
-    for (int r = 0; r < 16; ++r) {
+    for (int r = 0; r < 16; r += 4) {
       const int e = d * 32 + mfma32_row(r, half);
-      if (e < width) out[e] = (T)(dq[d][r] * p.scale);
+      if (e < p.D) store4(out + e, dq[d][r] * p.scale, dq[d][r + 1] * p.scale, dq[d][r + 2] * p.scale, dq[d][r + 3] * p.scale);
     }
 }
 
 // ---- gradients of the keys and values ----------------------------------------------------------------------------------------------
-template <class T, int DP, int QT>
-__global__ __launch_bounds__(256) void attn_masked_dkv_kernel(MaskP p) {
-  using TL = Tile<T, DP, QT>;
+// Eight waves own 128 keys (four own 64 where a wave of 128 fp32 columns needs all registers), two waves the same 32: the first half form dv (S and one more product a tile), the others dk (S, do.v and
+// one more).  S is formed twice, 40 tile products instead of 32, but a wave then needs 64 accumulators instead of 128 and two waves
+// fit a SIMD, one's exponentials under the other's matrix work: a single wave with both took 978 us where this takes #### (2 x 4096
+// tokens, 16 heads of 128).  Where the key blocks are few, `nsplit` workgroups share the query tiles of one (every nsplit-th tile, so
+// the split is even under a causal mask too); their 32-bit sums are added in order by dkv_join_kernel.
+template <class T, int DP, int QT, int NT>
+__global__ __launch_bounds__(NT, NT / 256) void attn_masked_dkv_kernel(MaskP p) {
+  using TL = Tile<T, DP, QT, NT>;
+  constexpr int NW = NT / 128, KEYS = 32 * NW;                  // waves of either kind; keys of the workgroup
   constexpr int NP = TL::NCH / 2, ND = DP / 32, NS = QT / 32;
-  __shared__ __align__(16) char smem[4 * TL::BYTES + 6 * QT * 4 + 32];      // Q, dO of two tiles; lse, delta, ids; flags of the waves
+  __shared__ __align__(16) char smem[4 * TL::BYTES + 6 * QT * 4 + 64];      // Q, dO of two tiles; lse, delta, ids; flags of the waves
   auto sq = [&](int buf) { return smem + buf * TL::BYTES; };
   auto sd = [&](int buf) { return smem + (2 + buf) * TL::BYTES; };
   float* const slse = (float*)(smem + 4 * TL::BYTES);           // [2][QT]
   float* const sdel = slse + 2 * QT;
   int* const sid = (int*)(sdel + 2 * QT);
-  int* const sbad = sid + 2 * QT;
+  int* const sbad = sid + 2 * QT;                               // [8]
   const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, half = lane >> 5;
-  const int b = blockIdx.x / p.Hk, hk = blockIdx.x - b * p.Hk;
-  const int k0 = blockIdx.y * 128;                               // (causal: the first keys are seen by most queries)
-  const int t = k0 + wave * 32 + (lane & 31);
+  const bool keys = wave >= NW;                                 // this wave forms dk, else dv
+  const int b = blockIdx.x / p.Hk, hk = blockIdx.x - b * p.Hk, split = blockIdx.z;
+  const int k0 = blockIdx.y * KEYS;                               // (causal: the first keys are seen by most queries)
+  const int t = k0 + (wave & (NW - 1)) * 32 + (lane & 31);
   const bool tok = t < p.Sk;
   u32x4 kf[NP], vf[NP];
   own_row<T, NP>(kf, (const T*)p.k + b * p.ks[0] + (long)t * p.ks[1] + hk * p.ks[2], tok, p.D);
-  own_row<T, NP>(vf, (const T*)p.v + b * p.vs[0] + (long)t * p.vs[1] + hk * p.vs[2], tok, p.D);
+  own_row<T, NP>(vf, (const T*)p.v + b * p.vs[0] + (long)t * p.vs[1] + hk * p.vs[2], tok && keys, p.D);
   const int prefix = p.prefix ? p.prefix[b] : 0;
   const int myid = p.doc_k ? (tok ? p.doc_k[b * p.dcs[1] + t] : -1) : 0;
-  const int klast = min(k0 + 127, p.Sk - 1);
+  const int klast = min(k0 + KEYS - 1, p.Sk - 1);
   const int4 *rq = nullptr;
   int4 kr = make_int4(0, 0, 0, 0);
   if (p.doc_q) {
     const int nk = (p.Sk + RG - 1) / RG;
     const int4* rk = p.rk + (long)b * nk + k0 / RG;
     kr = rk[0];
-    if (k0 / RG + 1 < nk) {
+    if (KEYS > RG && k0 / RG + 1 < nk) {
       const int4 x = rk[1];
       kr = make_int4(min(kr.x, x.x), max(kr.y, x.y), kr.z | x.z, 0);
     }
@@ -656,14 +708,15 @@ __global__ __launch_bounds__(256) void attn_masked_dkv_kernel(MaskP p) {
   // the first query that sees this lane's key, documents aside
   const int lim = myid < 0 || !tok ? 0x7fffffff : p.causal && t >= prefix ? t - p.off : 0;
   auto seen = [&](int i, int id) { return i >= lim && i < p.Sq && id == myid; };
-  f32x16 dk[ND], dv[ND];
+  f32x16 acc[ND];
 #pragma unroll
   for (int d = 0; d < ND; ++d)
 #pragma unroll
-    for (int r = 0; r < 16; ++r) { dk[d][r] = 0.f; dv[d][r] = 0.f; }
+    for (int r = 0; r < 16; ++r) acc[d][r] = 0.f;
   typename TL::Regs gq, gd;
   float glse = 0.f, gdel = 0.f;
   int gid = 0;
+  bool dirty = false;
   for (int g = 0; g < p.G; ++g) {
     const int h = hk * p.G + g;
     const T* Q = (const T*)p.q + b * p.qs[0] + h * p.qs[2];
@@ -672,22 +725,22 @@ __global__ __launch_bounds__(256) void attn_masked_dkv_kernel(MaskP p) {
     const float* del = p.delta + ((long)b * p.H + h) * p.Sq;
     const Score sc(p, h);
     Tiles<RG / QT> it;
-    it.init(rq, first, (p.Sq + QT - 1) / QT, kr.x, kr.y);
+    it.init(rq, first, (p.Sq + QT - 1) / QT, kr.x, kr.y, p.nsplit, split);
     auto fetch = [&](int tq) {
       TL::load(gq, Q, p.qs[1], tq * QT, p.Sq, p.D);
       TL::load(gd, DO, p.dos[1], tq * QT, p.Sq, p.D);
       if (threadIdx.x < QT) {
         const int i = tq * QT + threadIdx.x;
         glse = i < p.Sq ? lse[i] : __builtin_inff();
-        if (glse == NEG_INF) glse = __builtin_inff();
+        if (glse == NEG_INF) glse = __builtin_inff();            // sees nothing: every probability is zero
         gdel = i < p.Sq ? del[i] : 0.f;
         gid = p.doc_q ? (i < p.Sq ? p.doc_q[b * p.dcs[0] + i] : -1) : 0;
       }
     };
     auto put = [&](int buf, bool full) {
       if (!full) {
-        const bool x = TL::clean(gq), y = TL::clean(gd), bad = x || y;
-        if (lane == 0) sbad[buf * 4 + wave] = bad;
+        dirty |= TL::clean(gq);
+        dirty |= TL::clean(gd);
       }
       TL::store(sq(buf), gq);
       TL::store(sd(buf), gd);
@@ -712,25 +765,29 @@ __global__ __launch_bounds__(256) void attn_masked_dkv_kernel(MaskP p) {
       for (int n = 0; n < NS; ++n) {
         f32x16 s, dp;
 #pragma unroll
-        for (int r = 0; r < 16; ++r) { s[r] = 0.f; dp[r] = 0.f; }
+        for (int r = 0; r < 16; ++r) s[r] = 0.f;
 #pragma unroll
         for (int c = 0; c < NP; ++c) s = mfma32<T>(TL::rows(sq(buf), n * 32, c), kf[c], s);
-#pragma unroll
-        for (int c = 0; c < NP; ++c) dp = mfma32<T>(TL::rows(sd(buf), n * 32, c), vf[c], dp);
-#pragma unroll
-        for (int r4 = 0; r4 < 4; ++r4) {
-          const f32x4 de = *(const f32x4*)(sdel + buf * QT + n * 32 + 8 * r4 + 4 * half);
-#pragma unroll
-          for (int w = 0; w < 4; ++w) dp[4 * r4 + w] -= de[w];
-        }
         float m0 = sc.mul;
+        if (keys) {
+#pragma unroll
+          for (int r = 0; r < 16; ++r) dp[r] = 0.f;
+#pragma unroll
+          for (int c = 0; c < NP; ++c) dp = mfma32<T>(TL::rows(sd(buf), n * 32, c), vf[c], dp);
+#pragma unroll
+          for (int r4 = 0; r4 < 4; ++r4) {
+            const f32x4 de = *(const f32x4*)(sdel + buf * QT + n * 32 + 8 * r4 + 4 * half);
+#pragma unroll
+            for (int w = 0; w < 4; ++w) dp[4 * r4 + w] -= de[w];
+          }
+        }
         if (sc.capped) {
           m0 = 1.f;
 #pragma unroll
           for (int r = 0; r < 16; ++r) {
             const float th = tanh_from_exp2(s[r] * sc.mul);
             s[r] = sc.cap2 * th;
-            dp[r] *= 1.f - th * th;
+            if (keys) dp[r] *= 1.f - th * th;
           }
         }
         if (p.slopes) {
@@ -743,12 +800,11 @@ __global__ __launch_bounds__(256) void attn_masked_dkv_kernel(MaskP p) {
         for (int r4 = 0; r4 < 4; ++r4) {
           const f32x4 ls = *(const f32x4*)(slse + buf * QT + n * 32 + 8 * r4 + 4 * half);
 #pragma unroll
-          for (int w = 0; w < 4; ++w) {
-            const int r = 4 * r4 + w;
-            s[r] = exp2_hw(__builtin_fmaf(s[r], m0, -ls[w]));
-            dp[r] *= s[r];
-          }
+          for (int w = 0; w < 4; ++w) s[4 * r4 + w] = exp2_hw(__builtin_fmaf(s[4 * r4 + w], m0, -ls[w]));
         }
+        if (keys)
+#pragma unroll
+          for (int r = 0; r < 16; ++r) s[r] *= dp[r];
         if (!full) {
 #pragma unroll
           for (int r4 = 0; r4 < 4; ++r4) {
@@ -756,35 +812,14 @@ __global__ __launch_bounds__(256) void attn_masked_dkv_kernel(MaskP p) {
             const i32x4 id = *(const i32x4*)(sid + buf * QT + j0);
 #pragma unroll
             for (int w = 0; w < 4; ++w)
-              if (j0 + w < lim - tq * QT || id[w] != myid) { s[4 * r4 + w] = 0.f; dp[4 * r4 + w] = 0.f; }
+              if (j0 + w < lim - tq * QT || id[w] != myid) s[4 * r4 + w] = 0.f;
           }
         }
         u32x4 pk[2];
         pack_tile<T>(s, pk);
+        const char* x = keys ? sq(buf) : sd(buf);
 #pragma unroll
-        for (int d = 0; d < ND; ++d) dv[d] = TL::cols(sd(buf), n * 32, d, pk, s, dv[d]);
-        pack_tile<T>(dp, pk);
-#pragma unroll
-        for (int d = 0; d < ND; ++d) dk[d] = TL::cols(sq(buf), n * 32, d, pk, dp, dk[d]);
-      }
-      if (!full && any_flag(sbad + buf * 4)) {
-        const int width = width_here(p);
-        for (int j = 0; j < QT; ++j) {
-          const int i = tq * QT + j;
-          if (!seen(i, sid[buf * QT + j])) continue;
-          const T *r1 = DO + (long)i * p.dos[1], *r2 = Q + (long)i * p.qs[1];
-#pragma unroll
-          for (int d = 0; d < ND; ++d)
-#pragma unroll
-            for (int r = 0; r < 16; ++r) {
-              const int e = d * 32 + mfma32_row(r, half);
-              if (e < width) {
-                const float x = (float)r1[e], y = (float)r2[e];
-                if (!(fabsf(x) < __builtin_inff())) dv[d][r] += x;
-                if (!(fabsf(y) < __builtin_inff())) dk[d][r] += y;
-              }
-            }
-        }
+        for (int d = 0; d < ND; ++d) acc[d] = TL::cols(x, n * 32, d, pk, s, acc[d]);
       }
       if (tn >= 0) put(buf ^ 1, fulln);
       __syncthreads();
@@ -793,20 +828,53 @@ __global__ __launch_bounds__(256) void attn_masked_dkv_kernel(MaskP p) {
       full = fulln;
     }
   }
+  if (lane == 0) sbad[wave] = dirty;
+  __syncthreads();
+  if (any_flag<NT / 64>(sbad)) {                                      // as in the forward kernel, over both sides' rows
+    for (int g = 0; g < p.G; ++g) {
+      const int h = hk * p.G + g;
+      Tiles<RG / QT> it;
+      it.init(rq, first, (p.Sq + QT - 1) / QT, kr.x, kr.y, p.nsplit, split);
+      for (int tq = it.next(); tq >= 0; tq = it.next()) {
+        if (whole(tq)) continue;
+        __syncthreads();
+        TL::encode(sq(0), (const T*)p.q + b * p.qs[0] + h * p.qs[2], p.qs[1], tq * QT, p.Sq, p.D);
+        TL::encode(sd(0), (const T*)p.d_o + b * p.dos[0] + h * p.dos[2], p.dos[1], tq * QT, p.Sq, p.D);
+        if (threadIdx.x < QT) sid[threadIdx.x] = tq * QT + (int)threadIdx.x < p.Sq && p.doc_q ? p.doc_q[b * p.dcs[0] + tq * QT + threadIdx.x] : 0;
+        __syncthreads();
+        add_seen<TL, QT>(acc, keys ? sq(0) : sd(0), [&](int j) { return seen(tq * QT + j, sid[j]); });
+      }
+    }
+  }
   if (!tok) return;
-  const int width = width_here(p);
-  T* ok = (T*)p.dk + b * p.dks[0] + (long)t * p.dks[1] + hk * p.dks[2];
-  T* ov = (T*)p.dv + b * p.dvs[0] + (long)t * p.dvs[1] + hk * p.dvs[2];
+  const float mul = keys ? p.scale : 1.f;
+  const long* st = keys ? p.dks : p.dvs;
+  T* out = (T*)(keys ? p.dk : p.dv) + b * st[0] + (long)t * st[1] + hk * st[2];
+  float* part = p.part + ((((long)split * 2 + keys) * p.B + b) * p.Sk + t) * p.Hk * p.D + (long)hk * p.D;
 #pragma unroll
   for (int d = 0; d < ND; ++d)
 #pragma unroll
-    for (int r = 0; r < 16; ++r) {
+    for (int r = 0; r < 16; r += 4) {
       const int e = d * 32 + mfma32_row(r, half);
-      if (e < width) {
-        ok[e] = (T)(dk[d][r] * p.scale);
-        ov[e] = (T)dv[d][r];
-      }
+      if (e >= p.D) continue;
+      if (p.nsplit == 1) store4(out + e, acc[d][r] * mul, acc[d][r + 1] * mul, acc[d][r + 2] * mul, acc[d][r + 3] * mul);
+      else *(f32x4*)(part + e) = f32x4{acc[d][r], acc[d][r + 1], acc[d][r + 2], acc[d][r + 3]};
     }
+}
+
+// dk, dv = the splits' sums, in order; four elements a thread, dk on blockIdx.y = 1
+template <class T>
+__global__ __launch_bounds__(256) void dkv_join_kernel(MaskP p) {
+  const long n = (long)p.B * p.Sk * p.Hk * p.D, i = ((long)blockIdx.x * 256 + threadIdx.x) * 4;
+  const int keys = blockIdx.y;
+  if (i >= n) return;
+  f32x4 a = *(const f32x4*)(p.part + keys * n + i);
+  for (int s = 1; s < p.nsplit; ++s) a += *(const f32x4*)(p.part + (2L * s + keys) * n + i);
+  const float mul = keys ? p.scale : 1.f;
+  const int d = (int)(i % p.D);
+  const long row = i / p.D, hk = row % p.Hk, bt = row / p.Hk, t = bt % p.Sk, b = bt / p.Sk;
+  const long* st = keys ? p.dks : p.dvs;
+  store4((T*)(keys ? p.dk : p.dv) + b * st[0] + t * st[1] + hk * st[2] + d, a[0] * mul, a[1] * mul, a[2] * mul, a[3] * mul);
 }
 
 // ---- C entries -----------------------------------------------------------------------------------------------------------------------
@@ -843,6 +911,28 @@ template <class F> static void with_tile(int dtype, int D, F&& f) {
   });
 }
 
+// Workgroups that share a key block's query tiles: a power of two, until the 128-key blocks of all key heads fill the chip's 256 CUs
+// twice (one workgroup a CU at a time; two rounds even out a causal mask), never more than there are tiles.  Each split writes and reads
+// 16 bytes a key element more, the backward of 2 x 4096 tokens on 2 x 4 key heads of 128 gains #### over one split.
+static int dkv_split(int B, int Sq, int Sk, int Hk) {
+  const long blocks = (long)B * Hk * ((Sk + 127) / 128);
+  int n = 1;
+  while (n < 16 && blocks * n < 512 && 2 * n <= (Sq + 63) / 64) n *= 2;
+  return n;
+}
+// Floats of scratch the backward pass needs: delta, and the sums of split key blocks
+static long bwd_floats(int B, int Sq, int Sk, int H, int Hk, int D, long* delta) {
+  *delta = ((long)B * H * Sq + 3) / 4 * 4;
+  const int n = dkv_split(B, Sq, Sk, Hk);
+  return *delta + (n > 1 ? 2L * n * B * Sk * Hk * D : 0);
+}
+extern "C" int aot_attn_masked_bwd_floats(int B, int Sq, int Sk, int H, int Hk, int D, long* floats) {
+  if (!floats || B < 0 || Sq < 0 || Sk < 0 || Hk < 1 || H < Hk || H % Hk || D < 1) return AOT_ERR_BADARG;
+  long delta;
+  *floats = bwd_floats(B, Sq, Sk, H, Hk, D, &delta);
+  return AOT_OK;
+}
+
 extern "C" int aot_attn_masked(const void* q, const void* k, const void* v, void* out, float* lse, const float* slopes, const int* doc_q,
                                const int* doc_k, const int* prefix, void* ranges, int dtype, int B, int Sq, int Sk, int H, int Hk, int D,
                                int causal, float scale, float softcap, const long* strides, void* stream) {
@@ -855,7 +945,7 @@ extern "C" int aot_attn_masked(const void* q, const void* k, const void* v, void
   for (int i = 0; i < 3; ++i) { p.qs[i] = strides[i]; p.ks[i] = strides[3 + i]; p.vs[i] = strides[6 + i]; p.os[i] = strides[9 + i]; }
   p.dcs[0] = strides[12]; p.dcs[1] = strides[13];
   const int es = dtype_size(dtype);
-  if (!rows_aligned(q, p.qs, es) || !rows_aligned(k, p.ks, es) || !rows_aligned(v, p.vs, es)) return AOT_ERR_BADARG;
+  if (!rows_aligned(q, p.qs, es) || !rows_aligned(k, p.ks, es) || !rows_aligned(v, p.vs, es) || !rows_aligned(out, p.os, es)) return AOT_ERR_BADARG;
   mask_common(p, B, Sq, Sk, H, Hk, D, causal, scale, softcap, slopes, doc_q, doc_k, prefix, ranges);
   hipStream_t st = (hipStream_t)stream;
   if (doc_q) range_launch(p, st);
@@ -867,16 +957,16 @@ extern "C" int aot_attn_masked(const void* q, const void* k, const void* v, void
 }
 
 extern "C" int aot_attn_masked_bwd(const void* q, const void* k, const void* v, const void* out, const float* lse, const void* dout, void* dq, void* dk,
-                                   void* dv, const float* slopes, const int* doc_q, const int* doc_k, const int* prefix, void* ranges, float* delta,
+                                   void* dv, const float* slopes, const int* doc_q, const int* doc_k, const int* prefix, void* ranges, float* work, long work_floats,
                                    int dtype, int B, int Sq, int Sk, int H, int Hk, int D, int causal, float scale, float softcap, const long* strides,
                                    void* stream) {
   int rc = mask_args(dtype, B, Sq, Sk, H, Hk, D, softcap, doc_q, doc_k, ranges, strides);
   if (rc) return rc;
   if (B == 0 || (Sq == 0 && Sk == 0)) return AOT_OK;
-  if ((Sq && (!q || !out || !lse || !dout || !dq || !delta)) || (Sk && (!k || !v || !dk || !dv))) return AOT_ERR_BADARG;
+  if ((Sq && (!q || !out || !lse || !dout || !dq)) || (Sk && (!k || !v || !dk || !dv))) return AOT_ERR_BADARG;
   MaskP p{};
   p.q = (const char*)q; p.k = (const char*)k; p.v = (const char*)v; p.o = (const char*)out; p.d_o = (const char*)dout;
-  p.lse = (float*)lse; p.delta = delta; p.dq = (char*)dq; p.dk = (char*)dk; p.dv = (char*)dv;
+  p.lse = (float*)lse; p.dq = (char*)dq; p.dk = (char*)dk; p.dv = (char*)dv;
   for (int i = 0; i < 3; ++i) {
     p.qs[i] = strides[i]; p.ks[i] = strides[3 + i]; p.vs[i] = strides[6 + i]; p.os[i] = strides[9 + i]; p.dos[i] = strides[12 + i];
     p.dqs[i] = strides[15 + i]; p.dks[i] = strides[18 + i]; p.dvs[i] = strides[21 + i];
@@ -884,13 +974,25 @@ extern "C" int aot_attn_masked_bwd(const void* q, const void* k, const void* v, 
   p.dcs[0] = strides[24]; p.dcs[1] = strides[25];
   const int es = dtype_size(dtype);
   if (!rows_aligned(q, p.qs, es) || !rows_aligned(k, p.ks, es) || !rows_aligned(v, p.vs, es) || !rows_aligned(out, p.os, es) ||
-      !rows_aligned(dout, p.dos, es)) return AOT_ERR_BADARG;
+      !rows_aligned(dout, p.dos, es) || !rows_aligned(dq, p.dqs, es) || !rows_aligned(dk, p.dks, es) || !rows_aligned(dv, p.dvs, es) ||
+      !aligned16(work)) return AOT_ERR_BADARG;
+  long delta;
+  if (!work || work_floats < bwd_floats(B, Sq, Sk, H, Hk, D, &delta)) return AOT_ERR_BADARG;
+  p.delta = work;
+  p.part = work + delta;
+  p.nsplit = dkv_split(B, Sq, Sk, Hk);
   mask_common(p, B, Sq, Sk, H, Hk, D, causal, scale, softcap, slopes, doc_q, doc_k, prefix, ranges);
   hipStream_t st = (hipStream_t)stream;
   if (doc_q) range_launch(p, st);
   with_tile(dtype, D, [&](auto t, auto dp, auto kt) {
-    if (Sq) hipLaunchKernelGGL((attn_masked_dq_kernel<decltype(t), decltype(dp)::value, decltype(kt)::value>), dim3(B * H, cdiv(Sq, 128)), dim3(256), 0, st, p);
-    if (Sk) hipLaunchKernelGGL((attn_masked_dkv_kernel<decltype(t), decltype(dp)::value, decltype(kt)::value>), dim3(B * Hk, cdiv(Sk, 128)), dim3(256), 0, st, p);
+    constexpr int KT = decltype(dp)::value == 128 ? 32 : 64;     // (two 64-row tiles of 128 columns in flight cost spills here)
+    if (Sq) hipLaunchKernelGGL((attn_masked_dq_kernel<decltype(t), decltype(dp)::value, KT>), dim3(B * H, cdiv(Sq, 128)), dim3(256), 0, st, p);
+    if (Sk) {
+      constexpr int NT = sizeof(t) == 4 && decltype(dp)::value == 128 ? 256 : 512;
+      hipLaunchKernelGGL((attn_masked_dkv_kernel<decltype(t), decltype(dp)::value, decltype(kt)::value, NT>), dim3(B * Hk, cdiv(Sk, NT / 4), p.nsplit),
+                         dim3(NT), 0, st, p);
+      if (p.nsplit > 1) hipLaunchKernelGGL((dkv_join_kernel<decltype(t)>), dim3(cdiv((long)B * Sk * Hk * D, 1024), 2), dim3(256), 0, st, p);
+    }
   });
   AOT_LAUNCH_CHECK();
 }

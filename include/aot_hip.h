@@ -548,13 +548,14 @@ int aot_attn_masked(const void* q, const void* k, const void* v, void* out, floa
                     const int* doc_k, const int* prefix, void* ranges, int dtype, int B, int Sq, int Sk, int H, int Hk, int D,
                     int causal, float scale, float softcap, const long* strides, void* stream);
 /* Its gradients: out and lse from the forward call on the same arguments, dout -> dq, dk, dv (key heads: summed over the query heads
- * that share them); delta: scratch of B * H * Sq floats.  Probabilities and score gradients are rounded to `dtype` for the products they
+ * that share them); work: scratch of aot_attn_masked_bwd_floats floats, 16-byte aligned.  Probabilities and score gradients are rounded to `dtype` for the products they
  * enter (fp16: what is below 6e-8 is lost, as in any fp16 gradient -- scale the loss).  No atomics: results repeat bit for bit.
  * strides: q k v out dout dq dk dv (b s h each), doc_q b, doc_k b (26). */
 int aot_attn_masked_bwd(const void* q, const void* k, const void* v, const void* out, const float* lse, const void* dout, void* dq, void* dk,
-                        void* dv, const float* slopes, const int* doc_q, const int* doc_k, const int* prefix, void* ranges, float* delta,
+                        void* dv, const float* slopes, const int* doc_q, const int* doc_k, const int* prefix, void* ranges, float* work, long work_floats,
                         int dtype, int B, int Sq, int Sk, int H, int Hk, int D, int causal, float scale, float softcap, const long* strides,
                         void* stream);
+int aot_attn_masked_bwd_floats(int B, int Sq, int Sk, int H, int Hk, int D, long* floats);
 
 /* Attention of ONE new token per sequence over a paged cache: q / out [B, H, D]; entry t < lengths[b] of sequence b lies at place t % page
  * of page table[b, t / page] (max_pages a row) of k_pages / v_pages.  The new token's own key and value are already in the cache (entry

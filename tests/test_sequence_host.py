@@ -42,10 +42,10 @@ def test_c_entries_refuse_before_any_launch():
     assert masked(D=132) == -2 and masked(D=33) == -2 and masked(dtype=1, D=36) == -2 and masked(Sk=(1 << 22) + 1) == -2
     assert masked(B=0) == 0 and masked(Sq=0, q=None) == 0
 
-    def bwd(Sq=1, Sk=1, dk=P(16), delta=P(16), do=P(16), st=z26, D=32):
-        return lib.aot_attn_masked_bwd(P(16), P(16), P(16), P(16), P(16), do, P(16), dk, P(16), None, None, None, None, None, delta, 2, 1, Sq, Sk, 1, 1, D, 0,
+    def bwd(Sq=1, Sk=1, dk=P(16), delta=P(16), do=P(16), st=z26, D=32, floats=1 << 20):
+        return lib.aot_attn_masked_bwd(P(16), P(16), P(16), P(16), P(16), do, P(16), dk, P(16), None, None, None, None, None, delta, floats, 2, 1, Sq, Sk, 1, 1, D, 0,
                                        1.0, 0.0, st, None)
-    assert bwd(dk=None) == -1 and bwd(delta=None) == -1 and bwd(do=P(18)) == -1 and bwd(st=None) == -1 and bwd(D=136) == -2
+    assert bwd(floats=3) == -1 and bwd(delta=P(20)) == -1 and bwd(dk=P(24)) == -1 and bwd(dk=None) == -1 and bwd(delta=None) == -1 and bwd(do=P(18)) == -1 and bwd(st=None) == -1 and bwd(D=136) == -2
     assert bwd(Sq=0, Sk=0, dk=None) == 0
 
     def paged(dtype=0, B=1, H=1, Hk=1, D=32, page=16, mp=1, pages=4, cap=0.0, q=P(16), kp=P(16), work=None, floats=0, w=None, st=z15, table=P(16)):
