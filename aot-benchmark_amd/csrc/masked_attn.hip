@@ -300,7 +300,7 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void attn_masked_fwd_k
   auto sv = [&](int buf) { return smem + (2 + buf) * TL::BYTES; };
   int* const sid = (int*)(smem + 4 * TL::BYTES);                // [2][KT]
   int* const sbad = sid + 2 * KT;                               // [4]
-  const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, half = lane >> 5;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, half = lane >> 5;
   const Head hd = head_of(blockIdx.x, p);
   const int q0 = (p.causal ? gridDim.y - 1 - blockIdx.y : blockIdx.y) * 128;      // the long rows of a causal mask first
   const int i = q0 + wave * 32 + (lane & 31);
@@ -482,7 +482,7 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void attn_masked_dq_ke
   auto sv = [&](int buf) { return smem + (2 + buf) * TL::BYTES; };
   int* const sid = (int*)(smem + 4 * TL::BYTES);
   int* const sbad = sid + 2 * KT;
-  const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, half = lane >> 5;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, half = lane >> 5;
   const Head hd = head_of(blockIdx.x, p);
   const int q0 = (p.causal ? gridDim.y - 1 - blockIdx.y : blockIdx.y) * 128;
   const int i = q0 + wave * 32 + (lane & 31);
@@ -671,7 +671,7 @@ __global__ __launch_bounds__(NT, NT / 256) void attn_masked_dkv_kernel(MaskP p) 
   float* const sdel = slse + 2 * QT;
   int* const sid = (int*)(sdel + 2 * QT);
   int* const sbad = sid + 2 * QT;                               // [8]
-  const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, half = lane >> 5;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, half = lane >> 5;
   const bool keys = wave >= NW;                                 // this wave forms dk, else dv
   const int b = blockIdx.x / p.Hk, hk = blockIdx.x - b * p.Hk, split = blockIdx.z;
   const int k0 = blockIdx.y * KEYS;                               // (causal: the first keys are seen by most queries)
