@@ -55,7 +55,7 @@ __global__ __launch_bounds__(256) void paged_attn_kernel(PagedP p) {
   constexpr int PW = EW < 4 ? EW : 4;                                                       // PW of them a load
   __shared__ float sm[4][16], sl[4][16];
   __shared__ float so[2][16][DP + 4];
-  const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, n = lane & 15, kg = lane >> 4;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, n = lane & 15, kg = lane >> 4;
   const int qt = blockIdx.y / p.Hk, hk = blockIdx.y - qt * p.Hk, b = blockIdx.z, split = blockIdx.x;
   const int len = max(0, min(p.lengths[b], p.cap_len));
   const int t_begin = split * p.chunk, t_end = min(len, t_begin + p.chunk);
@@ -85,33 +85,82 @@ __global__ __launch_bounds__(256) void paged_attn_kernel(PagedP p) {
   for (int e = 0; e < E; ++e) o[e] = f32x4{0.f, 0.f, 0.f, 0.f};
   float m = NEG_INF, l = 0.f;
 
-  for (int t0 = t_begin + wave * 32; t0 < t_end; t0 += 128) {
-    u32x4 kf[2][NC];
+  // A block's pages: one lookup for each half of 16 entries, wave-uniform; -1 where a lane-wise look at every entry is needed
+  const bool coarse = p.page_shift >= 4;
+  struct Pages { int a, b; };
+  auto pages_of = [&](int t0) {
+    Pages r{-1, -1};
+    if (coarse && t0 + 32 <= len) {
+      r.a = __builtin_amdgcn_readfirstlane(table[t0 >> p.page_shift]);
+      r.b = __builtin_amdgcn_readfirstlane(table[(t0 + 16) >> p.page_shift]);
+      if (r.a >= p.num_pages || r.b >= p.num_pages) r.a = -1;
+      if (r.b < 0) r.a = -1;
+    }
+    return r;
+  };
+  struct Block { u32x4 kf[2][NC]; unsigned vf[8][EW]; unsigned ok; };
+  const long in_mask = (1 << p.page_shift) - 1;
+  const long k_lane = n * p.ks[1], v_lane = 4 * kg * p.vs[1];
+  auto load = [&](Block& x, int t0, const Pages& pg) {
+    if (pg.a >= 0) {
+      x.ok = 255;
+#pragma unroll
+      for (int T2 = 0; T2 < 2; ++T2) {
+        const long page = T2 ? pg.b : pg.a, in = (t0 + 16 * T2) & in_mask;
+        const T* kb = (const T*)p.k + page * p.ks[0] + in * p.ks[1] + hk * p.ks[2];
+        const T* vb = (const T*)p.v + page * p.vs[0] + in * p.vs[1] + hk * p.vs[2];
+#pragma unroll
+        for (int c = 0; c < NC; ++c) {
+          const int d = (c * 4 + kg) * CE;
+          x.kf[T2][c] = d < p.D ? *(const u32x4*)(kb + k_lane + d) : u32x4{0, 0, 0, 0};
+        }
+#pragma unroll
+        for (int r = 0; r < 4; ++r)
+#pragma unroll
+          for (int i = 0; i < EW / PW; ++i) {
+            typedef unsigned piece __attribute__((ext_vector_type(PW)));
+            const int d = n * E + i * PW * 4 / (int)sizeof(T);
+            piece y = {};
+            if (d < p.D) y = *(const piece*)(vb + r * p.vs[1] + v_lane + d);
+#pragma unroll
+            for (int w = 0; w < PW; ++w) x.vf[4 * T2 + r][i * PW + w] = y[w];
+          }
+      }
+      return;
+    }
+    x.ok = 0;
 #pragma unroll
     for (int T2 = 0; T2 < 2; ++T2) {
       const T* row = entry<T>(p.k, p.ks, table, t0 + T2 * 16 + n, len, hk, p);
 #pragma unroll
       for (int c = 0; c < NC; ++c) {
         const int d = (c * 4 + kg) * CE;
-        kf[T2][c] = row && d < p.D ? *(const u32x4*)(row + d) : u32x4{0, 0, 0, 0};
+        x.kf[T2][c] = row && d < p.D ? *(const u32x4*)(row + d) : u32x4{0, 0, 0, 0};
       }
     }
-    unsigned vf[8][EW];
-    bool ok[8];
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
       const T* row = entry<T>(p.v, p.vs, table, t0 + (j >> 2) * 16 + kg * 4 + (j & 3), len, hk, p);
-      ok[j] = row != nullptr;
+      x.ok |= (row != nullptr) << j;
 #pragma unroll
       for (int i = 0; i < EW / PW; ++i) {                       // (D is whole 16-byte pieces: none is cut)
         typedef unsigned piece __attribute__((ext_vector_type(PW)));
         const int d = n * E + i * PW * 4 / (int)sizeof(T);
-        piece x = {};
-        if (ok[j] && d < p.D) x = *(const piece*)(row + d);
+        piece y = {};
+        if (row && d < p.D) y = *(const piece*)(row + d);
 #pragma unroll
-        for (int w = 0; w < PW; ++w) vf[j][i * PW + w] = x[w];
+        for (int w = 0; w < PW; ++w) x.vf[j][i * PW + w] = y[w];
       }
     }
+  };
+  Block blk;
+  const int t_first = t_begin + wave * 32;
+  Pages pg = t_first < t_end ? pages_of(t_first) : Pages{-1, -1};
+  for (int t0 = t_first; t0 < t_end; t0 += 128) {
+    load(blk, t0, pg);
+    if (t0 + 128 < t_end) pg = pages_of(t0 + 128);
+    auto& kf = blk.kf;
+    auto& vf = blk.vf;
     f32x4 s[2];
 #pragma unroll
     for (int T2 = 0; T2 < 2; ++T2) {
@@ -125,8 +174,8 @@ __global__ __launch_bounds__(256) void paged_attn_kernel(PagedP p) {
       const int t = t0 + (j >> 2) * 16 + kg * 4 + (j & 3);
       float y = s[j >> 2][j & 3] * mul;
       if (capped) y = cap2 * tanh_from_exp2(y);
-      if (p.slopes) y -= slope * fabsf((float)(qpos - (kpos ? (ok[j] ? kpos[t] : 0) : t)));
-      x[j] = ok[j] ? y : NEG_INF;
+      if (p.slopes) y -= slope * fabsf((float)(qpos - (kpos ? (blk.ok >> j & 1 ? kpos[t] : 0) : t)));
+      x[j] = blk.ok >> j & 1 ? y : NEG_INF;
       mx = fmaxf(mx, x[j]);
     }
     if (p.weights) {
