@@ -50,7 +50,7 @@ template <class T> __device__ __forceinline__ const T* entry(const char* pages, 
 }
 
 template <class T, int DP, bool SPLIT>
-__global__ __launch_bounds__(256) void paged_attn_kernel(PagedP p) {
+__global__ __launch_bounds__(256, sizeof(T) == 2 ? (DP == 128 ? 3 : DP == 256 ? 2 : 1) : DP == 128 ? 2 : 1) void paged_attn_kernel(PagedP p) {
   constexpr int CE = Elem<T>::CE, NC = DP / (4 * CE), E = DP / 16, EW = E * sizeof(T) / 4;   // EW dwords of a row a lane holds,
   constexpr int PW = EW < 4 ? EW : 4;                                                       // PW of them a load
   __shared__ float sm[4][16], sl[4][16];
@@ -277,24 +277,30 @@ __global__ __launch_bounds__(256) void paged_attn_kernel(PagedP p) {
   }
 }
 
-// First B * H workgroups: out = sum over the splits, in index order.  The others: weights += group sum of exp2(s - M) / L, one
-// thread an entry; every workgroup forms (M, L) of its heads from the splits' pairs itself.
+// First B * H workgroups: out = sum over the splits; thread groups of D / 4 take every so-many-th split, their sums are added in a fixed
+// order.  The others: weights += group sum of exp2(s - M) / L for 1024 entries of one key head, four a thread; every one forms (M, L) of its
+// heads from the splits' pairs, a wave a head.
+static constexpr int JOIN_KEYS = 1024;
 template <class T>
 __global__ __launch_bounds__(256) void paged_join_kernel(PagedP p) {
-  __shared__ float red[4];
   __shared__ float fac[1024];
-  const int tid = threadIdx.x;
-  auto total = [&](const float* ml, int ns, float& M, float& L) {       // whole workgroup; ns <= 1024
-    float m = NEG_INF;
+  __shared__ float red[8];
+  __shared__ f32x4 sum[256];
+  const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63;
+  const long nout = (long)p.B * p.H;
+  auto live_sum = [](float l) { return l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l); };      // no entry: zero; a NaN stays one
+  if (blockIdx.x < nout) {
+    const int b = blockIdx.x / p.H, h = blockIdx.x - b * p.H;
+    const int len = max(0, min(p.lengths[b], p.cap_len)), ns = (len + p.chunk - 1) / p.chunk;
+    const long at = ((long)b * p.H + h) * p.nsplit;
+    const float* ml = p.ml + at * 2;
+    float m = NEG_INF, l = 0.f;
     for (int i = tid; i < ns; i += 256) m = fmaxf(m, ml[2 * i]);
 #pragma unroll
     for (int d = 1; d < 64; d <<= 1) m = fmaxf(m, __shfl_xor(m, d));
+    if (lane == 0) red[wave] = m;
     __syncthreads();
-    if ((tid & 63) == 0) red[tid >> 6] = m;
-    __syncthreads();
-    M = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
-    const float mb = M == NEG_INF ? 0.f : M;
-    float l = 0.f;
+    const float M = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3])), mb = M == NEG_INF ? 0.f : M;
     for (int i = tid; i < ns; i += 256) {
       const float f = exp2_hw(ml[2 * i] - mb);
       fac[i] = f;
@@ -302,42 +308,63 @@ __global__ __launch_bounds__(256) void paged_join_kernel(PagedP p) {
     }
 #pragma unroll
     for (int d = 1; d < 64; d <<= 1) l += __shfl_xor(l, d);
+    if (lane == 0) red[4 + wave] = l;
     __syncthreads();
-    if ((tid & 63) == 0) red[tid >> 6] = l;
+    const float inv = live_sum(red[4] + red[5] + red[6] + red[7]);
+    const int nd = p.D / 4, groups = 256 / nd, g = tid / nd, d = (tid - g * nd) * 4;       // D is a multiple of 4, at most 256
+    f32x4 a{0.f, 0.f, 0.f, 0.f};
+    if (g < groups) {
+#pragma unroll 4
+      for (int i = g; i < ns; i += groups) a += *(const f32x4*)(p.part + (at + i) * p.D + d) * fac[i];
+      sum[tid] = a;
+    }
     __syncthreads();
-    L = red[0] + red[1] + red[2] + red[3];
-  };
-  const long nout = (long)p.B * p.H;
-  if (blockIdx.x < nout) {
-    const int b = blockIdx.x / p.H, h = blockIdx.x - b * p.H;
-    const int len = max(0, min(p.lengths[b], p.cap_len)), ns = (len + p.chunk - 1) / p.chunk;
-    float M, L;
-    const long at = ((long)b * p.H + h) * p.nsplit;
-    total(p.ml + at * 2, ns, M, L);
-    const float inv = L > 0.f ? 1.f / L : (L == 0.f ? 0.f : L);
-    T* out = (T*)p.out + b * p.os[0] + h * p.os[1];
-    for (int d = tid; d < p.D; d += 256) {
-      float a = 0.f;
-      for (int i = 0; i < ns; ++i) a += p.part[(at + i) * p.D + d] * fac[i];
-      out[d] = (T)(a * inv);
+    if (g == 0) {
+      for (int i = 1; i < groups; ++i) a += sum[i * nd + tid];
+      T* out = (T*)p.out + b * p.os[0] + h * p.os[1] + d;
+#pragma unroll
+      for (int w = 0; w < 4; ++w) out[w] = (T)(a[w] * inv);
     }
     return;
   }
   const long w = blockIdx.x - nout;
-  const int tiles = (p.cap_len + 255) / 256;
+  const int tiles = (p.cap_len + JOIN_KEYS - 1) / JOIN_KEYS;
   const int tile = (int)(w % tiles), bh = (int)(w / tiles), b = bh / p.Hk, hk = bh - b * p.Hk;
   const int len = max(0, min(p.lengths[b], p.cap_len)), ns = (len + p.chunk - 1) / p.chunk;
-  if (tile * 256 >= len) return;
-  const int t = tile * 256 + tid;
-  float acc = 0.f;
-  for (int g = 0; g < p.G; ++g) {
-    const long at = (long)b * p.H + hk * p.G + g;
-    float M, L;
-    total(p.ml + at * p.nsplit * 2, ns, M, L);
-    const float inv = L > 0.f ? 1.f / L : (L == 0.f ? 0.f : L), mb = M == NEG_INF ? 0.f : M;
-    if (t < len) acc += exp2_hw(p.scores[at * p.S + t] - mb) * inv;
+  const int t0 = tile * JOIN_KEYS;
+  if (t0 >= len) return;
+  float acc[4] = {0.f, 0.f, 0.f, 0.f};
+  for (int g0 = 0; g0 < p.G; g0 += 4) {
+    const int n = min(4, p.G - g0);
+    if (wave < n) {
+      const float* ml = p.ml + ((long)b * p.H + hk * p.G + g0 + wave) * p.nsplit * 2;
+      float m = NEG_INF, l = 0.f;
+      for (int i = lane; i < ns; i += 64) m = fmaxf(m, ml[2 * i]);
+#pragma unroll
+      for (int d = 1; d < 64; d <<= 1) m = fmaxf(m, __shfl_xor(m, d));
+      const float mb = m == NEG_INF ? 0.f : m;
+      for (int i = lane; i < ns; i += 64) l += ml[2 * i + 1] * exp2_hw(ml[2 * i] - mb);
+#pragma unroll
+      for (int d = 1; d < 64; d <<= 1) l += __shfl_xor(l, d);
+      if (lane == 0) { red[wave] = mb; red[4 + wave] = live_sum(l); }
+    }
+    __syncthreads();
+    for (int i = 0; i < n; ++i) {
+      const float* sc = p.scores + ((long)b * p.H + hk * p.G + g0 + i) * p.S;
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        const int t = t0 + tid + 256 * k;
+        if (t < len) acc[k] += exp2_hw(sc[t] - red[i]) * red[4 + i];
+      }
+    }
+    __syncthreads();
   }
-  if (t < len) p.weights[b * p.ws[0] + hk * p.ws[1] + t] += acc;
+  float* out = p.weights + b * p.ws[0] + hk * p.ws[1];
+#pragma unroll
+  for (int k = 0; k < 4; ++k) {
+    const int t = t0 + tid + 256 * k;
+    if (t < len) out[t] += acc[k];
+  }
 }
 
 static int pow2_at_least(long x) {
@@ -417,7 +444,7 @@ extern "C" int aot_paged_attn(const void* q, const void* k_pages, const void* v_
   hipError_t e = hipGetLastError();
   if (e != hipSuccess) return (int)e;
   if (split) {
-    const long blocks = (long)B * H + (weights ? (long)B * Hk * ((cap + 255) / 256) : 0);
+    const long blocks = (long)B * H + (weights ? (long)B * Hk * ((cap + JOIN_KEYS - 1) / JOIN_KEYS) : 0);
     if (blocks > 0x7fffffffL) return AOT_ERR_UNSUPPORTED;
     with_dtype(dtype, [&](auto t) { hipLaunchKernelGGL((paged_join_kernel<decltype(t)>), dim3((unsigned)blocks), dim3(256), 0, st, p); });
   }

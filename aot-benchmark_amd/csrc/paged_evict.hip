@@ -2,9 +2,9 @@
 // first `sink`, the last `recent`, and of the others the heaviest, ties to the lower index; NaN weights count as the lightest.  The
 // kept entries move, in order, into the pages of new_table, so pages that other sequences share stay as they are.
 //
-// Two launches.  Select: one workgroup a row; a radix select (four 8-bit digits of an order-preserving key, histograms in shared
-// memory) finds the weight of the last entry that stays, one block scan turns the kept flags into places.  It is bound by reading
-// the weights (from L2 after the first digit) and by the scan's latency.  Move: 16-byte pieces of the kept K / V rows, bound by
+// Two launches.  Select: one workgroup a row; a radix select (three digits of an order-preserving key, histograms in shared memory) finds
+// the weight of the last entry that stays, ballots turn the kept flags into places.  It is bound by reading the weights (five times, from
+// L2 after the first) and by latency.  Move: 16-byte pieces of the kept K / V rows, bound by
 // memory: each kept row is read once and written once.
 #include "seq_common.h"
 
@@ -52,12 +52,13 @@ __device__ __forceinline__ int block_scan(int x, int* lds, int* sum) {
 }
 
 __global__ __launch_bounds__(SEL_T) void evict_select_kernel(EvictP p) {
-  __shared__ int hist[256];
+  __shared__ int hist[2048];
   __shared__ int scan[SEL_T / 64];
   __shared__ int pick[2];
-  const int h = blockIdx.x, b = blockIdx.y, tid = threadIdx.x;
-  int len = p.lengths[b];
-  len = max(0, min(len, p.cap));
+  __shared__ int counts[SEL_T / 64][2];
+  const int h = blockIdx.x, b = blockIdx.y, tid = threadIdx.x, lane = tid & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int len = max(0, min(p.lengths[b], p.cap));
   const float* w = p.weights + b * p.ws[0] + h * p.ws[1];
   int* kept = p.kept + ((long)b * p.Hk + h) * p.budget;
   const int keep = min(len, p.budget);
@@ -67,35 +68,30 @@ __global__ __launch_bounds__(SEL_T) void evict_select_kernel(EvictP p) {
   int ties = 0;                                                             // of the entries equal to thr the first `ties` stay
   const bool all = keep == len;
   if (!all && want > 0) {
+    // Digits of 11, 11 and 10 bits: the first holds sign, exponent and two mantissa bits, so that weights of one magnitude still spread over
+    // several counters (with 8 bits a wave's 64 additions met in one or two and queued: 41 us for 128 rows of 16384, now ####)
     unsigned prefix = 0;
     int left = want;
-    for (int shift = 24; shift >= 0; shift -= 8) {
-      for (int i = tid; i < 256; i += SEL_T) hist[i] = 0;
+#pragma unroll 1
+    for (int d = 0; d < 3; ++d) {
+      const int shift = d == 0 ? 21 : d == 1 ? 10 : 0;
+      const unsigned digit = d == 2 ? 1023u : 2047u, above = d == 0 ? 0u : d == 1 ? ~0u << 21 : ~0u << 10;
+      hist[tid] = 0;
+      hist[tid + SEL_T] = 0;
       __syncthreads();
-      const unsigned mask = shift == 24 ? 0u : ~0u << (shift + 8);
+#pragma unroll 4
       for (int t = lo + tid; t < hi; t += SEL_T) {
         const unsigned key = weight_key(w[t]);
-        if ((key & mask) == prefix) atomicAdd(&hist[(key >> shift) & 255], 1);
+        if ((key & above) == prefix) atomicAdd(&hist[(key >> shift) & digit], 1);
       }
       __syncthreads();
-      if (tid < 64) {                                                       // from the heaviest digit down: where does `left` run out
-        int c[4], s = 0;
-#pragma unroll
-        for (int i = 0; i < 4; ++i) { c[i] = hist[255 - 4 * tid - i]; s += c[i]; }
-        int inc = s;
-#pragma unroll
-        for (int d = 1; d < 64; d <<= 1) {
-          const int y = __shfl_up(inc, d);
-          if (tid >= d) inc += y;
-        }
-        int before = inc - s;
-        if (before < left && inc >= left) {
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            if (before < left && before + c[i] >= left) { pick[0] = 255 - 4 * tid - i; pick[1] = left - before; }
-            before += c[i];
-          }
-        }
+      const int c1 = hist[2047 - 2 * tid], c0 = hist[2046 - 2 * tid];       // from the heaviest digit down: where does `left` run out
+      int sum;
+      const int before = block_scan(c1 + c0, scan, &sum);
+      if (before < left && before + c1 + c0 >= left) {
+        const bool first = before + c1 >= left;
+        pick[0] = first ? 2047 - 2 * tid : 2046 - 2 * tid;
+        pick[1] = first ? left - before : left - before - c1;
       }
       __syncthreads();
       prefix |= (unsigned)pick[0] << shift;
@@ -105,38 +101,49 @@ __global__ __launch_bounds__(SEL_T) void evict_select_kernel(EvictP p) {
     thr = prefix;
     ties = left;
   }
-  // a thread owns a run of entries: count, scan, write
-  const int per = (len + SEL_T - 1) / SEL_T, t0 = min(tid * per, len), t1 = min(t0 + per, len);
+  // a wave owns a run of entries: count, exchange the counts, then place the kept ones by ballots
+  const int per = ((len + SEL_T - 1) / SEL_T) * 64, t0 = min(wave * per, len), t1 = min(t0 + per, len);
+  const unsigned long long below = (1ull << lane) - 1;
+  auto kind = [&](int t, float x, bool& sure, bool& tie) {
+    const unsigned key = weight_key(x);
+    const bool mid = !all && t >= lo && t < hi;
+    sure = t < t1 && (!mid || (want > 0 && key > thr));
+    tie = t < t1 && mid && want > 0 && key == thr;
+  };
   int heavier = 0, equal = 0;
-  for (int t = t0; t < t1; ++t) {
-    if (all || t < lo || t >= hi) ++heavier;
-    else if (want > 0) {
-      const unsigned key = weight_key(w[t]);
-      heavier += key > thr;
-      equal += key == thr;
-    }
+#pragma unroll 4
+  for (int t = t0 + lane; t < t0 + per; t += 64) {
+    bool sure, tie;
+    kind(t, t < t1 ? w[t] : 0.f, sure, tie);
+    heavier += __popcll(__ballot(sure));
+    equal += __popcll(__ballot(tie));
   }
-  int sum;
-  int eq0 = block_scan(equal, scan, &sum);
-  const int mine = heavier + max(0, min(equal, ties - eq0));
-  int at = block_scan(mine, scan, &sum);
+  if (lane == 0) { counts[wave][0] = heavier; counts[wave][1] = equal; }
+  __syncthreads();
+  int at = 0, eq = 0;
+  for (int i = 0; i < wave; ++i) {
+    at += counts[i][0] + max(0, min(counts[i][1], ties - eq));
+    eq += counts[i][1];
+  }
   float* nw = p.new_weights + b * p.nws[0] + h * p.nws[1];
   const int* pos = p.pos ? p.pos + b * p.pss[0] + h * p.pss[1] : nullptr;
   int* np = p.pos ? p.new_pos + b * p.nps[0] + h * p.nps[1] : nullptr;
-  for (int t = t0; t < t1; ++t) {
-    bool stay = all || t < lo || t >= hi;
-    const float x = w[t];
-    if (!stay && want > 0) {
-      const unsigned key = weight_key(x);
-      stay = key > thr;
-      if (key == thr) stay = eq0++ < ties;
-    }
+#pragma unroll 4
+  for (int t = t0 + lane; t < t0 + per; t += 64) {
+    const float x = t < t1 ? w[t] : 0.f;
+    bool sure, tie;
+    kind(t, x, sure, tie);
+    const unsigned long long teq = __ballot(tie);
+    const bool stay = sure || (tie && eq + __popcll(teq & below) < ties);
+    const unsigned long long go = __ballot(stay);
     if (stay) {
-      kept[at] = t;
-      nw[at] = x;
-      if (pos) np[at] = pos[t];
-      ++at;
+      const int j = at + __popcll(go & below);
+      kept[j] = t;
+      nw[j] = x;
+      if (pos) np[j] = pos[t];
     }
+    at += __popcll(go);
+    eq += __popcll(teq);
   }
   for (int i = keep + tid; i < p.budget; i += SEL_T) kept[i] = -1;
   for (int i = keep + tid; i < p.S; i += SEL_T) {
