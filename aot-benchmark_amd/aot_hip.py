@@ -1043,58 +1043,49 @@ def _need(ok, what, *args):
         raise AotHipError(what % args)
 
 
-class _OnDevice:
-    """The launch runs on the tensors' device, whichever is current, on that device's current stream."""
-
-    def __init__(self, *tensors):
-        dev = None
-        for t in tensors:
-            if t is None:
-                continue
-            if not t.is_cuda:
-                raise AotHipError('AOT HIP ops need ROCm device tensors (got %s); there is no CPU fallback' % t.device)
-            if dev is None:
-                dev = t.get_device()
-            elif t.get_device() != dev:
-                raise AotHipError('tensors on different devices: cuda:%d and cuda:%d' % (dev, t.get_device()))
-        self.dev = dev
-
-    def __enter__(self):
-        self.prev = torch.cuda.current_device()
-        if self.prev != self.dev:
-            torch.cuda.set_device(self.dev)
-        return torch._C._cuda_getCurrentRawStream(self.dev)
-
-    def __exit__(self, *exc):
-        if self.prev != self.dev:
-            torch.cuda.set_device(self.prev)
-        return False
+def _device_of(first, *tensors):
+    """The one device of all tensors (the launch runs there, on that device's current stream, whichever device is current)."""
+    dev = first.get_device()
+    for t in tensors:
+        if t is not None and t.get_device() != dev:
+            raise AotHipError('tensors on different devices: %s and %s' % (first.device, t.device))
+    if dev < 0:
+        raise AotHipError('AOT HIP ops need ROCm device tensors (got %s); there is no CPU fallback' % first.device)
+    return dev
 
 
-def _longs(*tensors):
-    """Host array of the leading dimensions' element strides (0 where a dimension has one place, whatever torch says there)."""
-    out = []
-    for t, n in tensors:
-        if t is None:
-            out += [0] * n
-        else:
-            sh, st = t.shape, t.stride()
-            out += [st[i] if sh[i] > 1 else 0 for i in range(n)]
-    return (_L * len(out))(*out)
+_current_device = torch._C._cuda_getDevice if hasattr(torch._C, '_cuda_getDevice') else None
+_raw_stream = getattr(torch._C, '_cuda_getCurrentRawStream', None)
+_LONGS = [None] + [_L * n for n in range(1, 32)]
+
+
+def _strides(t, n):
+    """Element strides of the first n dimensions, 0 where a dimension has one place (whatever torch says there)."""
+    st = t.stride()[:n]
+    sh = t.shape
+    return st if 1 not in sh else tuple([0 if sh[i] == 1 else st[i] for i in range(n)])
+
+
+def _longs(values):
+    """Host array of strides."""
+    return _LONGS[len(values)](*values)
 
 
 def _ptr(t):
     return None if t is None else t.data_ptr()
 
 
+_NO2, _NO3 = (0, 0), (0, 0, 0)
+
+
 def _rows(t):
     """t as the row kernels read it: last dimension dense, rows of 16-byte pieces at 16-byte addresses; a dense copy where it is not."""
-    n = 16 // t.element_size()
-    st = t.stride()
-    if t.numel() and ((st[-1] != 1 and t.shape[-1] > 1) or t.data_ptr() % 16 or any(s % n for s, d in zip(st[:-1], t.shape[:-1]) if d > 1)):
-        c = t.contiguous()
-        return c.clone(memory_format=torch.contiguous_format) if c.data_ptr() % 16 else c
-    return t
+    if t.is_contiguous() and t.data_ptr() % 16 == 0 and t.shape[-1] * t.element_size() % 16 == 0:
+        return t
+    if (t.stride(-1) == 1 or t.shape[-1] <= 1) and _whole_pieces(t, 16):
+        return t
+    c = t.contiguous()
+    return c.clone(memory_format=torch.contiguous_format) if c.data_ptr() % 16 else c
 
 
 def _dense_last(t):
@@ -1102,86 +1093,111 @@ def _dense_last(t):
 
 
 def _check_int32(name, t, shape):
-    _need(t.dtype == torch.int32 and tuple(t.shape) == tuple(shape), '%s must be int32 %s (got %s %s)', name, tuple(shape), t.dtype, tuple(t.shape))
+    if t.dtype != torch.int32 or t.shape != shape:
+        raise AotHipError('%s must be int32 %s (got %s %s)' % (name, tuple(shape), t.dtype, tuple(t.shape)))
 
 
 def _check_freqs(freqs, D):
-    _need(freqs.dtype == torch.float64 and freqs.dim() == 1 and freqs.is_contiguous() and 1 <= freqs.numel() <= D // 2,
-          'freqs must be a dense float64 vector of at most %d frequencies', D // 2)
-    return 2 * freqs.numel()
+    n = freqs.numel()
+    if freqs.dtype != torch.float64 or freqs.dim() != 1 or not freqs.is_contiguous() or n < 1 or n > D // 2:
+        raise AotHipError('freqs must be a dense float64 vector of at most %d frequencies' % (D // 2))
+    return 2 * n
 
 
 def rope(q, k, pos, freqs, interleaved=False, mscale=1.0, inverse=False, stream=None):
     """Rotary positions of q [B, S, H, D] and k [B, S, Hk, D] (or None) at pos [B, S] int32, freqs [rot / 2] float64 radians a position:
     (q', k') (aot_rope; the first rot elements of a head turn, inverse: the gradient's direction)."""
-    _need(q.dim() == 4 and q.dtype in _DTYPE, 'rope: q must be [B, S, H, D] of float32 / float16 / bfloat16 (got %s %s)', tuple(q.shape), q.dtype)
+    dtype = _DTYPE.get(q.dtype)
+    if q.dim() != 4 or dtype is None:
+        raise AotHipError('rope: q must be [B, S, H, D] of float32 / float16 / bfloat16 (got %s %s)' % (tuple(q.shape), q.dtype))
     B, S, H, D = q.shape
-    _need(k is None or (k.dim() == 4 and k.shape[:2] == q.shape[:2] and k.shape[3] == D and k.dtype == q.dtype),
-          'rope: k must be [B, S, Hk, D] like q')
+    if k is not None and (k.dim() != 4 or k.dtype != q.dtype or k.shape[:2] != q.shape[:2] or k.shape[3] != D):
+        raise AotHipError('rope: k must be [B, S, Hk, D] like q')
     _check_int32('rope: pos', pos, (B, S))
     rot = _check_freqs(freqs, D)
-    _need(D <= 1024 and (not interleaved or D % 2 == 0), 'rope: head width %d not supported', D)
-    with _OnDevice(q, k, pos, freqs) as s:
-        q = _dense_last(q)
-        k = _dense_last(k)
-        if interleaved:
-            q, k = _rows(q), (None if k is None else _rows(k))
-        qo = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-        ko = torch.empty(k.shape, dtype=k.dtype, device=k.device) if k is not None else None
-        Hk = 0 if k is None else k.shape[2]
-        if H + Hk and B * S:
-            _chk(load().aot_rope(_ptr(q), _ptr(k), _ptr(qo), _ptr(ko), pos.data_ptr(), freqs.data_ptr(), _DTYPE[q.dtype], B, S, H, Hk, D,
-                                 rot, int(interleaved), int(inverse), mscale, _longs((q, 3), (k, 3), (qo, 3), (ko, 3), (pos, 2)),
-                                 stream if stream is not None else s), 'aot_rope')
+    if D > 1024 or (interleaved and D % 2):
+        raise AotHipError('rope: head width %d not supported' % D)
+    dev = _device_of(q, k, pos, freqs)
+    if _current_device() != dev:
+        with torch.cuda.device(dev):
+            return rope(q, k, pos, freqs, interleaved, mscale, inverse, stream)
+    q = _rows(q) if interleaved else _dense_last(q)
+    qo = torch.empty((B, S, H, D), dtype=q.dtype, device=q.device)
+    ko, Hk, more = None, 0, _NO3
+    if k is not None:
+        k = _rows(k) if interleaved else _dense_last(k)
+        Hk = k.shape[2]
+        ko = torch.empty((B, S, Hk, D), dtype=k.dtype, device=k.device)
+        more = _strides(k, 3)
+    if H + Hk and B * S:
+        st = _strides(q, 3) + more + (S * H * D, H * D, D) + (S * Hk * D, Hk * D, D) + _strides(pos, 2)
+        _chk(load().aot_rope(q.data_ptr(), _ptr(k), qo.data_ptr(), _ptr(ko), pos.data_ptr(), freqs.data_ptr(), dtype, B, S, H, Hk, D, rot,
+                             1 if interleaved else 0, 1 if inverse else 0, mscale, _longs(st), _raw_stream(dev) if stream is None else stream),
+             'aot_rope')
     return qo, ko
 
 
 def _check_pages(name, k_pages, v_pages, dtype, D=None, Hk=None):
-    _need(k_pages.dim() == 4 and k_pages.shape == v_pages.shape and k_pages.dtype == dtype and v_pages.dtype == dtype,
-          '%s: k_pages and v_pages must both be [pages, page, Hk, D] of %s', name, dtype)
-    P, page, h, d = k_pages.shape
-    _need((D is None or d == D) and (Hk is None or h == Hk), '%s: pages of %d heads of width %d do not fit the tokens', name, h, d)
-    _need(page >= 1 and page & (page - 1) == 0, '%s: the page size must be a power of two (got %d)', name, page)
-    _need(P * page <= _I32_MAX, '%s: a pool of %d places is too large', name, P * page)
-    for t in (k_pages, v_pages):
-        _need(t.stride(3) == 1 or d == 1, '%s: the last dimension of the pages must be dense', name)
+    shape = k_pages.shape
+    if len(shape) != 4 or v_pages.shape != shape or k_pages.dtype != dtype or v_pages.dtype != dtype:
+        raise AotHipError('%s: k_pages and v_pages must both be [pages, page, Hk, D] of %s' % (name, dtype))
+    P, page, h, d = shape
+    if (D is not None and d != D) or (Hk is not None and h != Hk):
+        raise AotHipError('%s: pages of %d heads of width %d do not fit the tokens' % (name, h, d))
+    if page < 1 or page & (page - 1):
+        raise AotHipError('%s: the page size must be a power of two (got %d)' % (name, page))
+    if P * page > _I32_MAX:
+        raise AotHipError('%s: a pool of %d places is too large' % (name, P * page))
+    if (k_pages.stride(3) != 1 or v_pages.stride(3) != 1) and d != 1:
+        raise AotHipError('%s: the last dimension of the pages must be dense' % name)
     return P, page, h, d
 
 
-def _check_page_rows(name, *pools):
-    for t in pools:
-        n = 16 // t.element_size()
-        _need(not t.numel() or (t.shape[3] % n == 0 and t.data_ptr() % 16 == 0 and all(x % n == 0 for x, d in zip(t.stride()[:3], t.shape[:3]) if d > 1)),
-              '%s: page rows must be whole 16-byte pieces at 16-byte addresses', name)
+def _whole_pieces(t, bytes_):
+    """Whether every row of t (its last dimension) is whole pieces of that many bytes at such addresses."""
+    n = bytes_ // t.element_size()
+    return not t.numel() or (t.shape[-1] % n == 0 and t.data_ptr() % bytes_ == 0 and not any(x % n for x in _strides(t, t.dim() - 1)))
 
 
 def rope_append(q, k, v, pos, freqs, slots, k_pages, v_pages, interleaved=False, mscale=1.0, stream=None):
     """New tokens q [N, H, D] (or None), k / v [N, Hk, D] at pos [N]: turns q and k, writes the turned keys and the values to the cache places
     slots [N] int32 (page id * page + place; negative: not written) of k_pages / v_pages [pages, page, Hk, D], returns the turned q
     (aot_rope_append)."""
-    _need(k.dim() == 3 and k.dtype in _DTYPE and v.shape == k.shape and v.dtype == k.dtype, 'rope_append: k and v must both be [N, Hk, D]')
+    dtype = _DTYPE.get(k.dtype)
+    if k.dim() != 3 or dtype is None or v.shape != k.shape or v.dtype != k.dtype:
+        raise AotHipError('rope_append: k and v must both be [N, Hk, D] of float32 / float16 / bfloat16')
     N, Hk, D = k.shape
-    _need(q is None or (q.dim() == 3 and q.shape[0] == N and q.shape[2] == D and q.dtype == k.dtype), 'rope_append: q must be [N, H, D] like k')
+    if q is not None and (q.dim() != 3 or q.shape[0] != N or q.shape[2] != D or q.dtype != k.dtype):
+        raise AotHipError('rope_append: q must be [N, H, D] like k')
     _check_int32('rope_append: pos', pos, (N,))
     _check_int32('rope_append: slots', slots, (N,))
     rot = _check_freqs(freqs, D)
-    _need(D <= 1024 and (not interleaved or D % 2 == 0), 'rope_append: head width %d not supported', D)
+    if D > 1024 or (interleaved and D % 2):
+        raise AotHipError('rope_append: head width %d not supported' % D)
     P, page, _, _ = _check_pages('rope_append', k_pages, v_pages, k.dtype, D, Hk)
+    if interleaved and not (_whole_pieces(k_pages, 2 * k.element_size()) and _whole_pieces(v_pages, 2 * k.element_size())):
+        raise AotHipError('rope_append: interleaved pairs need pages aligned to pairs')
+    dev = _device_of(k, v, q, pos, freqs, slots, k_pages, v_pages)
+    if _current_device() != dev:
+        with torch.cuda.device(dev):
+            return rope_append(q, k, v, pos, freqs, slots, k_pages, v_pages, interleaved, mscale, stream)
+    k, v, pos, slots = _dense_last(k), _dense_last(v), pos.contiguous(), slots.contiguous()
     if interleaved:
-        for t in (k_pages, v_pages):
-            _need(t.data_ptr() % (2 * t.element_size()) == 0 and all(x % 2 == 0 for x, d in zip(t.stride()[:3], t.shape[:3]) if d > 1),
-                  'rope_append: interleaved pairs need pages aligned to pairs')
-    with _OnDevice(q, k, v, pos, freqs, slots, k_pages, v_pages) as s:
-        q, k, v = _dense_last(q), _dense_last(k), _dense_last(v)
-        pos, slots = pos.contiguous(), slots.contiguous()
-        if interleaved:
-            q, k, v = (None if q is None else _rows(q)), _rows(k), _rows(v)
-        qo = torch.empty(q.shape, dtype=q.dtype, device=q.device) if q is not None else None
-        if N and Hk:
-            _chk(load().aot_rope_append(_ptr(q), _ptr(k), _ptr(v), _ptr(qo), _ptr(k_pages), _ptr(v_pages), pos.data_ptr(), slots.data_ptr(),
-                                        freqs.data_ptr(), _DTYPE[k.dtype], N, 0 if q is None else q.shape[1], Hk, D, rot, int(interleaved),
-                                        mscale, page, P, _longs((q, 2), (k, 2), (v, 2), (qo, 2), (k_pages, 3), (v_pages, 3)),
-                                        stream if stream is not None else s), 'aot_rope_append')
+        k, v = _rows(k), _rows(v)
+    qo, H = None, 0
+    st = _strides(k, 2) + _strides(v, 2)
+    if q is not None:
+        q = _rows(q) if interleaved else _dense_last(q)
+        H = q.shape[1]
+        qo = torch.empty((N, H, D), dtype=q.dtype, device=q.device)
+        st = _strides(q, 2) + st + (H * D, D)
+    else:
+        st = _NO2 + st + _NO2
+    if N and Hk:
+        _chk(load().aot_rope_append(_ptr(q), k.data_ptr(), v.data_ptr(), _ptr(qo), k_pages.data_ptr(), v_pages.data_ptr(), pos.data_ptr(),
+                                    slots.data_ptr(), freqs.data_ptr(), dtype, N, H, Hk, D, rot, 1 if interleaved else 0, mscale, page, P,
+                                    _longs(st + _strides(k_pages, 3) + _strides(v_pages, 3)), _raw_stream(dev) if stream is None else stream),
+             'aot_rope_append')
     return qo
 
 
@@ -1207,18 +1223,24 @@ def _masked_args(name, q, k, v, scale, softcap, slopes, doc_q, doc_k, prefix):
 def attn_masked(q, k, v, scale=None, causal=False, softcap=0.0, slopes=None, doc_q=None, doc_k=None, prefix=None, stream=None):
     """Attention under masks (aot_attn_masked): q [B, Sq, H, D], k / v [B, Sk, Hk, D] -> (out [B, Sq, H, D], lse [B, H, Sq] in powers of two)."""
     B, Sq, Sk, H, Hk, D, scale = _masked_args('attn_masked', q, k, v, scale, softcap, slopes, doc_q, doc_k, prefix)
-    with _OnDevice(q, k, v, slopes, doc_q, doc_k, prefix) as s:
-        q, k, v = _rows(q), _rows(k), _rows(v)
+    dev = _device_of(q, k, v, slopes, doc_q, doc_k, prefix)
+    if _current_device() != dev:
+        with torch.cuda.device(dev):
+            return attn_masked(q, k, v, scale, causal, softcap, slopes, doc_q, doc_k, prefix, stream)
+    q, k, v = _rows(q), _rows(k), _rows(v)
+    out = torch.empty((B, Sq, H, D), dtype=q.dtype, device=q.device)
+    lse = torch.empty((B, H, Sq), dtype=torch.float32, device=q.device)
+    docs, ranges = _NO2, None
+    if doc_q is not None:
         doc_q, doc_k = _dense_last(doc_q), _dense_last(doc_k)
+        docs = _strides(doc_q, 1) + _strides(doc_k, 1)
+        ranges = torch.empty(4 * B * (-(-Sq // 64) + -(-Sk // 64)), dtype=torch.int32, device=q.device)
+    if B and Sq:
         prefix = None if prefix is None else prefix.contiguous()
-        out = torch.empty((B, Sq, H, D), dtype=q.dtype, device=q.device)
-        lse = torch.empty((B, H, Sq), dtype=torch.float32, device=q.device)
-        ranges = torch.empty(4 * B * (-(-Sq // 64) + -(-Sk // 64)), dtype=torch.int32, device=q.device) if doc_q is not None else None
-        if B and Sq:
-            _chk(load().aot_attn_masked(_ptr(q), _ptr(k), _ptr(v), _ptr(out), _ptr(lse), _ptr(slopes), _ptr(doc_q), _ptr(doc_k) or _ptr(doc_q),
-                                        _ptr(prefix), _ptr(ranges), _DTYPE[q.dtype], B, Sq, Sk, H, Hk, D, int(causal), scale, softcap,
-                                        _longs((q, 3), (k, 3), (v, 3), (out, 3), (doc_q, 1), (doc_k, 1)), stream if stream is not None else s),
-                 'aot_attn_masked')
+        _chk(load().aot_attn_masked(q.data_ptr(), _ptr(k), _ptr(v), out.data_ptr(), lse.data_ptr(), _ptr(slopes), _ptr(doc_q), _ptr(doc_k) or _ptr(doc_q),
+                                    _ptr(prefix), _ptr(ranges), _DTYPE[q.dtype], B, Sq, Sk, H, Hk, D, 1 if causal else 0, scale, softcap,
+                                    _longs(_strides(q, 3) + _strides(k, 3) + _strides(v, 3) + (Sq * H * D, H * D, D) + docs),
+                                    _raw_stream(dev) if stream is None else stream), 'aot_attn_masked')
     return out, lse
 
 
@@ -1227,60 +1249,79 @@ def attn_masked_bwd(dout, q, k, v, out, lse, scale=None, causal=False, softcap=0
     B, Sq, Sk, H, Hk, D, scale = _masked_args('attn_masked_bwd', q, k, v, scale, softcap, slopes, doc_q, doc_k, prefix)
     _need(dout.shape == q.shape and out.shape == q.shape and dout.dtype == q.dtype and out.dtype == q.dtype, 'attn_masked_bwd: out and dout must be like q')
     _need(lse.dtype == torch.float32 and tuple(lse.shape) == (B, H, Sq) and lse.is_contiguous(), 'attn_masked_bwd: lse must be dense float32 [B, H, Sq]')
-    with _OnDevice(q, k, v, out, dout, lse, slopes, doc_q, doc_k, prefix) as s:
-        q, k, v, out, dout = _rows(q), _rows(k), _rows(v), _rows(out), _rows(dout)
+    dev = _device_of(q, k, v, out, dout, lse, slopes, doc_q, doc_k, prefix)
+    if _current_device() != dev:
+        with torch.cuda.device(dev):
+            return attn_masked_bwd(dout, q, k, v, out, lse, scale, causal, softcap, slopes, doc_q, doc_k, prefix, stream)
+    q, k, v, out, dout = _rows(q), _rows(k), _rows(v), _rows(out), _rows(dout)
+    where = dict(dtype=q.dtype, device=q.device)
+    dq, dk, dv = torch.empty((B, Sq, H, D), **where), torch.empty((B, Sk, Hk, D), **where), torch.empty((B, Sk, Hk, D), **where)
+    n = _L()
+    _chk(load().aot_attn_masked_bwd_floats(B, Sq, Sk, H, Hk, D, ctypes.addressof(n)), 'aot_attn_masked_bwd_floats')
+    work = torch.empty(max(n.value, 1), dtype=torch.float32, device=q.device)
+    docs, ranges = _NO2, None
+    if doc_q is not None:
         doc_q, doc_k = _dense_last(doc_q), _dense_last(doc_k)
+        docs = _strides(doc_q, 1) + _strides(doc_k, 1)
+        ranges = torch.empty(4 * B * (-(-Sq // 64) + -(-Sk // 64)), dtype=torch.int32, device=q.device)
+    if B and (Sq or Sk):
         prefix = None if prefix is None else prefix.contiguous()
-        dev = q.device
-        dq = torch.empty((B, Sq, H, D), dtype=q.dtype, device=dev)
-        dk = torch.empty((B, Sk, Hk, D), dtype=q.dtype, device=dev)
-        dv = torch.empty((B, Sk, Hk, D), dtype=q.dtype, device=dev)
-        n = _L()
-        _chk(load().aot_attn_masked_bwd_floats(B, Sq, Sk, H, Hk, D, ctypes.addressof(n)), 'aot_attn_masked_bwd_floats')
-        work = torch.empty(max(n.value, 1), dtype=torch.float32, device=dev)
-        ranges = torch.empty(4 * B * (-(-Sq // 64) + -(-Sk // 64)), dtype=torch.int32, device=dev) if doc_q is not None else None
-        if B and (Sq or Sk):
-            _chk(load().aot_attn_masked_bwd(_ptr(q), _ptr(k), _ptr(v), _ptr(out), _ptr(lse), _ptr(dout), _ptr(dq), _ptr(dk), _ptr(dv), _ptr(slopes),
-                                            _ptr(doc_q) or _ptr(doc_k), _ptr(doc_k) or _ptr(doc_q), _ptr(prefix), _ptr(ranges), _ptr(work), n.value, _DTYPE[q.dtype],
-                                            B, Sq, Sk, H, Hk, D, int(causal), scale, softcap,
-                                            _longs((q, 3), (k, 3), (v, 3), (out, 3), (dout, 3), (dq, 3), (dk, 3), (dv, 3), (doc_q, 1), (doc_k, 1)),
-                                            stream if stream is not None else s), 'aot_attn_masked_bwd')
+        qs, ks = (Sq * H * D, H * D, D), (Sk * Hk * D, Hk * D, D)
+        _chk(load().aot_attn_masked_bwd(_ptr(q), _ptr(k), _ptr(v), _ptr(out), _ptr(lse), _ptr(dout), _ptr(dq), _ptr(dk), _ptr(dv), _ptr(slopes),
+                                        _ptr(doc_q) or _ptr(doc_k), _ptr(doc_k) or _ptr(doc_q), _ptr(prefix), _ptr(ranges), work.data_ptr(), n.value,
+                                        _DTYPE[q.dtype], B, Sq, Sk, H, Hk, D, 1 if causal else 0, scale, softcap,
+                                        _longs(_strides(q, 3) + _strides(k, 3) + _strides(v, 3) + _strides(out, 3) + _strides(dout, 3) + qs + ks + ks + docs),
+                                        _raw_stream(dev) if stream is None else stream), 'aot_attn_masked_bwd')
     return dq, dk, dv
 
 
 def paged_attn(q, k_pages, v_pages, table, lengths, scale=None, softcap=0.0, slopes=None, weights=None, key_pos=None, out=None, stream=None):
     """One new token per sequence, q [B, H, D], over a paged cache (aot_paged_attn): table [B, max_pages] and lengths [B] int32, k_pages /
     v_pages [pages, page, Hk, D]; weights [B, Hk, S] float32 is added to in place, key_pos [B, Hk, S] int32, S >= max_pages * page."""
-    _need(q.dim() == 3 and q.dtype in _DTYPE, 'paged_attn: q must be [B, H, D] of float32 / float16 / bfloat16')
+    dtype = _DTYPE.get(q.dtype)
+    if q.dim() != 3 or dtype is None:
+        raise AotHipError('paged_attn: q must be [B, H, D] of float32 / float16 / bfloat16')
     B, H, D = q.shape
     P, page, Hk, _ = _check_pages('paged_attn', k_pages, v_pages, q.dtype, D)
-    _need(Hk >= 1 and H >= Hk and H % Hk == 0, 'paged_attn: %d query heads on %d key heads', H, Hk)
-    _need(1 <= D <= 256 and D * q.element_size() % 16 == 0, 'paged_attn: head width %d of %s not supported (whole 16-byte pieces, at most 256)', D, q.dtype)
-    _check_page_rows('paged_attn', k_pages, v_pages)
-    _need(table.dim() == 2 and table.dtype == torch.int32 and table.shape[0] == B, 'paged_attn: table must be int32 [B, max_pages]')
+    if Hk < 1 or H < Hk or H % Hk:
+        raise AotHipError('paged_attn: %d query heads on %d key heads' % (H, Hk))
+    if D < 1 or D > 256 or D * q.element_size() % 16:
+        raise AotHipError('paged_attn: head width %d of %s not supported (whole 16-byte pieces, at most 256)' % (D, q.dtype))
+    if not (_whole_pieces(k_pages, 16) and _whole_pieces(v_pages, 16)):
+        raise AotHipError('paged_attn: page rows must be whole 16-byte pieces at 16-byte addresses')
+    if table.dim() != 2 or table.dtype != torch.int32 or table.shape[0] != B:
+        raise AotHipError('paged_attn: table must be int32 [B, max_pages]')
     mp = table.shape[1]
     cap = mp * page
-    _need(cap <= _I32_MAX and B <= 65535, 'paged_attn: sizes beyond 2^31 entries or 65535 sequences')
+    if cap > _I32_MAX or B > 65535:
+        raise AotHipError('paged_attn: sizes beyond 2^31 entries or 65535 sequences')
     _check_int32('paged_attn: lengths', lengths, (B,))
-    _need(softcap >= 0, 'paged_attn: softcap must not be negative')
-    _need(slopes is None or (slopes.dtype == torch.float32 and tuple(slopes.shape) == (H,) and slopes.is_contiguous()), 'paged_attn: slopes must be dense float32 [H]')
+    if not softcap >= 0:
+        raise AotHipError('paged_attn: softcap must not be negative')
+    if slopes is not None and (slopes.dtype != torch.float32 or tuple(slopes.shape) != (H,) or not slopes.is_contiguous()):
+        raise AotHipError('paged_attn: slopes must be dense float32 [H]')
     for name, t, dt in (('weights', weights, torch.float32), ('key_pos', key_pos, torch.int32)):
-        _need(t is None or (t.dtype == dt and t.dim() == 3 and t.shape[:2] == (B, Hk) and t.shape[2] >= cap and (t.stride(2) == 1 or t.shape[2] <= 1)),
-              'paged_attn: %s must be %s [B, Hk, at least %d], last dimension dense', name, dt, cap)
-    _need(out is None or (out.shape == q.shape and out.dtype == q.dtype and (out.stride(2) == 1 or D == 1)), 'paged_attn: out must be like q')
-    with _OnDevice(q, k_pages, v_pages, table, lengths, slopes, weights, key_pos, out) as s:
-        lib = load()
-        q = _rows(q)
-        table, lengths = _dense_last(table), lengths.contiguous()
-        if out is None:
-            out = torch.empty((B, H, D), dtype=q.dtype, device=q.device)
-        n = _L()
-        _chk(lib.aot_paged_attn_work_floats(B, H, Hk, D, page, mp, int(weights is not None), ctypes.addressof(n)), 'aot_paged_attn_work_floats')
-        work = torch.empty(n.value, dtype=torch.float32, device=q.device) if n.value else None
-        _chk(lib.aot_paged_attn(_ptr(q), _ptr(k_pages), _ptr(v_pages), _ptr(table), _ptr(lengths), _ptr(slopes), _ptr(key_pos), _ptr(weights), _ptr(out),
-                                _ptr(work), n.value, _DTYPE[q.dtype], B, H, Hk, D, page, mp, P, float(D ** -0.5 if scale is None else scale), softcap,
-                                _longs((q, 2), (out, 2), (k_pages, 3), (v_pages, 3), (table, 1), (weights, 2), (key_pos, 2)),
-                                stream if stream is not None else s), 'aot_paged_attn')
+        if t is not None and (t.dtype != dt or t.dim() != 3 or t.shape[0] != B or t.shape[1] != Hk or t.shape[2] < cap or
+                              (t.stride(2) != 1 and t.shape[2] > 1)):
+            raise AotHipError('paged_attn: %s must be %s [B, Hk, at least %d], last dimension dense' % (name, dt, cap))
+    if out is not None and (out.shape != q.shape or out.dtype != q.dtype or (out.stride(2) != 1 and D != 1)):
+        raise AotHipError('paged_attn: out must be like q')
+    dev = _device_of(q, k_pages, v_pages, table, lengths, slopes, weights, key_pos, out)
+    if _current_device() != dev:
+        with torch.cuda.device(dev):
+            return paged_attn(q, k_pages, v_pages, table, lengths, scale, softcap, slopes, weights, key_pos, out, stream)
+    lib = load()
+    q, table, lengths = _rows(q), _dense_last(table), lengths.contiguous()
+    if out is None:
+        out = torch.empty((B, H, D), dtype=q.dtype, device=q.device)
+    n = _L()
+    _chk(lib.aot_paged_attn_work_floats(B, H, Hk, D, page, mp, 0 if weights is None else 1, ctypes.addressof(n)), 'aot_paged_attn_work_floats')
+    work = torch.empty(n.value, dtype=torch.float32, device=q.device) if n.value else None
+    st = _strides(q, 2) + _strides(out, 2) + _strides(k_pages, 3) + _strides(v_pages, 3) + _strides(table, 1) + \
+        (_NO2 if weights is None else _strides(weights, 2)) + (_NO2 if key_pos is None else _strides(key_pos, 2))
+    _chk(lib.aot_paged_attn(_ptr(q), _ptr(k_pages), _ptr(v_pages), _ptr(table), _ptr(lengths), _ptr(slopes), _ptr(key_pos), _ptr(weights), _ptr(out),
+                            _ptr(work), n.value, dtype, B, H, Hk, D, page, mp, P, D ** -0.5 if scale is None else scale, softcap, _longs(st),
+                            _raw_stream(dev) if stream is None else stream), 'aot_paged_attn')
     return out
 
 
@@ -1288,34 +1329,44 @@ def paged_evict(k_pages, v_pages, table, lengths, weights, new_table, budget, si
     """Keeps `budget` entries of every cache row -- the first `sink`, the last `recent`, the heaviest by weights [B, Hk, S] -- and copies them into
     the pages of new_table [B, new_pages] (aot_paged_evict): (kept [B, Hk, budget] old indices or -1, new lengths [B], new weights, new
     key_pos or None)."""
-    _need(k_pages.dtype in _DTYPE, 'paged_evict: pages must be float32 / float16 / bfloat16')
+    dtype = _DTYPE.get(k_pages.dtype)
+    if dtype is None:
+        raise AotHipError('paged_evict: pages must be float32 / float16 / bfloat16')
     P, page, Hk, D = _check_pages('paged_evict', k_pages, v_pages, k_pages.dtype)
-    _need(table.dim() == 2 and new_table.dim() == 2 and table.dtype == torch.int32 and new_table.dtype == torch.int32 and table.shape[0] == new_table.shape[0],
-          'paged_evict: table and new_table must be int32 [B, pages]')
+    if table.dim() != 2 or new_table.dim() != 2 or table.dtype != torch.int32 or new_table.dtype != torch.int32 or table.shape[0] != new_table.shape[0]:
+        raise AotHipError('paged_evict: table and new_table must be int32 [B, pages]')
     B, mp = table.shape
     npg = new_table.shape[1]
     _check_int32('paged_evict: lengths', lengths, (B,))
-    _need(weights.dtype == torch.float32 and weights.dim() == 3 and weights.shape[:2] == (B, Hk) and weights.shape[2] >= mp * page,
-          'paged_evict: weights must be float32 [B, Hk, at least %d]', mp * page)
-    _need(key_pos is None or (key_pos.dtype == torch.int32 and key_pos.shape == weights.shape), 'paged_evict: key_pos must be int32, shaped like weights')
+    if weights.dtype != torch.float32 or weights.dim() != 3 or weights.shape[0] != B or weights.shape[1] != Hk or weights.shape[2] < mp * page:
+        raise AotHipError('paged_evict: weights must be float32 [B, Hk, at least %d]' % (mp * page))
+    if key_pos is not None and (key_pos.dtype != torch.int32 or key_pos.shape != weights.shape):
+        raise AotHipError('paged_evict: key_pos must be int32, shaped like weights')
     budget, sink, recent = int(budget), int(sink), int(recent)
-    _need(budget >= 1 and sink >= 0 and recent >= 0 and sink + recent <= budget, 'paged_evict: sink %d + recent %d must fit the budget %d', sink, recent, budget)
-    _need(npg * page >= budget, 'paged_evict: new_table holds %d entries, the budget is %d', npg * page, budget)
-    _need(mp * page <= _I32_MAX and B <= 65535 and Hk <= 65535, 'paged_evict: sizes beyond 2^31 entries or 65535 rows')
+    if budget < 1 or sink < 0 or recent < 0 or sink + recent > budget:
+        raise AotHipError('paged_evict: sink %d + recent %d must fit the budget %d' % (sink, recent, budget))
+    if npg * page < budget:
+        raise AotHipError('paged_evict: new_table holds %d entries, the budget is %d' % (npg * page, budget))
+    if mp * page > _I32_MAX or npg * page > _I32_MAX or B > 65535 or Hk > 65535:
+        raise AotHipError('paged_evict: sizes beyond 2^31 entries or 65535 rows')
+    dev = _device_of(k_pages, v_pages, table, lengths, weights, new_table, key_pos)
+    if _current_device() != dev:
+        with torch.cuda.device(dev):
+            return paged_evict(k_pages, v_pages, table, lengths, weights, new_table, budget, sink, recent, key_pos, stream)
+    if mp and table.data_ptr() == new_table.data_ptr():
+        raise AotHipError('paged_evict: new_table must not be table')
     S = weights.shape[2]
-    with _OnDevice(k_pages, v_pages, table, lengths, weights, new_table, key_pos) as s:
-        dev = weights.device
-        _need(not (mp and npg) or table.data_ptr() != new_table.data_ptr(), 'paged_evict: new_table must not be table')
-        table, new_table, lengths = _dense_last(table), _dense_last(new_table), lengths.contiguous()
-        weights, key_pos = _dense_last(weights), _dense_last(key_pos)
-        kept = torch.empty((B, Hk, budget), dtype=torch.int32, device=dev)
-        new_lengths = torch.empty(B, dtype=torch.int32, device=dev)
-        new_weights = torch.empty((B, Hk, S), dtype=torch.float32, device=dev)
-        new_pos = torch.empty((B, Hk, S), dtype=torch.int32, device=dev) if key_pos is not None else None
-        if B and Hk:
-            _need(mp > 0, 'paged_evict: table has no pages')
-            _chk(load().aot_paged_evict(_ptr(k_pages), _ptr(v_pages), _ptr(table), _ptr(new_table), _ptr(lengths), _ptr(weights), _ptr(key_pos), _ptr(kept),
-                                        _ptr(new_lengths), _ptr(new_weights), _ptr(new_pos), _DTYPE[k_pages.dtype], B, Hk, D, S, page, mp, npg, P, budget,
-                                        sink, recent, _longs((k_pages, 3), (v_pages, 3), (table, 1), (new_table, 1), (weights, 2), (new_weights, 2),
-                                                             (key_pos, 2), (new_pos, 2)), stream if stream is not None else s), 'aot_paged_evict')
+    table, new_table, lengths, weights, key_pos = _dense_last(table), _dense_last(new_table), lengths.contiguous(), _dense_last(weights), _dense_last(key_pos)
+    kept = torch.empty((B, Hk, budget), dtype=torch.int32, device=k_pages.device)
+    new_lengths = torch.empty(B, dtype=torch.int32, device=k_pages.device)
+    new_weights = torch.empty((B, Hk, S), dtype=torch.float32, device=k_pages.device)
+    new_pos = torch.empty((B, Hk, S), dtype=torch.int32, device=k_pages.device) if key_pos is not None else None
+    if B and Hk:
+        if not mp:
+            raise AotHipError('paged_evict: table has no pages')
+        st = _strides(k_pages, 3) + _strides(v_pages, 3) + _strides(table, 1) + _strides(new_table, 1) + _strides(weights, 2) + (Hk * S, S)
+        st += _NO2 + _NO2 if key_pos is None else _strides(key_pos, 2) + (Hk * S, S)
+        _chk(load().aot_paged_evict(_ptr(k_pages), _ptr(v_pages), _ptr(table), _ptr(new_table), _ptr(lengths), _ptr(weights), _ptr(key_pos), _ptr(kept),
+                                    _ptr(new_lengths), _ptr(new_weights), _ptr(new_pos), dtype, B, Hk, D, S, page, mp, npg, P, budget,
+                                    sink, recent, _longs(st), _raw_stream(dev) if stream is None else stream), 'aot_paged_evict')
     return kept, new_lengths, new_weights, new_pos
