@@ -97,9 +97,9 @@ _SIGS = {
     'aot_window_scatter_f32': [_P, _P] + [_I] * 4 + [_F, _P],
     'aot_rope': [_P] * 6 + [_I] * 9 + [_F, _P, _P],
     'aot_rope_append': [_P] * 9 + [_I] * 7 + [_F, _I, _L, _P, _P],
-    'aot_attn_masked': [_P] * 10 + [_I] * 8 + [_F, _F, _P, _P],
-    'aot_attn_masked_bwd': [_P] * 15 + [_L] + [_I] * 8 + [_F, _F, _P, _P],
-    'aot_attn_masked_bwd_floats': [_I] * 6 + [_P],
+    'aot_attn_masked': [_P] * 12 + [_L] + [_I] * 8 + [_F, _F, _P, _P],
+    'aot_attn_masked_bwd': [_P] * 16 + [_L] + [_I] * 8 + [_F, _F, _P, _P],
+    'aot_attn_masked_floats': [_I] * 7 + [_P],
     'aot_paged_attn': [_P] * 10 + [_L] + [_I] * 7 + [_L, _F, _F, _P, _P],
     'aot_paged_attn_work_floats': [_I] * 7 + [_P],
     'aot_paged_evict': [_P] * 11 + [_I] * 8 + [_L] + [_I] * 3 + [_P, _P],
@@ -1220,16 +1220,26 @@ def _masked_args(name, q, k, v, scale, softcap, slopes, doc_q, doc_k, prefix):
     return B, Sq, Sk, H, Hk, D, float(D ** -0.5 if scale is None else scale)
 
 
-def attn_masked(q, k, v, scale=None, causal=False, softcap=0.0, slopes=None, doc_q=None, doc_k=None, prefix=None, stream=None):
-    """Attention under masks (aot_attn_masked): q [B, Sq, H, D], k / v [B, Sk, Hk, D] -> (out [B, Sq, H, D], lse [B, H, Sq] in powers of two)."""
+def _masked_work(B, Sq, Sk, H, Hk, D, backward, device):
+    n = _L()
+    _chk(load().aot_attn_masked_floats(B, Sq, Sk, H, Hk, D, backward, ctypes.addressof(n)), 'aot_attn_masked_floats')
+    return (torch.empty(n.value, dtype=torch.float32, device=device) if n.value else None), n.value
+
+
+def attn_masked(q, k, v, scale=None, causal=False, softcap=0.0, slopes=None, doc_q=None, doc_k=None, prefix=None, residual=False,
+                stream=None):
+    """Attention under masks (aot_attn_masked): q [B, Sq, H, D], k / v [B, Sk, Hk, D] -> (out [B, Sq, H, D], lse [B, H, Sq] in powers of two,
+    residual): residual=True asks for what rounding a 16-bit out left, which sharpens attn_masked_bwd; else (and for float32) it is None."""
     B, Sq, Sk, H, Hk, D, scale = _masked_args('attn_masked', q, k, v, scale, softcap, slopes, doc_q, doc_k, prefix)
     dev = _device_of(q, k, v, slopes, doc_q, doc_k, prefix)
     if _current_device() != dev:
         with torch.cuda.device(dev):
-            return attn_masked(q, k, v, scale, causal, softcap, slopes, doc_q, doc_k, prefix, stream)
+            return attn_masked(q, k, v, scale, causal, softcap, slopes, doc_q, doc_k, prefix, residual, stream)
     q, k, v = _rows(q), _rows(k), _rows(v)
     out = torch.empty((B, Sq, H, D), dtype=q.dtype, device=q.device)
     lse = torch.empty((B, H, Sq), dtype=torch.float32, device=q.device)
+    res = torch.empty_like(out) if residual and out.element_size() == 2 else None
+    work, n = _masked_work(B, Sq, Sk, H, Hk, D, 0, q.device)
     docs, ranges = _NO2, None
     if doc_q is not None:
         doc_q, doc_k = _dense_last(doc_q), _dense_last(doc_k)
@@ -1237,28 +1247,27 @@ def attn_masked(q, k, v, scale=None, causal=False, softcap=0.0, slopes=None, doc
         ranges = torch.empty(4 * B * (-(-Sq // 64) + -(-Sk // 64)), dtype=torch.int32, device=q.device)
     if B and Sq:
         prefix = None if prefix is None else prefix.contiguous()
-        _chk(load().aot_attn_masked(q.data_ptr(), _ptr(k), _ptr(v), out.data_ptr(), lse.data_ptr(), _ptr(slopes), _ptr(doc_q), _ptr(doc_k) or _ptr(doc_q),
-                                    _ptr(prefix), _ptr(ranges), _DTYPE[q.dtype], B, Sq, Sk, H, Hk, D, 1 if causal else 0, scale, softcap,
+        _chk(load().aot_attn_masked(q.data_ptr(), _ptr(k), _ptr(v), out.data_ptr(), _ptr(res), lse.data_ptr(), _ptr(slopes), _ptr(doc_q),
+                                    _ptr(doc_k) or _ptr(doc_q), _ptr(prefix), _ptr(ranges), _ptr(work), n, _DTYPE[q.dtype], B, Sq, Sk, H, Hk, D, 1 if causal else 0, scale, softcap,
                                     _longs(_strides(q, 3) + _strides(k, 3) + _strides(v, 3) + (Sq * H * D, H * D, D) + docs),
                                     _raw_stream(dev) if stream is None else stream), 'aot_attn_masked')
-    return out, lse
+    return out, lse, res
 
 
-def attn_masked_bwd(dout, q, k, v, out, lse, scale=None, causal=False, softcap=0.0, slopes=None, doc_q=None, doc_k=None, prefix=None, stream=None):
+def attn_masked_bwd(dout, q, k, v, out, lse, residual=None, scale=None, causal=False, softcap=0.0, slopes=None, doc_q=None, doc_k=None, prefix=None, stream=None):
     """Gradients of attn_masked (aot_attn_masked_bwd): its inputs, results and the gradient of out -> (dq, dk, dv)."""
     B, Sq, Sk, H, Hk, D, scale = _masked_args('attn_masked_bwd', q, k, v, scale, softcap, slopes, doc_q, doc_k, prefix)
     _need(dout.shape == q.shape and out.shape == q.shape and dout.dtype == q.dtype and out.dtype == q.dtype, 'attn_masked_bwd: out and dout must be like q')
     _need(lse.dtype == torch.float32 and tuple(lse.shape) == (B, H, Sq) and lse.is_contiguous(), 'attn_masked_bwd: lse must be dense float32 [B, H, Sq]')
-    dev = _device_of(q, k, v, out, dout, lse, slopes, doc_q, doc_k, prefix)
+    _need(residual is None or (residual.shape == q.shape and residual.dtype == q.dtype and residual.is_contiguous()), 'attn_masked_bwd: residual must be dense, like q')
+    dev = _device_of(q, k, v, out, dout, lse, residual, slopes, doc_q, doc_k, prefix)
     if _current_device() != dev:
         with torch.cuda.device(dev):
-            return attn_masked_bwd(dout, q, k, v, out, lse, scale, causal, softcap, slopes, doc_q, doc_k, prefix, stream)
+            return attn_masked_bwd(dout, q, k, v, out, lse, residual, scale, causal, softcap, slopes, doc_q, doc_k, prefix, stream)
     q, k, v, out, dout = _rows(q), _rows(k), _rows(v), _rows(out), _rows(dout)
     where = dict(dtype=q.dtype, device=q.device)
     dq, dk, dv = torch.empty((B, Sq, H, D), **where), torch.empty((B, Sk, Hk, D), **where), torch.empty((B, Sk, Hk, D), **where)
-    n = _L()
-    _chk(load().aot_attn_masked_bwd_floats(B, Sq, Sk, H, Hk, D, ctypes.addressof(n)), 'aot_attn_masked_bwd_floats')
-    work = torch.empty(max(n.value, 1), dtype=torch.float32, device=q.device)
+    work, n = _masked_work(B, Sq, Sk, H, Hk, D, 1, q.device)
     docs, ranges = _NO2, None
     if doc_q is not None:
         doc_q, doc_k = _dense_last(doc_q), _dense_last(doc_k)
@@ -1267,8 +1276,8 @@ def attn_masked_bwd(dout, q, k, v, out, lse, scale=None, causal=False, softcap=0
     if B and (Sq or Sk):
         prefix = None if prefix is None else prefix.contiguous()
         qs, ks = (Sq * H * D, H * D, D), (Sk * Hk * D, Hk * D, D)
-        _chk(load().aot_attn_masked_bwd(_ptr(q), _ptr(k), _ptr(v), _ptr(out), _ptr(lse), _ptr(dout), _ptr(dq), _ptr(dk), _ptr(dv), _ptr(slopes),
-                                        _ptr(doc_q) or _ptr(doc_k), _ptr(doc_k) or _ptr(doc_q), _ptr(prefix), _ptr(ranges), work.data_ptr(), n.value,
+        _chk(load().aot_attn_masked_bwd(_ptr(q), _ptr(k), _ptr(v), _ptr(out), _ptr(residual), _ptr(lse), _ptr(dout), _ptr(dq), _ptr(dk), _ptr(dv), _ptr(slopes),
+                                        _ptr(doc_q) or _ptr(doc_k), _ptr(doc_k) or _ptr(doc_q), _ptr(prefix), _ptr(ranges), _ptr(work), n,
                                         _DTYPE[q.dtype], B, Sq, Sk, H, Hk, D, 1 if causal else 0, scale, softcap,
                                         _longs(_strides(q, 3) + _strides(k, 3) + _strides(v, 3) + _strides(out, 3) + _strides(dout, 3) + qs + ks + ks + docs),
                                         _raw_stream(dev) if stream is None else stream), 'aot_attn_masked_bwd')

@@ -48,8 +48,8 @@ _DEFS = {
     'rope_append': '(Tensor? q, Tensor k, Tensor v, Tensor pos, Tensor freqs, Tensor slots, Tensor(a!) k_pages, Tensor(b!) v_pages, '
                    'bool interleaved, float mscale) -> Tensor?',
     'attn_masked': '(Tensor q, Tensor k, Tensor v, float? scale, bool causal, float softcap, Tensor? slopes, Tensor? doc_q, Tensor? doc_k, '
-                   'Tensor? prefix) -> (Tensor, Tensor)',
-    'attn_masked_bwd': '(Tensor dout, Tensor q, Tensor k, Tensor v, Tensor out, Tensor lse, float? scale, bool causal, float softcap, '
+                   'Tensor? prefix, bool residual) -> (Tensor, Tensor, Tensor?)',
+    'attn_masked_bwd': '(Tensor dout, Tensor q, Tensor k, Tensor v, Tensor out, Tensor lse, Tensor? residual, float? scale, bool causal, float softcap, '
                        'Tensor? slopes, Tensor? doc_q, Tensor? doc_k, Tensor? prefix) -> (Tensor, Tensor, Tensor)',
     'paged_attn': '(Tensor q, Tensor k_pages, Tensor v_pages, Tensor table, Tensor lengths, float? scale, float softcap, Tensor? slopes, '
                   'Tensor(a!)? weights, Tensor? key_pos) -> Tensor',

@@ -29,15 +29,16 @@
 static constexpr int RG = 64;                                  // tokens a document range covers
 
 struct MaskP {
-  const char *q, *k, *v, *o, *d_o;
-  char *out, *dq, *dk, *dv;
+  const char *q, *k, *v, *o, *res, *d_o;
+  char *out, *res_out, *dq, *dk, *dv;
   float *lse, *delta;
   const float* slopes;
   const int *doc_q, *doc_k, *prefix;
   const int4 *rq, *rk;                                         // (smallest id >= 0, largest id, 1 if any is negative, 0) of RG tokens
   long qs[3], ks[3], vs[3], os[3], dos[3], dqs[3], dks[3], dvs[3], dcs[2];
   float* part;                                                 // split key blocks: [nsplit][dv, dk][B][Sk][Hk][D]
-  int B, Sq, Sk, H, Hk, G, D, causal, off, nsplit;
+  float *qpart, *ml;                                           // split keys: sums [qsplit][B][Sq][H][D], (m, l) [qsplit][B][Sq][H][2]
+  int B, Sq, Sk, H, Hk, G, D, causal, off, nsplit, qsplit;
   float scale, softcap;
 };
 
@@ -267,6 +268,14 @@ struct Score {
   }
 };
 
+// four elements e .. of an output row, and what their rounding left (for the backward pass' do.o) where it is asked for
+template <class T> __device__ __forceinline__ void store_out(const MaskP& p, long at, long row, int e, const f32x4& x) {
+  store4((T*)p.out + at + e, x[0], x[1], x[2], x[3]);
+  if constexpr (sizeof(T) == 2)
+    if (p.res_out)
+      store4((T*)p.res_out + row * p.D + e, x[0] - (float)(T)x[0], x[1] - (float)(T)x[1], x[2] - (float)(T)x[2], x[3] - (float)(T)x[3]);
+}
+
 // acc += what the encoded tile's rows that `seen` admits add to each column
 template <class TL, int R, int ND, class F> __device__ __forceinline__ void add_seen(f32x16 (&acc)[ND], const char* lds, F&& seen) {
   const int half = (threadIdx.x & 63) >> 5;
@@ -327,7 +336,7 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void attn_masked_fwd_k
   }
   const int tend = p.causal ? min(p.Sk, max(qlast + p.off + 1, prefix)) : p.Sk;
   Tiles<RG / KT> it;
-  it.init(rk, 0, (max(tend, 0) + KT - 1) / KT, qr.x, qr.y);
+  it.init(rk, 0, (max(tend, 0) + KT - 1) / KT, qr.x, qr.y, p.qsplit, blockIdx.z);
 
   auto whole = [&](int t) {                                      // every pair of the tile is seen
     const int a = t * KT, z = a + KT - 1;
@@ -448,7 +457,7 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void attn_masked_fwd_k
   if (lane == 0) sbad[wave] = dirty;
   __syncthreads();
   if (any_flag<4>(sbad)) {
-    it.init(rk, 0, (max(tend, 0) + KT - 1) / KT, qr.x, qr.y);
+    it.init(rk, 0, (max(tend, 0) + KT - 1) / KT, qr.x, qr.y, p.qsplit, blockIdx.z);
     for (t = it.next(); t >= 0; t = it.next()) {
       if (whole(t)) continue;
       __syncthreads();
@@ -460,16 +469,53 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void attn_masked_fwd_k
   }
   l += __shfl_xor(l, 32);
   if (!iok) return;
+  const long row = ((long)hd.b * p.Sq + i) * p.H + hd.h;
+  if (p.qsplit > 1) {
+    const long at = blockIdx.z * (long)p.B * p.Sq * p.H + row;
+    float* part = p.qpart + at * p.D;
+#pragma unroll
+    for (int d = 0; d < ND; ++d)
+#pragma unroll
+      for (int r = 0; r < 16; r += 4) {
+        const int e = d * 32 + mfma32_row(r, half);
+        if (e < p.D) *(f32x4*)(part + e) = f32x4{o[d][r], o[d][r + 1], o[d][r + 2], o[d][r + 3]};
+      }
+    if (half == 0) { p.ml[2 * at] = m; p.ml[2 * at + 1] = l; }
+    return;
+  }
   const float inv = l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l);
-  T* out = (T*)p.out + hd.b * p.os[0] + (long)i * p.os[1] + hd.h * p.os[2];
+  const long at = hd.b * p.os[0] + (long)i * p.os[1] + hd.h * p.os[2];
 #pragma unroll
   for (int d = 0; d < ND; ++d)
 #pragma unroll
     for (int r = 0; r < 16; r += 4) {
       const int e = d * 32 + mfma32_row(r, half);
-      if (e < p.D) store4(out + e, o[d][r] * inv, o[d][r + 1] * inv, o[d][r + 2] * inv, o[d][r + 3] * inv);
+      if (e < p.D) store_out<T>(p, at, row, e, f32x4{o[d][r] * inv, o[d][r + 1] * inv, o[d][r + 2] * inv, o[d][r + 3] * inv});
     }
   if (half == 0) p.lse[((long)hd.b * p.H + hd.h) * p.Sq + i] = l == 0.f ? NEG_INF : m + log2f(l);
+}
+
+// Split keys joined: four elements of a row a thread, the splits in order
+template <class T>
+__global__ __launch_bounds__(256) void attn_masked_join_kernel(MaskP p) {
+  const int nd = p.D / 4;
+  const long rows = (long)p.B * p.Sq * p.H, n = (long)blockIdx.x * 256 + threadIdx.x, row = n / nd;
+  if (row >= rows) return;
+  const int d = (int)(n - row * nd) * 4;
+  float m = NEG_INF, l = 0.f;
+  for (int s = 0; s < p.qsplit; ++s) m = fmaxf(m, p.ml[2 * (s * rows + row)]);
+  const float base = m == NEG_INF ? 0.f : m;
+  f32x4 a{0.f, 0.f, 0.f, 0.f};
+  for (int s = 0; s < p.qsplit; ++s) {
+    const long at = s * rows + row;
+    const float f = exp2_hw(p.ml[2 * at] - base);
+    l += p.ml[2 * at + 1] * f;
+    a += *(const f32x4*)(p.qpart + at * p.D + d) * f;
+  }
+  const float inv = l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l);
+  const long bi = row / p.H, h = row - bi * p.H, b = bi / p.Sq, i = bi - b * p.Sq;
+  store_out<T>(p, b * p.os[0] + i * p.os[1] + h * p.os[2], row, d, a * inv);
+  if (d == 0) p.lse[(b * p.H + h) * p.Sq + i] = l == 0.f ? NEG_INF : m + log2f(l);
 }
 
 // ---- gradient of the queries -----------------------------------------------------------------------------------------------------
@@ -507,11 +553,22 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void attn_masked_dq_ke
           delta += half_to_float<T>((u16)(of[c][w] >> 16)) * half_to_float<T>((u16)(df[c][w] >> 16));
         }
       }
+    if constexpr (sizeof(T) == 2)
+      if (p.res) {                                               // what the output's rounding left
+        own_row<T, NP>(of, (const T*)p.res + (((long)hd.b * p.Sq + i) * p.H + hd.h) * p.D, iok, p.D);
+#pragma unroll
+        for (int c = 0; c < NP; ++c)
+#pragma unroll
+          for (int w = 0; w < 4; ++w) {
+            delta += half_to_float<T>((u16)of[c][w]) * half_to_float<T>((u16)df[c][w]);
+            delta += half_to_float<T>((u16)(of[c][w] >> 16)) * half_to_float<T>((u16)(df[c][w] >> 16));
+          }
+      }
     delta += __shfl_xor(delta, 32);
   }
   float lse = iok ? p.lse[at] : __builtin_inff();
   if (lse == NEG_INF) { lse = __builtin_inff(); delta = 0.f; }   // sees nothing: every probability is zero
-  if (iok && half == 0) p.delta[at] = delta;
+  if (iok && half == 0 && blockIdx.z == 0) p.delta[at] = delta;
   const Score sc(p, hd.h);
   const int prefix = p.prefix ? p.prefix[hd.b] : 0;
   const int myid = p.doc_q ? (iok ? p.doc_q[hd.b * p.dcs[0] + i] : -1) : 0;
@@ -530,7 +587,7 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void attn_masked_dq_ke
   }
   const int tend = p.causal ? min(p.Sk, max(qlast + p.off + 1, prefix)) : p.Sk;
   Tiles<RG / KT> it;
-  it.init(rk, 0, (max(tend, 0) + KT - 1) / KT, qr.x, qr.y);
+  it.init(rk, 0, (max(tend, 0) + KT - 1) / KT, qr.x, qr.y, p.qsplit, blockIdx.z);
   auto whole = [&](int t) {
     const int a = t * KT, z = a + KT - 1;
     if (z >= p.Sk) return false;
@@ -632,7 +689,7 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void attn_masked_dq_ke
   if (lane == 0) sbad[wave] = dirty;
   __syncthreads();
   if (any_flag<4>(sbad)) {
-    it.init(rk, 0, (max(tend, 0) + KT - 1) / KT, qr.x, qr.y);
+    it.init(rk, 0, (max(tend, 0) + KT - 1) / KT, qr.x, qr.y, p.qsplit, blockIdx.z);
     for (t = it.next(); t >= 0; t = it.next()) {
       if (whole(t)) continue;
       __syncthreads();
@@ -644,12 +701,15 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void attn_masked_dq_ke
   }
   if (!iok) return;
   T* out = (T*)p.dq + hd.b * p.dqs[0] + (long)i * p.dqs[1] + hd.h * p.dqs[2];
+  float* part = p.qpart + (((long)blockIdx.z * p.B + hd.b) * p.Sq + i) * p.H * p.D + (long)hd.h * p.D;
 #pragma unroll
   for (int d = 0; d < ND; ++d)
 #pragma unroll
     for (int r = 0; r < 16; r += 4) {
       const int e = d * 32 + mfma32_row(r, half);
-      if (e < p.D) store4(out + e, dq[d][r] * p.scale, dq[d][r + 1] * p.scale, dq[d][r + 2] * p.scale, dq[d][r + 3] * p.scale);
+      if (e >= p.D) continue;
+      if (p.qsplit == 1) store4(out + e, dq[d][r] * p.scale, dq[d][r + 1] * p.scale, dq[d][r + 2] * p.scale, dq[d][r + 3] * p.scale);
+      else *(f32x4*)(part + e) = f32x4{dq[d][r], dq[d][r + 1], dq[d][r + 2], dq[d][r + 3]};
     }
 }
 
@@ -658,7 +718,7 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void attn_masked_dq_ke
 // one more).  S is formed twice, 40 tile products instead of 32, but a wave then needs 64 accumulators instead of 128 and two waves
 // fit a SIMD, one's exponentials under the other's matrix work: a single wave with both took 978 us where this takes #### (2 x 4096
 // tokens, 16 heads of 128).  Where the key blocks are few, `nsplit` workgroups share the query tiles of one (every nsplit-th tile, so
-// the split is even under a causal mask too); their 32-bit sums are added in order by dkv_join_kernel.
+// the split is even under a causal mask too); their 32-bit sums are added in order by sum_join_kernel.
 template <class T, int DP, int QT, int NT>
 __global__ __launch_bounds__(NT, NT / 256) void attn_masked_dkv_kernel(MaskP p) {
   using TL = Tile<T, DP, QT, NT>;
@@ -862,19 +922,22 @@ __global__ __launch_bounds__(NT, NT / 256) void attn_masked_dkv_kernel(MaskP p) 
     }
 }
 
-// dk, dv = the splits' sums, in order; four elements a thread, dk on blockIdx.y = 1
+// out[b, t, h] = mul times the sum of the splits [n][B][S][H][D], in order; four elements a thread
+struct SumP { const float* part; char* out; long st[3], next; int n, S, H, D; float mul; };
 template <class T>
-__global__ __launch_bounds__(256) void dkv_join_kernel(MaskP p) {
-  const long n = (long)p.B * p.Sk * p.Hk * p.D, i = ((long)blockIdx.x * 256 + threadIdx.x) * 4;
-  const int keys = blockIdx.y;
-  if (i >= n) return;
-  f32x4 a = *(const f32x4*)(p.part + keys * n + i);
-  for (int s = 1; s < p.nsplit; ++s) a += *(const f32x4*)(p.part + (2L * s + keys) * n + i);
-  const float mul = keys ? p.scale : 1.f;
+__global__ __launch_bounds__(256) void sum_join_kernel(SumP p, long total) {
+  const long i = ((long)blockIdx.x * 256 + threadIdx.x) * 4;
+  if (i >= total) return;
+  f32x4 a = *(const f32x4*)(p.part + i);
+  for (int s = 1; s < p.n; ++s) a += *(const f32x4*)(p.part + s * p.next + i);
   const int d = (int)(i % p.D);
-  const long row = i / p.D, hk = row % p.Hk, bt = row / p.Hk, t = bt % p.Sk, b = bt / p.Sk;
-  const long* st = keys ? p.dks : p.dvs;
-  store4((T*)(keys ? p.dk : p.dv) + b * st[0] + t * st[1] + hk * st[2] + d, a[0] * mul, a[1] * mul, a[2] * mul, a[3] * mul);
+  const long row = i / p.D, h = row % p.H, bt = row / p.H, t = bt % p.S, b = bt / p.S;
+  store4((T*)p.out + b * p.st[0] + t * p.st[1] + h * p.st[2] + d, a[0] * p.mul, a[1] * p.mul, a[2] * p.mul, a[3] * p.mul);
+}
+template <class T>
+static void sum_join(const float* part, char* out, const long* st, long next, int n, int B, int S, int H, int D, float mul, hipStream_t stream) {
+  const long total = (long)B * S * H * D;
+  hipLaunchKernelGGL(sum_join_kernel<T>, dim3(cdiv(total, 1024)), dim3(256), 0, stream, SumP{part, out, {st[0], st[1], st[2]}, next, n, S, H, D, mul}, total);
 }
 
 // ---- C entries -----------------------------------------------------------------------------------------------------------------------
@@ -911,53 +974,67 @@ template <class F> static void with_tile(int dtype, int D, F&& f) {
   });
 }
 
-// Workgroups that share a key block's query tiles: a power of two, until the 128-key blocks of all key heads fill the chip's 256 CUs
-// twice (one workgroup a CU at a time; two rounds even out a causal mask), never more than there are tiles.  Each split writes and reads
-// 16 bytes a key element more, the backward of 2 x 4096 tokens on 2 x 4 key heads of 128 gains #### over one split.
-static int dkv_split(int B, int Sq, int Sk, int Hk) {
-  const long blocks = (long)B * Hk * ((Sk + 127) / 128);
+// Where the blocks of 128 queries (or of keys) are too few for the chip's 256 CUs twice over, several workgroups share the tiles of one
+// block, every n-th tile each (even under a causal mask), a power of two of them (split keys: with at least four tiles each).  Their 32-bit sums go
+// through a workspace: 8 bytes an element and split more.  2047 queries on 8191 keys, 16 heads of 64: #### us in one piece, #### in two.
+static int mask_split(long blocks, int tiles) {
   int n = 1;
-  while (n < 16 && blocks * n < 512 && 2 * n <= (Sq + 63) / 64) n *= 2;
+  while (n < 16 && blocks * n < 512 && 8 * n <= tiles) n *= 2;
   return n;
 }
-// Floats of scratch the backward pass needs: delta, and the sums of split key blocks
-static long bwd_floats(int B, int Sq, int Sk, int H, int Hk, int D, long* delta) {
-  *delta = ((long)B * H * Sq + 3) / 4 * 4;
-  const int n = dkv_split(B, Sq, Sk, Hk);
-  return *delta + (n > 1 ? 2L * n * B * Sk * Hk * D : 0);
+static int q_split(int B, int Sq, int Sk, int H) { return mask_split((long)B * H * ((Sq + 127) / 128), (Sk + 63) / 64); }
+static int k_split(int B, int Sq, int Sk, int Hk) { return mask_split((long)B * Hk * ((Sk + 127) / 128), (Sq + 63) / 64 * 4); }
+// Floats of scratch: forward (sums, then (m, l), of split keys); backward (delta, sums of split keys, sums of split queries)
+static long fwd_floats(int B, int Sq, int Sk, int H, int D) {
+  const int n = q_split(B, Sq, Sk, H);
+  return n > 1 ? (long)n * B * Sq * H * (D + 2) : 0;
 }
-extern "C" int aot_attn_masked_bwd_floats(int B, int Sq, int Sk, int H, int Hk, int D, long* floats) {
+struct BwdWork { long qpart, part, all; };
+static BwdWork bwd_floats(int B, int Sq, int Sk, int H, int Hk, int D) {
+  const int n = q_split(B, Sq, Sk, H), m = k_split(B, Sq, Sk, Hk);
+  BwdWork w;
+  w.qpart = ((long)B * H * Sq + 3) / 4 * 4;
+  w.part = w.qpart + (n > 1 ? (long)n * B * Sq * H * D : 0);
+  w.all = w.part + (m > 1 ? 2L * m * B * Sk * Hk * D : 0);
+  return w;
+}
+extern "C" int aot_attn_masked_floats(int B, int Sq, int Sk, int H, int Hk, int D, int backward, long* floats) {
   if (!floats || B < 0 || Sq < 0 || Sk < 0 || Hk < 1 || H < Hk || H % Hk || D < 1) return AOT_ERR_BADARG;
-  long delta;
-  *floats = bwd_floats(B, Sq, Sk, H, Hk, D, &delta);
+  *floats = backward ? bwd_floats(B, Sq, Sk, H, Hk, D).all : fwd_floats(B, Sq, Sk, H, D);
   return AOT_OK;
 }
 
-extern "C" int aot_attn_masked(const void* q, const void* k, const void* v, void* out, float* lse, const float* slopes, const int* doc_q,
-                               const int* doc_k, const int* prefix, void* ranges, int dtype, int B, int Sq, int Sk, int H, int Hk, int D,
+extern "C" int aot_attn_masked(const void* q, const void* k, const void* v, void* out, void* residual, float* lse, const float* slopes,
+                               const int* doc_q, const int* doc_k, const int* prefix, void* ranges, float* work, long work_floats, int dtype, int B, int Sq, int Sk, int H, int Hk, int D,
                                int causal, float scale, float softcap, const long* strides, void* stream) {
   int rc = mask_args(dtype, B, Sq, Sk, H, Hk, D, softcap, doc_q, doc_k, ranges, strides);
   if (rc) return rc;
   if (B == 0 || Sq == 0) return AOT_OK;
   if (!q || !out || !lse || (Sk && (!k || !v))) return AOT_ERR_BADARG;
   MaskP p{};
-  p.q = (const char*)q; p.k = (const char*)k; p.v = (const char*)v; p.out = (char*)out; p.lse = lse;
+  p.q = (const char*)q; p.k = (const char*)k; p.v = (const char*)v; p.out = (char*)out; p.res_out = (char*)residual; p.lse = lse;
   for (int i = 0; i < 3; ++i) { p.qs[i] = strides[i]; p.ks[i] = strides[3 + i]; p.vs[i] = strides[6 + i]; p.os[i] = strides[9 + i]; }
   p.dcs[0] = strides[12]; p.dcs[1] = strides[13];
   const int es = dtype_size(dtype);
   if (!rows_aligned(q, p.qs, es) || !rows_aligned(k, p.ks, es) || !rows_aligned(v, p.vs, es) || !rows_aligned(out, p.os, es)) return AOT_ERR_BADARG;
   mask_common(p, B, Sq, Sk, H, Hk, D, causal, scale, softcap, slopes, doc_q, doc_k, prefix, ranges);
+  const long need = fwd_floats(B, Sq, Sk, H, D);
+  if (!aligned16(residual) || (need && (!work || !aligned16(work) || work_floats < need))) return AOT_ERR_BADARG;
+  p.qsplit = q_split(B, Sq, Sk, H);
+  p.qpart = work;
+  p.ml = work + (long)p.qsplit * B * Sq * H * D;
   hipStream_t st = (hipStream_t)stream;
   if (doc_q) range_launch(p, st);
-  const dim3 grid(B * H, cdiv(Sq, 128));
+  const dim3 grid(B * H, cdiv(Sq, 128), p.qsplit);
   with_tile(dtype, D, [&](auto t, auto dp, auto kt) {
     hipLaunchKernelGGL((attn_masked_fwd_kernel<decltype(t), decltype(dp)::value, decltype(kt)::value>), grid, dim3(256), 0, st, p);
+    if (p.qsplit > 1) hipLaunchKernelGGL(attn_masked_join_kernel<decltype(t)>, dim3(cdiv((long)B * Sq * H * (D / 4), 256)), dim3(256), 0, st, p);
   });
   AOT_LAUNCH_CHECK();
 }
 
-extern "C" int aot_attn_masked_bwd(const void* q, const void* k, const void* v, const void* out, const float* lse, const void* dout, void* dq, void* dk,
-                                   void* dv, const float* slopes, const int* doc_q, const int* doc_k, const int* prefix, void* ranges, float* work, long work_floats,
+extern "C" int aot_attn_masked_bwd(const void* q, const void* k, const void* v, const void* out, const void* residual, const float* lse,
+                                   const void* dout, void* dq, void* dk, void* dv, const float* slopes, const int* doc_q, const int* doc_k, const int* prefix, void* ranges, float* work, long work_floats,
                                    int dtype, int B, int Sq, int Sk, int H, int Hk, int D, int causal, float scale, float softcap, const long* strides,
                                    void* stream) {
   int rc = mask_args(dtype, B, Sq, Sk, H, Hk, D, softcap, doc_q, doc_k, ranges, strides);
@@ -965,7 +1042,7 @@ extern "C" int aot_attn_masked_bwd(const void* q, const void* k, const void* v, 
   if (B == 0 || (Sq == 0 && Sk == 0)) return AOT_OK;
   if ((Sq && (!q || !out || !lse || !dout || !dq)) || (Sk && (!k || !v || !dk || !dv))) return AOT_ERR_BADARG;
   MaskP p{};
-  p.q = (const char*)q; p.k = (const char*)k; p.v = (const char*)v; p.o = (const char*)out; p.d_o = (const char*)dout;
+  p.q = (const char*)q; p.k = (const char*)k; p.v = (const char*)v; p.o = (const char*)out; p.res = (const char*)residual; p.d_o = (const char*)dout;
   p.lse = (float*)lse; p.dq = (char*)dq; p.dk = (char*)dk; p.dv = (char*)dv;
   for (int i = 0; i < 3; ++i) {
     p.qs[i] = strides[i]; p.ks[i] = strides[3 + i]; p.vs[i] = strides[6 + i]; p.os[i] = strides[9 + i]; p.dos[i] = strides[12 + i];
@@ -976,22 +1053,31 @@ extern "C" int aot_attn_masked_bwd(const void* q, const void* k, const void* v, 
   if (!rows_aligned(q, p.qs, es) || !rows_aligned(k, p.ks, es) || !rows_aligned(v, p.vs, es) || !rows_aligned(out, p.os, es) ||
       !rows_aligned(dout, p.dos, es) || !rows_aligned(dq, p.dqs, es) || !rows_aligned(dk, p.dks, es) || !rows_aligned(dv, p.dvs, es) ||
       !aligned16(work)) return AOT_ERR_BADARG;
-  long delta;
-  if (!work || work_floats < bwd_floats(B, Sq, Sk, H, Hk, D, &delta)) return AOT_ERR_BADARG;
+  const BwdWork w = bwd_floats(B, Sq, Sk, H, Hk, D);
+  if (!aligned16(residual) || (w.all && (!work || work_floats < w.all))) return AOT_ERR_BADARG;
   p.delta = work;
-  p.part = work + delta;
-  p.nsplit = dkv_split(B, Sq, Sk, Hk);
+  p.qpart = work + w.qpart;
+  p.part = work + w.part;
+  p.qsplit = q_split(B, Sq, Sk, H);
+  p.nsplit = k_split(B, Sq, Sk, Hk);
   mask_common(p, B, Sq, Sk, H, Hk, D, causal, scale, softcap, slopes, doc_q, doc_k, prefix, ranges);
   hipStream_t st = (hipStream_t)stream;
   if (doc_q) range_launch(p, st);
   with_tile(dtype, D, [&](auto t, auto dp, auto kt) {
     constexpr int KT = decltype(dp)::value == 128 ? 32 : 64;     // (two 64-row tiles of 128 columns in flight cost spills here)
-    if (Sq) hipLaunchKernelGGL((attn_masked_dq_kernel<decltype(t), decltype(dp)::value, KT>), dim3(B * H, cdiv(Sq, 128)), dim3(256), 0, st, p);
+    if (Sq) {
+      hipLaunchKernelGGL((attn_masked_dq_kernel<decltype(t), decltype(dp)::value, KT>), dim3(B * H, cdiv(Sq, 128), p.qsplit), dim3(256), 0, st, p);
+      if (p.qsplit > 1) sum_join<decltype(t)>(p.qpart, p.dq, p.dqs, (long)B * Sq * H * D, p.qsplit, B, Sq, H, D, scale, st);
+    }
     if (Sk) {
       constexpr int NT = sizeof(t) == 4 && decltype(dp)::value == 128 ? 256 : 512;
       hipLaunchKernelGGL((attn_masked_dkv_kernel<decltype(t), decltype(dp)::value, decltype(kt)::value, NT>), dim3(B * Hk, cdiv(Sk, NT / 4), p.nsplit),
                          dim3(NT), 0, st, p);
-      if (p.nsplit > 1) hipLaunchKernelGGL((dkv_join_kernel<decltype(t)>), dim3(cdiv((long)B * Sk * Hk * D, 1024), 2), dim3(256), 0, st, p);
+      if (p.nsplit > 1) {
+        const long n = (long)B * Sk * Hk * D;
+        sum_join<decltype(t)>(p.part, p.dv, p.dvs, 2 * n, p.nsplit, B, Sk, Hk, D, 1.f, st);
+        sum_join<decltype(t)>(p.part + n, p.dk, p.dks, 2 * n, p.nsplit, B, Sk, Hk, D, scale, st);
+      }
     }
   });
   AOT_LAUNCH_CHECK();

@@ -111,7 +111,6 @@ __global__ __launch_bounds__(SEL_T) void evict_select_kernel(EvictP p) {
     tie = t < t1 && mid && want > 0 && key == thr;
   };
   int heavier = 0, equal = 0;
-#pragma unroll 4
   for (int t = t0 + lane; t < t0 + per; t += 64) {
     bool sure, tie;
     kind(t, t < t1 ? w[t] : 0.f, sure, tie);
@@ -128,7 +127,6 @@ __global__ __launch_bounds__(SEL_T) void evict_select_kernel(EvictP p) {
   float* nw = p.new_weights + b * p.nws[0] + h * p.nws[1];
   const int* pos = p.pos ? p.pos + b * p.pss[0] + h * p.pss[1] : nullptr;
   int* np = p.pos ? p.new_pos + b * p.nps[0] + h * p.nps[1] : nullptr;
-#pragma unroll 4
   for (int t = t0 + lane; t < t0 + per; t += 64) {
     const float x = t < t1 ? w[t] : 0.f;
     bool sure, tie;

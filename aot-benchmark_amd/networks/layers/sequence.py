@@ -87,16 +87,16 @@ class _RopeOne(Function):
 class _MaskedAttention(Function):
     @staticmethod
     def forward(ctx, q, k, v, slopes, doc_q, doc_k, prefix, scale, causal, softcap):
-        out, lse = aot_hip.attn_masked(q, k, v, scale, causal, softcap, slopes, doc_q, doc_k, prefix)
-        ctx.save_for_backward(q, k, v, out, lse, slopes, doc_q, doc_k, prefix)
+        out, lse, res = aot_hip.attn_masked(q, k, v, scale, causal, softcap, slopes, doc_q, doc_k, prefix, residual=any(ctx.needs_input_grad[:3]))
+        ctx.save_for_backward(q, k, v, out, lse, res, slopes, doc_q, doc_k, prefix)
         ctx.more = (scale, causal, softcap)
         return out
 
     @staticmethod
     @once_differentiable
     def backward(ctx, dout):
-        q, k, v, out, lse, slopes, doc_q, doc_k, prefix = ctx.saved_tensors
-        return aot_hip.attn_masked_bwd(dout, q, k, v, out, lse, *ctx.more, slopes, doc_q, doc_k, prefix) + (None,) * 7
+        q, k, v, out, lse, res, slopes, doc_q, doc_k, prefix = ctx.saved_tensors
+        return aot_hip.attn_masked_bwd(dout, q, k, v, out, lse, res, *ctx.more, slopes, doc_q, doc_k, prefix) + (None,) * 7
 
 
 def masked_attention(q, k, v, scale=None, causal=False, softcap=0.0, slopes=None, doc_q=None, doc_k=None, prefix=None):

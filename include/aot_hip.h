@@ -542,20 +542,25 @@ int aot_rope_append(const void* q, const void* k, const void* v, void* qo, void*
  * Key t is seen if (not causal, or t <= i + Sk - Sq, or t < prefix[b]) and (no documents, or doc_q[b, i] == doc_k[b, t] >= 0).  A negative
  * document id marks padding.  What masked places hold (NaN, infinities) does not reach the result.  prefix [B] or NULL (read with causal
  * only); doc_q [B, Sq] / doc_k [B, Sk] both or neither, then `ranges` is scratch of 16 * B * (ceil(Sq / 64) + ceil(Sk / 64)) bytes, 16-byte
- * aligned.  D <= 128, rows of whole 16-byte pieces, 16-byte aligned.  Sq, Sk <= 2^22.
+ * aligned.  residual (16-bit types, dense [B, Sq, H, D], or NULL): what rounding out left, for the backward call.  work: scratch of
+ * aot_attn_masked_floats(.., 0, ..) floats (0: may be NULL), 16-byte aligned.  D <= 128, rows of whole 16-byte pieces, 16-byte aligned, outputs
+ * too.  Sq, Sk <= 2^22.
  * strides: q b s h, k b s h, v b s h, out b s h, doc_q b, doc_k b (14).  Beside aot_attn_f32 (attention.py:82-117). */
-int aot_attn_masked(const void* q, const void* k, const void* v, void* out, float* lse, const float* slopes, const int* doc_q,
-                    const int* doc_k, const int* prefix, void* ranges, int dtype, int B, int Sq, int Sk, int H, int Hk, int D,
+int aot_attn_masked(const void* q, const void* k, const void* v, void* out, void* residual, float* lse, const float* slopes,
+                    const int* doc_q, const int* doc_k, const int* prefix, void* ranges, float* work, long work_floats, int dtype, int B, int Sq, int Sk, int H, int Hk, int D,
                     int causal, float scale, float softcap, const long* strides, void* stream);
 /* Its gradients: out and lse from the forward call on the same arguments, dout -> dq, dk, dv (key heads: summed over the query heads
- * that share them); work: scratch of aot_attn_masked_bwd_floats floats, 16-byte aligned.  Probabilities and score gradients are rounded to `dtype` for the products they
+ * that share them); residual as written by the forward call, or NULL
+ * (do.o is then formed from the rounded output: for 16-bit types its error adds about a third to dq's and dk's); work: scratch of
+ * aot_attn_masked_floats(.., 1, ..) floats, 16-byte aligned.  Probabilities and score gradients are rounded to `dtype` for the products they
  * enter (fp16: what is below 6e-8 is lost, as in any fp16 gradient -- scale the loss).  No atomics: results repeat bit for bit.
  * strides: q k v out dout dq dk dv (b s h each), doc_q b, doc_k b (26). */
-int aot_attn_masked_bwd(const void* q, const void* k, const void* v, const void* out, const float* lse, const void* dout, void* dq, void* dk,
-                        void* dv, const float* slopes, const int* doc_q, const int* doc_k, const int* prefix, void* ranges, float* work, long work_floats,
+int aot_attn_masked_bwd(const void* q, const void* k, const void* v, const void* out, const void* residual, const float* lse,
+                        const void* dout, void* dq, void* dk, void* dv, const float* slopes, const int* doc_q, const int* doc_k, const int* prefix, void* ranges, float* work, long work_floats,
                         int dtype, int B, int Sq, int Sk, int H, int Hk, int D, int causal, float scale, float softcap, const long* strides,
                         void* stream);
-int aot_attn_masked_bwd_floats(int B, int Sq, int Sk, int H, int Hk, int D, long* floats);
+/* Floats of `work` of the two calls above */
+int aot_attn_masked_floats(int B, int Sq, int Sk, int H, int Hk, int D, int backward, long* floats);
 
 /* Attention of ONE new token per sequence over a paged cache: q / out [B, H, D]; entry t < lengths[b] of sequence b lies at place t % page
  * of page table[b, t / page] (max_pages a row) of k_pages / v_pages.  The new token's own key and value are already in the cache (entry

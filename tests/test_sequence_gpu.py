@@ -548,9 +548,9 @@ def test_dispatcher_ops_are_the_same_calls(seq):
         a, b = ops.rope(q, k, pos, freqs, False, 1.0, False)
         c, d = seq.rope(q, k, pos, freqs)
         assert torch.equal(a, c) and torch.equal(b, d)
-        out, lse = ops.attn_masked(q, k, v, None, True, 5.0, None, None, None, None)
+        out, lse, res = ops.attn_masked(q, k, v, None, True, 5.0, None, None, None, None, True)
         assert torch.equal(out, seq.masked_attention(q, k, v, causal=True, softcap=5.0)) and lse.shape == (1, 2, 70)
-        g = ops.attn_masked_bwd(q, q, k, v, out, lse, None, True, 5.0, None, None, None, None)
+        g = ops.attn_masked_bwd(q, q, k, v, out, lse, res, None, True, 5.0, None, None, None, None)
         assert [x.shape for x in g] == [q.shape, k.shape, v.shape]
         kp, vp, table, _ = cache(2, 40, 16, 2, 64, dt, 3)
         n = torch.tensor([40, 7], dtype=torch.int32, device='cuda')

@@ -34,16 +34,16 @@ def test_c_entries_refuse_before_any_launch():
         assert append(**bad) == -1, bad
     assert append(pages=1 << 28) == -2 and append(N=0) == 0
 
-    def masked(dtype=0, B=1, Sq=1, Sk=1, H=1, Hk=1, D=32, cap=0.0, q=P(16), k=P(16), dq=None, dk=None, rng=None, st=z14, lse=P(16)):
-        return lib.aot_attn_masked(q, k, P(16), P(16), lse, None, dq, dk, None, rng, dtype, B, Sq, Sk, H, Hk, D, 1, 1.0, cap, st, None)
+    def masked(dtype=0, B=1, Sq=1, Sk=1, H=1, Hk=1, D=32, cap=0.0, q=P(16), k=P(16), dq=None, dk=None, rng=None, st=z14, lse=P(16), res=None):
+        return lib.aot_attn_masked(q, k, P(16), P(16), res, lse, None, dq, dk, None, rng, None, 0, dtype, B, Sq, Sk, H, Hk, D, 1, 1.0, cap, st, None)
     for bad in (dict(dtype=7), dict(H=3, Hk=2), dict(Hk=0), dict(cap=-1.0), dict(cap=math.nan), dict(dq=P(16)), dict(dq=P(16), dk=P(16)), dict(q=P(24)), dict(q=None),
-                dict(k=None), dict(lse=None), dict(st=None), dict(st=L(0, 33, *[0] * 12)), dict(Sq=-1), dict(D=0)):
+                dict(k=None), dict(lse=None), dict(st=None), dict(res=P(24)), dict(Sk=4096), dict(st=L(0, 33, *[0] * 12)), dict(Sq=-1), dict(D=0)):
         assert masked(**bad) == -1, bad
     assert masked(D=132) == -2 and masked(D=33) == -2 and masked(dtype=1, D=36) == -2 and masked(Sk=(1 << 22) + 1) == -2
     assert masked(B=0) == 0 and masked(Sq=0, q=None) == 0
 
     def bwd(Sq=1, Sk=1, dk=P(16), delta=P(16), do=P(16), st=z26, D=32, floats=1 << 20):
-        return lib.aot_attn_masked_bwd(P(16), P(16), P(16), P(16), P(16), do, P(16), dk, P(16), None, None, None, None, None, delta, floats, 2, 1, Sq, Sk, 1, 1, D, 0,
+        return lib.aot_attn_masked_bwd(P(16), P(16), P(16), P(16), None, P(16), do, P(16), dk, P(16), None, None, None, None, None, delta, floats, 2, 1, Sq, Sk, 1, 1, D, 0,
                                        1.0, 0.0, st, None)
     assert bwd(floats=3) == -1 and bwd(delta=P(20)) == -1 and bwd(dk=P(24)) == -1 and bwd(dk=None) == -1 and bwd(delta=None) == -1 and bwd(do=P(18)) == -1 and bwd(st=None) == -1 and bwd(D=136) == -2
     assert bwd(Sq=0, Sk=0, dk=None) == 0
