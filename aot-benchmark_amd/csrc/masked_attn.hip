@@ -86,17 +86,23 @@ template <class T> __device__ __forceinline__ void pack_tile(const f32x16& p, u3
 template <class T, int DP, int R, int NT> struct Tile {           // NT threads stage it
   static constexpr int CE = Elem<T>::CE, NCH = DP / CE, N = (R * NCH + NT - 1) / NT, ROWB = DP * (int)sizeof(T), BYTES = R * ROWB;
   static constexpr bool EVEN = R * NCH % NT == 0;                 // (else some threads have nothing to stage)
-  static __device__ __forceinline__ int at(int row, int c) {      // byte offset of piece c of a row
-    if constexpr (NCH >= 16) {
-      const int f = sizeof(T) == 2 ? ((row & 3) << 2) | ((row >> 2) & 3) : ((row & 4) << 1) | ((row & 8) >> 1) | (row & 3);
-      return row * ROWB + ((c ^ f) << 4);
-    } else if constexpr (NCH == 8) {
-      const int l = row >> 1, f = sizeof(T) == 2 ? ((l & 1) << 2) | ((l >> 1) & 3) : (l & 7) | ((l & 2) << 2);
-      return l * 256 + ((((row & 1) * 8 + c) ^ f) << 4);
-    } else {
-      const int l = row >> 2;
-      return l * 256 + ((((row & 3) * 4 + c) ^ (l & 3)) << 4);
-    }
+  // Byte offset of piece c of a row: its line, and a swizzled place in the line.  `place` is linear over xor in the bits of row and c,
+  // so at(row + dr, c + dc) = (at(row, c) ^ place(dr, dc) * 16) + line(dr) * 256 where the bits do not overlap: a lane keeps one offset
+  // for each way of reading and a read's own constants cost one xor, not a register each.
+  static constexpr __device__ __forceinline__ int place(int row, int c) {
+    if constexpr (NCH >= 16) return c ^ (sizeof(T) == 2 ? ((row & 3) << 2) | ((row >> 2) & 3) : ((row & 4) << 1) | ((row & 8) >> 1) | (row & 3));
+    else if constexpr (NCH == 8) {
+      const int l = row >> 1;
+      return ((row & 1) * 8 + c) ^ (sizeof(T) == 2 ? ((l & 1) << 2) | ((l >> 1) & 3) : (l & 7) | ((l & 2) << 2));
+    } else return ((row & 3) * 4 + c) ^ ((row >> 2) & 3);
+  }
+  static constexpr __device__ __forceinline__ int line(int row) { return (row * ROWB) & -(NCH >= 16 ? ROWB : 256); }
+  static __device__ __forceinline__ int at(int row, int c) { return line(row) + (place(row, c) << 4); }
+  static __device__ __forceinline__ int row_base() { return at(threadIdx.x & 31, (threadIdx.x >> 5) & 1); }
+  static __device__ __forceinline__ int col_base() {
+    const int lane = threadIdx.x & 63, i = lane & 15;
+    if constexpr (sizeof(T) == 2) return at(4 * (lane >> 5) + (i >> 2), ((lane >> 4) & 1) * 2 + ((i & 3) >> 1)) + (i & 1) * 8;
+    else return at(4 * (lane >> 5), (lane & 31) >> 2) + (lane & 3) * 4;
   }
   static __device__ __forceinline__ void pack(const f32x16& p, u32x4 (&pk)[2]) { pack_tile<T>(p, pk); }
   struct Regs { u32x4 r[N]; };
@@ -152,39 +158,35 @@ template <class T, int DP, int R, int NT> struct Tile {           // NT threads 
       if (EVEN || n < R * NCH) *(u32x4*)(lds + at(n / NCH, n % NCH)) = g.r[i];
     }
   }
-  // first operand of a product over the columns: lane = row row0 + (lane & 31), piece 2 c + lane / 32
-  static __device__ __forceinline__ u32x4 rows(const char* lds, int row0, int c) {
-    const int lane = threadIdx.x & 63;
-    return *(const u32x4*)(lds + row0 * ROWB + at(lane & 31, 2 * c + (lane >> 5)));
+  // first operand of a product over the columns: lane = row 32 n + (lane & 31), piece 2 c + lane / 32.  o: the tile's offset + row_base()
+  static __device__ __forceinline__ u32x4 rows(const char* lds, int o, int n, int c) {
+    return *(const u32x4*)(lds + (o ^ (place(0, 2 * c) << 4)) + n * 32 * ROWB);
   }
-  // 16-bit: first operand of a product over 16 rows (row0 + 16 kb ..) of the tile, in score-tile order: lane = column 32 db + (lane & 31)
-  static __device__ __forceinline__ u32x4 col16(const char* lds, int row0, int db, int kb) {
-    const int lane = threadIdx.x & 63, i = lane & 15, c = db * 4 + ((lane >> 4) & 1) * 2 + ((i & 3) >> 1), sub = (i & 1) * 8;
+  // 16-bit: first operand of a product over 16 rows (32 n + 16 kb ..) of the tile, in score-tile order: lane = column 32 db + (lane & 31).
+  // o: the tile's offset + col_base()
+  static __device__ __forceinline__ u32x4 col16(const char* lds, int o, int n, int db, int kb) {
+    typedef short s16x4 __attribute__((ext_vector_type(4)));
+    typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
     u32x4 a;
 #pragma unroll
     for (int s = 0; s < 2; ++s) {
-      const int row = 8 * s + 4 * (lane >> 5) + (i >> 2);
-      typedef short s16x4 __attribute__((ext_vector_type(4)));
-      typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
-      const s16x4 x = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(lds + (row0 + 16 * kb) * ROWB + at(row, c) + sub));
+      const s16x4 x = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(lds + (o ^ (place(8 * s, 4 * db) << 4)) + line(8 * s) + (32 * n + 16 * kb) * ROWB));
       const u32x2 y = __builtin_bit_cast(u32x2, x);
       a[2 * s] = y[0];
       a[2 * s + 1] = y[1];
     }
     return a;
   }
-  // acc[column 32 db + i][lane's own column] += sum over rows row0 .. row0 + 31 of tile[row][column] * p[row], p in score-tile order
-  static __device__ __forceinline__ f32x16 cols(const char* lds, int row0, int db, const u32x4 (&pk)[2], const f32x16& p, f32x16 acc) {
-    const int lane = threadIdx.x & 63;
+  // acc[column 32 db + i][lane's own column] += sum over rows 32 n .. of tile[row][column] * p[row], p in score-tile order
+  static __device__ __forceinline__ f32x16 cols(const char* lds, int o, int n, int db, const u32x4 (&pk)[2], const f32x16& p, f32x16 acc) {
     if constexpr (sizeof(T) == 2) {
 #pragma unroll
-      for (int kb = 0; kb < 2; ++kb) acc = mfma32<T>(col16(lds, row0, db, kb), pk[kb], acc);
+      for (int kb = 0; kb < 2; ++kb) acc = mfma32<T>(col16(lds, o, n, db, kb), pk[kb], acc);
     } else {
-      const int d = db * 32 + (lane & 31), c = d / CE, e = d % CE;
 #pragma unroll
       for (int r = 0; r < 16; ++r) {
-        const int row = mfma32_row(r & 7, lane >> 5);
-        const float a = *(const float*)(lds + (row0 + 16 * (r >> 3)) * ROWB + at(row, c) + e * 4);
+        const int dr = mfma32_row(r & 7, 0);
+        const float a = *(const float*)(lds + (o ^ (place(dr, 8 * db) << 4)) + line(dr) + (32 * n + 16 * (r >> 3)) * ROWB);
         acc = __builtin_amdgcn_mfma_f32_32x32x2f32(a, p[r], acc, 0, 0, 0);
       }
     }
@@ -278,7 +280,7 @@ template <class T> __device__ __forceinline__ void store_out(const MaskP& p, lon
 
 // acc += what the encoded tile's rows that `seen` admits add to each column
 template <class TL, int R, int ND, class F> __device__ __forceinline__ void add_seen(f32x16 (&acc)[ND], const char* lds, F&& seen) {
-  const int half = (threadIdx.x & 63) >> 5;
+  const int half = (threadIdx.x & 63) >> 5, cb = TL::col_base();
 #pragma unroll 1
   for (int n = 0; n < R / 32; ++n) {
     f32x16 one;
@@ -292,7 +294,7 @@ template <class TL, int R, int ND, class F> __device__ __forceinline__ void add_
       f32x16 z;
 #pragma unroll
       for (int r = 0; r < 16; ++r) z[r] = 0.f;
-      z = TL::cols(lds, n * 32, d, pk, one, z);
+      z = TL::cols(lds, cb, n, d, pk, one, z);
 #pragma unroll
       for (int r = 0; r < 16; ++r) acc[d][r] += TL::decode(z[r]);
     }
@@ -305,8 +307,9 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void attn_masked_fwd_k
   using TL = Tile<T, DP, KT, 256>;
   constexpr int NP = TL::NCH / 2, ND = DP / 32, NS = KT / 32;
   __shared__ __align__(16) char smem[4 * TL::BYTES + 2 * KT * 4 + 32];      // K, V of two tiles; ids; flags of the waves
-  auto sk = [&](int buf) { return smem + buf * TL::BYTES; };
-  auto sv = [&](int buf) { return smem + (2 + buf) * TL::BYTES; };
+  const int rb = TL::row_base(), cb = TL::col_base();
+  auto sk = [&](int buf) { return buf * TL::BYTES; };          // offsets of the tiles
+  auto sv = [&](int buf) { return (2 + buf) * TL::BYTES; };
   int* const sid = (int*)(smem + 4 * TL::BYTES);                // [2][KT]
   int* const sbad = sid + 2 * KT;                               // [4]
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, half = lane >> 5;
@@ -362,8 +365,8 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void attn_masked_fwd_k
   };
   auto put = [&](int buf, bool full) {
     if (!full) dirty |= TL::clean(gv);
-    TL::store(sk(buf), gk);
-    TL::store(sv(buf), gv);
+    TL::store(smem + sk(buf), gk);
+    TL::store(smem + sv(buf), gv);
     if (threadIdx.x < KT) sid[buf * KT + threadIdx.x] = gid;
   };
 
@@ -389,7 +392,7 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void attn_masked_fwd_k
 #pragma unroll
       for (int r = 0; r < 16; ++r) s[n][r] = 0.f;
 #pragma unroll
-      for (int c = 0; c < NP; ++c) s[n] = mfma32<T>(TL::rows(sk(buf), n * 32, c), qf[c], s[n]);
+      for (int c = 0; c < NP; ++c) s[n] = mfma32<T>(TL::rows(smem, sk(buf) + rb, n, c), qf[c], s[n]);
     }
     // in powers of two: s * m0 (plain scores are left as they are, the scale goes into the exponential's argument)
     float m0 = sc.mul;
@@ -445,7 +448,7 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void attn_masked_fwd_k
       u32x4 pk[2];
       pack_tile<T>(s[n], pk);
 #pragma unroll
-      for (int d = 0; d < ND; ++d) o[d] = TL::cols(sv(buf), n * 32, d, pk, s[n], o[d]);
+      for (int d = 0; d < ND; ++d) o[d] = TL::cols(smem, sv(buf) + cb, n, d, pk, s[n], o[d]);
     }
     if (tn >= 0) put(buf ^ 1, fulln);
     __syncthreads();
@@ -524,8 +527,9 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void attn_masked_dq_ke
   using TL = Tile<T, DP, KT, 256>;
   constexpr int NP = TL::NCH / 2, ND = DP / 32, NS = KT / 32;
   __shared__ __align__(16) char smem[4 * TL::BYTES + 2 * KT * 4 + 32];
-  auto sk = [&](int buf) { return smem + buf * TL::BYTES; };
-  auto sv = [&](int buf) { return smem + (2 + buf) * TL::BYTES; };
+  const int rb = TL::row_base(), cb = TL::col_base();
+  auto sk = [&](int buf) { return buf * TL::BYTES; };          // offsets of the tiles
+  auto sv = [&](int buf) { return (2 + buf) * TL::BYTES; };
   int* const sid = (int*)(smem + 4 * TL::BYTES);
   int* const sbad = sid + 2 * KT;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, half = lane >> 5;
@@ -611,8 +615,8 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void attn_masked_dq_ke
   };
   auto put = [&](int buf, bool full) {
     if (!full) dirty |= TL::clean(gk);
-    TL::store(sk(buf), gk);
-    TL::store(sv(buf), gv);
+    TL::store(smem + sk(buf), gk);
+    TL::store(smem + sv(buf), gv);
     if (threadIdx.x < KT) sid[buf * KT + threadIdx.x] = gid;
   };
   f32x16 dq[ND];
@@ -636,9 +640,9 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void attn_masked_dq_ke
 #pragma unroll
       for (int r = 0; r < 16; ++r) { s[r] = 0.f; dp[r] = 0.f; }
 #pragma unroll
-      for (int c = 0; c < NP; ++c) s = mfma32<T>(TL::rows(sk(buf), n * 32, c), qf[c], s);
+      for (int c = 0; c < NP; ++c) s = mfma32<T>(TL::rows(smem, sk(buf) + rb, n, c), qf[c], s);
 #pragma unroll
-      for (int c = 0; c < NP; ++c) dp = mfma32<T>(TL::rows(sv(buf), n * 32, c), df[c], dp);
+      for (int c = 0; c < NP; ++c) dp = mfma32<T>(TL::rows(smem, sv(buf) + rb, n, c), df[c], dp);
 #pragma unroll
       for (int r = 0; r < 16; ++r) dp[r] -= delta;
       float m0 = sc.mul;
@@ -677,7 +681,7 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void attn_masked_dq_ke
       u32x4 pk[2];
       pack_tile<T>(s, pk);
 #pragma unroll
-      for (int d = 0; d < ND; ++d) dq[d] = TL::cols(sk(buf), n * 32, d, pk, s, dq[d]);
+      for (int d = 0; d < ND; ++d) dq[d] = TL::cols(smem, sk(buf) + cb, n, d, pk, s, dq[d]);
     }
     if (tn >= 0) put(buf ^ 1, fulln);
     __syncthreads();
@@ -725,8 +729,9 @@ __global__ __launch_bounds__(NT, NT / 256) void attn_masked_dkv_kernel(MaskP p) 
   constexpr int NW = NT / 128, KEYS = 32 * NW;                  // waves of either kind; keys of the workgroup
   constexpr int NP = TL::NCH / 2, ND = DP / 32, NS = QT / 32;
   __shared__ __align__(16) char smem[4 * TL::BYTES + 6 * QT * 4 + 64];      // Q, dO of two tiles; lse, delta, ids; flags of the waves
-  auto sq = [&](int buf) { return smem + buf * TL::BYTES; };
-  auto sd = [&](int buf) { return smem + (2 + buf) * TL::BYTES; };
+  const int rb = TL::row_base(), cb = TL::col_base();
+  auto sq = [&](int buf) { return buf * TL::BYTES; };          // offsets of the tiles
+  auto sd = [&](int buf) { return (2 + buf) * TL::BYTES; };
   float* const slse = (float*)(smem + 4 * TL::BYTES);           // [2][QT]
   float* const sdel = slse + 2 * QT;
   int* const sid = (int*)(sdel + 2 * QT);
@@ -802,8 +807,8 @@ __global__ __launch_bounds__(NT, NT / 256) void attn_masked_dkv_kernel(MaskP p) 
         dirty |= TL::clean(gq);
         dirty |= TL::clean(gd);
       }
-      TL::store(sq(buf), gq);
-      TL::store(sd(buf), gd);
+      TL::store(smem + sq(buf), gq);
+      TL::store(smem + sd(buf), gd);
       if (threadIdx.x < QT) {
         slse[buf * QT + threadIdx.x] = glse;
         sdel[buf * QT + threadIdx.x] = gdel;
@@ -827,13 +832,13 @@ __global__ __launch_bounds__(NT, NT / 256) void attn_masked_dkv_kernel(MaskP p) 
 #pragma unroll
         for (int r = 0; r < 16; ++r) s[r] = 0.f;
 #pragma unroll
-        for (int c = 0; c < NP; ++c) s = mfma32<T>(TL::rows(sq(buf), n * 32, c), kf[c], s);
+        for (int c = 0; c < NP; ++c) s = mfma32<T>(TL::rows(smem, sq(buf) + rb, n, c), kf[c], s);
         float m0 = sc.mul;
         if (keys) {
 #pragma unroll
           for (int r = 0; r < 16; ++r) dp[r] = 0.f;
 #pragma unroll
-          for (int c = 0; c < NP; ++c) dp = mfma32<T>(TL::rows(sd(buf), n * 32, c), vf[c], dp);
+          for (int c = 0; c < NP; ++c) dp = mfma32<T>(TL::rows(smem, sd(buf) + rb, n, c), vf[c], dp);
 #pragma unroll
           for (int r4 = 0; r4 < 4; ++r4) {
             const f32x4 de = *(const f32x4*)(sdel + buf * QT + n * 32 + 8 * r4 + 4 * half);
@@ -877,9 +882,9 @@ __global__ __launch_bounds__(NT, NT / 256) void attn_masked_dkv_kernel(MaskP p) 
         }
         u32x4 pk[2];
         pack_tile<T>(s, pk);
-        const char* x = keys ? sq(buf) : sd(buf);
+        const int x = (keys ? sq(buf) : sd(buf)) + cb;
 #pragma unroll
-        for (int d = 0; d < ND; ++d) acc[d] = TL::cols(x, n * 32, d, pk, s, acc[d]);
+        for (int d = 0; d < ND; ++d) acc[d] = TL::cols(smem, x, n, d, pk, s, acc[d]);
       }
       if (tn >= 0) put(buf ^ 1, fulln);
       __syncthreads();
@@ -898,11 +903,11 @@ __global__ __launch_bounds__(NT, NT / 256) void attn_masked_dkv_kernel(MaskP p) 
       for (int tq = it.next(); tq >= 0; tq = it.next()) {
         if (whole(tq)) continue;
         __syncthreads();
-        TL::encode(sq(0), (const T*)p.q + b * p.qs[0] + h * p.qs[2], p.qs[1], tq * QT, p.Sq, p.D);
-        TL::encode(sd(0), (const T*)p.d_o + b * p.dos[0] + h * p.dos[2], p.dos[1], tq * QT, p.Sq, p.D);
+        TL::encode(smem + sq(0), (const T*)p.q + b * p.qs[0] + h * p.qs[2], p.qs[1], tq * QT, p.Sq, p.D);
+        TL::encode(smem + sd(0), (const T*)p.d_o + b * p.dos[0] + h * p.dos[2], p.dos[1], tq * QT, p.Sq, p.D);
         if (threadIdx.x < QT) sid[threadIdx.x] = tq * QT + (int)threadIdx.x < p.Sq && p.doc_q ? p.doc_q[b * p.dcs[0] + tq * QT + threadIdx.x] : 0;
         __syncthreads();
-        add_seen<TL, QT>(acc, keys ? sq(0) : sd(0), [&](int j) { return seen(tq * QT + j, sid[j]); });
+        add_seen<TL, QT>(acc, smem + (keys ? sq(0) : sd(0)), [&](int j) { return seen(tq * QT + j, sid[j]); });
       }
     }
   }
