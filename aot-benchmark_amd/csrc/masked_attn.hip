@@ -387,6 +387,7 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void attn_masked_fwd_k
     const bool fulln = tn >= 0 && whole(tn);
     if (tn >= 0) fetch(tn);
     f32x16 s[NS];
+    __builtin_amdgcn_s_setprio(1);
 #pragma unroll
     for (int n = 0; n < NS; ++n) {
 #pragma unroll
@@ -394,6 +395,7 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void attn_masked_fwd_k
 #pragma unroll
       for (int c = 0; c < NP; ++c) s[n] = mfma32<T>(TL::rows(smem, sk(buf) + rb, n, c), qf[c], s[n]);
     }
+    __builtin_amdgcn_s_setprio(0);
     // in powers of two: s * m0 (plain scores are left as they are, the scale goes into the exponential's argument)
     float m0 = sc.mul;
     if (sc.capped) {
@@ -447,8 +449,10 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void attn_masked_fwd_k
       for (int r = 0; r < 16; ++r) { s[n][r] = exp2_hw(__builtin_fmaf(s[n][r], m0, -base)); l += s[n][r]; }
       u32x4 pk[2];
       pack_tile<T>(s[n], pk);
+      __builtin_amdgcn_s_setprio(1);
 #pragma unroll
       for (int d = 0; d < ND; ++d) o[d] = TL::cols(smem, sv(buf) + cb, n, d, pk, s[n], o[d]);
+      __builtin_amdgcn_s_setprio(0);
     }
     if (tn >= 0) put(buf ^ 1, fulln);
     __syncthreads();
@@ -639,10 +643,12 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void attn_masked_dq_ke
       f32x16 s, dp;
 #pragma unroll
       for (int r = 0; r < 16; ++r) { s[r] = 0.f; dp[r] = 0.f; }
+      __builtin_amdgcn_s_setprio(1);
 #pragma unroll
       for (int c = 0; c < NP; ++c) s = mfma32<T>(TL::rows(smem, sk(buf) + rb, n, c), qf[c], s);
 #pragma unroll
       for (int c = 0; c < NP; ++c) dp = mfma32<T>(TL::rows(smem, sv(buf) + rb, n, c), df[c], dp);
+      __builtin_amdgcn_s_setprio(0);
 #pragma unroll
       for (int r = 0; r < 16; ++r) dp[r] -= delta;
       float m0 = sc.mul;
@@ -680,8 +686,10 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void attn_masked_dq_ke
       }
       u32x4 pk[2];
       pack_tile<T>(s, pk);
+      __builtin_amdgcn_s_setprio(1);
 #pragma unroll
       for (int d = 0; d < ND; ++d) dq[d] = TL::cols(smem, sk(buf) + cb, n, d, pk, s, dq[d]);
+      __builtin_amdgcn_s_setprio(0);
     }
     if (tn >= 0) put(buf ^ 1, fulln);
     __syncthreads();
@@ -831,6 +839,7 @@ __global__ __launch_bounds__(NT, NT / 256) void attn_masked_dkv_kernel(MaskP p) 
         f32x16 s, dp;
 #pragma unroll
         for (int r = 0; r < 16; ++r) s[r] = 0.f;
+        __builtin_amdgcn_s_setprio(1);
 #pragma unroll
         for (int c = 0; c < NP; ++c) s = mfma32<T>(TL::rows(smem, sq(buf) + rb, n, c), kf[c], s);
         float m0 = sc.mul;
@@ -846,6 +855,7 @@ __global__ __launch_bounds__(NT, NT / 256) void attn_masked_dkv_kernel(MaskP p) 
             for (int w = 0; w < 4; ++w) dp[4 * r4 + w] -= de[w];
           }
         }
+        __builtin_amdgcn_s_setprio(0);
         if (sc.capped) {
           m0 = 1.f;
 #pragma unroll
@@ -883,8 +893,10 @@ __global__ __launch_bounds__(NT, NT / 256) void attn_masked_dkv_kernel(MaskP p) 
         u32x4 pk[2];
         pack_tile<T>(s, pk);
         const int x = (keys ? sq(buf) : sd(buf)) + cb;
+        __builtin_amdgcn_s_setprio(1);
 #pragma unroll
         for (int d = 0; d < ND; ++d) acc[d] = TL::cols(smem, x, n, d, pk, s, acc[d]);
+        __builtin_amdgcn_s_setprio(0);
       }
       if (tn >= 0) put(buf ^ 1, fulln);
       __syncthreads();
