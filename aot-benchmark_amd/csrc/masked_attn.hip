@@ -726,21 +726,24 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void attn_masked_dq_ke
 }
 
 // ---- gradients of the keys and values ----------------------------------------------------------------------------------------------
-// Eight waves own 128 keys (four own 64 where a wave of 128 fp32 columns needs all registers), two waves the same 32: the first half form dv (S and one more product a tile), the others dk (S, do.v and
-// one more).  S is formed twice, 40 tile products instead of 32, but a wave then needs 64 accumulators instead of 128 and two waves
-// fit a SIMD, one's exponentials under the other's matrix work: a single wave with both took 978 us where this takes #### (2 x 4096
-// tokens, 16 heads of 128).  Where the key blocks are few, `nsplit` workgroups share the query tiles of one (every nsplit-th tile, so
-// the split is even under a causal mask too); their 32-bit sums are added in order by sum_join_kernel.
+// Eight waves own 128 keys (four own 64 where a wave of 128 fp32 columns needs all registers), two waves the same 32.  The first half of the
+// waves forms S, the probabilities and dv; the second half do.v, the score gradients and dk.  A wave then needs 64 accumulators (D = 128)
+// instead of 128 and two waves fit a SIMD, one's exponentials under the other's matrix work.  The probabilities (times the cap's derivative)
+// go through shared memory in 32 bits, lane to lane, and the second wave uses them one tile later, so the tile's one barrier suffices: the
+// tile of Q is kept a turn longer (three buffers).  One wave with both sums took 978 us for 2 x 4096 tokens and 16 heads of 128, two waves
+// that both formed S 984, this takes 837.  Where the key blocks are few, `nsplit` workgroups share the query tiles of one (every
+// nsplit-th tile, so the split is even under a causal mask too); their 32-bit sums are added in order by sum_join_kernel.
 template <class T, int DP, int QT, int NT>
 __global__ __launch_bounds__(NT, NT / 256) void attn_masked_dkv_kernel(MaskP p) {
   using TL = Tile<T, DP, QT, NT>;
   constexpr int NW = NT / 128, KEYS = 32 * NW;                  // waves of either kind; keys of the workgroup
   constexpr int NP = TL::NCH / 2, ND = DP / 32, NS = QT / 32;
-  __shared__ __align__(16) char smem[4 * TL::BYTES + 6 * QT * 4 + 64];      // Q, dO of two tiles; lse, delta, ids; flags of the waves
+  constexpr int XB = NW * NS * 4096;                            // probabilities of a tile: [pair][half tile][4][lane][4] floats
+  __shared__ __align__(16) char smem[5 * TL::BYTES + 2 * XB + 6 * QT * 4 + 64];   // dO of two tiles, Q of three; probabilities; lse, delta, ids; flags
   const int rb = TL::row_base(), cb = TL::col_base();
-  auto sq = [&](int buf) { return buf * TL::BYTES; };          // offsets of the tiles
-  auto sd = [&](int buf) { return (2 + buf) * TL::BYTES; };
-  float* const slse = (float*)(smem + 4 * TL::BYTES);           // [2][QT]
+  auto sd = [&](int buf) { return buf * TL::BYTES; };          // offsets of the tiles
+  auto sq = [&](int q3) { return (2 + q3) * TL::BYTES; };
+  float* const slse = (float*)(smem + 5 * TL::BYTES + 2 * XB);  // [2][QT]
   float* const sdel = slse + 2 * QT;
   int* const sid = (int*)(sdel + 2 * QT);
   int* const sbad = sid + 2 * QT;                               // [8]
@@ -750,9 +753,12 @@ __global__ __launch_bounds__(NT, NT / 256) void attn_masked_dkv_kernel(MaskP p) 
   const int k0 = blockIdx.y * KEYS;                               // (causal: the first keys are seen by most queries)
   const int t = k0 + (wave & (NW - 1)) * 32 + (lane & 31);
   const bool tok = t < p.Sk;
-  u32x4 kf[NP], vf[NP];
-  own_row<T, NP>(kf, (const T*)p.k + b * p.ks[0] + (long)t * p.ks[1] + hk * p.ks[2], tok, p.D);
-  own_row<T, NP>(vf, (const T*)p.v + b * p.vs[0] + (long)t * p.vs[1] + hk * p.vs[2], tok && keys, p.D);
+  u32x4 wf[NP];                                                 // the key's row of K, or (dk) of V
+  {
+    const long* st = keys ? p.vs : p.ks;
+    own_row<T, NP>(wf, (const T*)(keys ? p.v : p.k) + b * st[0] + (long)t * st[1] + hk * st[2], tok, p.D);
+  }
+  auto exchange = [&](int buf, int n) { return (f32x4*)(smem + 5 * TL::BYTES + buf * XB + ((wave & (NW - 1)) * NS + n) * 4096) + lane; };
   const int prefix = p.prefix ? p.prefix[b] : 0;
   const int myid = p.doc_k ? (tok ? p.doc_k[b * p.dcs[1] + t] : -1) : 0;
   const int klast = min(k0 + KEYS - 1, p.Sk - 1);
@@ -790,128 +796,188 @@ __global__ __launch_bounds__(NT, NT / 256) void attn_masked_dkv_kernel(MaskP p) 
   float glse = 0.f, gdel = 0.f;
   int gid = 0;
   bool dirty = false;
-  for (int g = 0; g < p.G; ++g) {
+  const Score sc(p, hk * p.G);                                   // (its slope is the first head's: taken per tile below)
+  // the tiles of all query heads that share the key head, one after the other
+  Tiles<RG / QT> it;
+  int g = 0;
+  auto start = [&]() { it.init(rq, first, (p.Sq + QT - 1) / QT, kr.x, kr.y, p.nsplit, split); };
+  auto next = [&]() {
+    int x = it.next();
+    while (x < 0 && ++g < p.G) {
+      start();
+      x = it.next();
+    }
+    return x;
+  };
+  auto fetch = [&](int tq, int g) {
     const int h = hk * p.G + g;
-    const T* Q = (const T*)p.q + b * p.qs[0] + h * p.qs[2];
-    const T* DO = (const T*)p.d_o + b * p.dos[0] + h * p.dos[2];
-    const float* lse = p.lse + ((long)b * p.H + h) * p.Sq;
-    const float* del = p.delta + ((long)b * p.H + h) * p.Sq;
-    const Score sc(p, h);
-    Tiles<RG / QT> it;
-    it.init(rq, first, (p.Sq + QT - 1) / QT, kr.x, kr.y, p.nsplit, split);
-    auto fetch = [&](int tq) {
-      TL::load(gq, Q, p.qs[1], tq * QT, p.Sq, p.D);
-      TL::load(gd, DO, p.dos[1], tq * QT, p.Sq, p.D);
-      if (threadIdx.x < QT) {
-        const int i = tq * QT + threadIdx.x;
-        glse = i < p.Sq ? lse[i] : __builtin_inff();
-        if (glse == NEG_INF) glse = __builtin_inff();            // sees nothing: every probability is zero
-        gdel = i < p.Sq ? del[i] : 0.f;
-        gid = p.doc_q ? (i < p.Sq ? p.doc_q[b * p.dcs[0] + i] : -1) : 0;
-      }
-    };
-    auto put = [&](int buf, bool full) {
-      if (!full) {
-        dirty |= TL::clean(gq);
-        dirty |= TL::clean(gd);
-      }
-      TL::store(smem + sq(buf), gq);
-      TL::store(smem + sd(buf), gd);
-      if (threadIdx.x < QT) {
-        slse[buf * QT + threadIdx.x] = glse;
-        sdel[buf * QT + threadIdx.x] = gdel;
-        sid[buf * QT + threadIdx.x] = gid;
-      }
-    };
-    __syncthreads();
-    int tq = it.next(), buf = 0;
-    bool full = tq >= 0 && whole(tq);
-    if (tq >= 0) fetch(tq);
-    __syncthreads();
-    if (tq >= 0) put(0, full);
-    __syncthreads();
-    while (tq >= 0) {
-      const int tn = it.next();
-      const bool fulln = tn >= 0 && whole(tn);
-      if (tn >= 0) fetch(tn);
+    TL::load(gq, (const T*)p.q + b * p.qs[0] + h * p.qs[2], p.qs[1], tq * QT, p.Sq, p.D);
+    TL::load(gd, (const T*)p.d_o + b * p.dos[0] + h * p.dos[2], p.dos[1], tq * QT, p.Sq, p.D);
+    if (threadIdx.x < QT) {
+      const int i = tq * QT + threadIdx.x;
+      const long at = ((long)b * p.H + h) * p.Sq + i;
+      glse = i < p.Sq ? p.lse[at] : __builtin_inff();
+      if (glse == NEG_INF) glse = __builtin_inff();              // sees nothing: every probability is zero
+      gdel = i < p.Sq ? p.delta[at] : 0.f;
+      gid = p.doc_q ? (i < p.Sq ? p.doc_q[b * p.dcs[0] + i] : -1) : 0;
+    }
+  };
+  auto put = [&](int buf, int q3, bool full) {
+    if (!full) {
+      dirty |= TL::clean(gq);
+      dirty |= TL::clean(gd);
+    }
+    TL::store(smem + sq(q3), gq);
+    TL::store(smem + sd(buf), gd);
+    if (threadIdx.x < QT) {
+      slse[buf * QT + threadIdx.x] = glse;
+      sdel[buf * QT + threadIdx.x] = gdel;
+      sid[buf * QT + threadIdx.x] = gid;
+    }
+  };
+  start();
+  int tq = next(), gcur = g, buf = 0, q3 = 0, qprev = 0;
+  bool full = tq >= 0 && whole(tq);
+  if (tq >= 0) {
+    fetch(tq, gcur);
+    put(0, 0, full);
+  }
+  __syncthreads();
+  auto walk = [&](auto role) {                                 // (a loop of its own for either kind of wave: same tiles, same barriers)
+    f32x16 dp[NS];                                               // dk's waves: do.v - D of the tile, until its probabilities are there
+    auto finish = [&]() {                                        // dk of the tile before: its probabilities, its rows of Q
 #pragma unroll
       for (int n = 0; n < NS; ++n) {
-        f32x16 s, dp;
+        __builtin_amdgcn_sched_barrier(0);                     // (one half tile at a time: both at once do not fit the registers)
+        const f32x4* x = exchange(buf ^ 1, n);
 #pragma unroll
-        for (int r = 0; r < 16; ++r) s[r] = 0.f;
+        for (int r4 = 0; r4 < 4; ++r4) {
+          const f32x4 pr = x[64 * r4];
+#pragma unroll
+          for (int w = 0; w < 4; ++w) dp[n][4 * r4 + w] = pr[w] == 0.f ? 0.f : pr[w] * dp[n][4 * r4 + w];     // (a masked pair's do.v may be anything)
+        }
+        u32x4 pk[2];
+        pack_tile<T>(dp[n], pk);
         __builtin_amdgcn_s_setprio(1);
 #pragma unroll
-        for (int c = 0; c < NP; ++c) s = mfma32<T>(TL::rows(smem, sq(buf) + rb, n, c), kf[c], s);
-        float m0 = sc.mul;
-        if (keys) {
+        for (int d = 0; d < ND; ++d) acc[d] = TL::cols(smem, sq(qprev) + cb, n, d, pk, dp[n], acc[d]);
+        __builtin_amdgcn_s_setprio(0);
+      }
+    };
+    if constexpr (decltype(role)::value) {                     // nothing before the first tile: probabilities of zero
 #pragma unroll
-          for (int r = 0; r < 16; ++r) dp[r] = 0.f;
+      for (int n = 0; n < NS; ++n)
 #pragma unroll
-          for (int c = 0; c < NP; ++c) dp = mfma32<T>(TL::rows(smem, sd(buf) + rb, n, c), vf[c], dp);
+        for (int r4 = 0; r4 < 4; ++r4) {
+          exchange(1, n)[64 * r4] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+          for (int w = 0; w < 4; ++w) dp[n][4 * r4 + w] = 0.f;
+        }
+    }
+    for (;;) {
+      if constexpr (decltype(role)::value)
+        finish();
+      if (tq < 0) break;
+      const int tn = next(), gn = g;
+      const bool fulln = tn >= 0 && whole(tn);
+      if (tn >= 0) fetch(tn, gn);
+      if constexpr (decltype(role)::value) {
+#pragma unroll
+        for (int n = 0; n < NS; ++n) {
+#pragma unroll
+          for (int r = 0; r < 16; ++r) dp[n][r] = 0.f;
+          __builtin_amdgcn_sched_barrier(0);
+          __builtin_amdgcn_s_setprio(1);
+#pragma unroll
+          for (int c = 0; c < NP; ++c) dp[n] = mfma32<T>(TL::rows(smem, sd(buf) + rb, n, c), wf[c], dp[n]);
+          __builtin_amdgcn_s_setprio(0);
 #pragma unroll
           for (int r4 = 0; r4 < 4; ++r4) {
             const f32x4 de = *(const f32x4*)(sdel + buf * QT + n * 32 + 8 * r4 + 4 * half);
 #pragma unroll
-            for (int w = 0; w < 4; ++w) dp[4 * r4 + w] -= de[w];
+            for (int w = 0; w < 4; ++w) dp[n][4 * r4 + w] -= de[w];
           }
         }
-        __builtin_amdgcn_s_setprio(0);
-        if (sc.capped) {
-          m0 = 1.f;
+      } else {
 #pragma unroll
-          for (int r = 0; r < 16; ++r) {
-            const float th = tanh_from_exp2(s[r] * sc.mul);
-            s[r] = sc.cap2 * th;
-            if (keys) dp[r] *= 1.f - th * th;
+        for (int n = 0; n < NS; ++n) {
+          f32x16 s, dcap;
+#pragma unroll
+          for (int r = 0; r < 16; ++r) s[r] = 0.f;
+          __builtin_amdgcn_sched_barrier(0);
+          __builtin_amdgcn_s_setprio(1);
+#pragma unroll
+          for (int c = 0; c < NP; ++c) s = mfma32<T>(TL::rows(smem, sq(q3) + rb, n, c), wf[c], s);
+          __builtin_amdgcn_s_setprio(0);
+          float m0 = sc.mul;
+          if (sc.capped) {
+            m0 = 1.f;
+#pragma unroll
+            for (int r = 0; r < 16; ++r) {
+              const float th = tanh_from_exp2(s[r] * sc.mul);
+              s[r] = sc.cap2 * th;
+              dcap[r] = 1.f - th * th;
+            }
           }
-        }
-        if (p.slopes) {
-          const float far = (float)(tq * QT + n * 32 + 4 * half + p.off - t);
+          if (p.slopes) {
+            const float slope = p.slopes[hk * p.G + gcur] * LOG2E, far = (float)(tq * QT + n * 32 + 4 * half + p.off - t);
 #pragma unroll
-          for (int r = 0; r < 16; ++r) s[r] = s[r] * m0 - sc.slope * fabsf(far + (float)mfma32_row(r, 0));
-          m0 = 1.f;
-        }
-#pragma unroll
-        for (int r4 = 0; r4 < 4; ++r4) {
-          const f32x4 ls = *(const f32x4*)(slse + buf * QT + n * 32 + 8 * r4 + 4 * half);
-#pragma unroll
-          for (int w = 0; w < 4; ++w) s[4 * r4 + w] = exp2_hw(__builtin_fmaf(s[4 * r4 + w], m0, -ls[w]));
-        }
-        if (keys)
-#pragma unroll
-          for (int r = 0; r < 16; ++r) s[r] *= dp[r];
-        if (!full) {
+            for (int r = 0; r < 16; ++r) s[r] = s[r] * m0 - slope * fabsf(far + (float)mfma32_row(r, 0));
+            m0 = 1.f;
+          }
 #pragma unroll
           for (int r4 = 0; r4 < 4; ++r4) {
-            const int j0 = n * 32 + 8 * r4 + 4 * half;
-            const i32x4 id = *(const i32x4*)(sid + buf * QT + j0);
+            const f32x4 ls = *(const f32x4*)(slse + buf * QT + n * 32 + 8 * r4 + 4 * half);
 #pragma unroll
-            for (int w = 0; w < 4; ++w)
-              if (j0 + w < lim - tq * QT || id[w] != myid) s[4 * r4 + w] = 0.f;
+            for (int w = 0; w < 4; ++w) s[4 * r4 + w] = exp2_hw(__builtin_fmaf(s[4 * r4 + w], m0, -ls[w]));
           }
-        }
-        u32x4 pk[2];
-        pack_tile<T>(s, pk);
-        const int x = (keys ? sq(buf) : sd(buf)) + cb;
-        __builtin_amdgcn_s_setprio(1);
+          if (!full) {
 #pragma unroll
-        for (int d = 0; d < ND; ++d) acc[d] = TL::cols(smem, x, n, d, pk, s, acc[d]);
-        __builtin_amdgcn_s_setprio(0);
+            for (int r4 = 0; r4 < 4; ++r4) {
+              const int j0 = n * 32 + 8 * r4 + 4 * half;
+              const i32x4 id = *(const i32x4*)(sid + buf * QT + j0);
+#pragma unroll
+              for (int w = 0; w < 4; ++w)
+                if (j0 + w < lim - tq * QT || id[w] != myid) s[4 * r4 + w] = 0.f;
+            }
+          }
+          f32x4* x = exchange(buf, n);
+          if (sc.capped)
+#pragma unroll
+            for (int r4 = 0; r4 < 4; ++r4)
+              x[64 * r4] = f32x4{s[4 * r4] * dcap[4 * r4], s[4 * r4 + 1] * dcap[4 * r4 + 1], s[4 * r4 + 2] * dcap[4 * r4 + 2], s[4 * r4 + 3] * dcap[4 * r4 + 3]};
+          else
+#pragma unroll
+            for (int r4 = 0; r4 < 4; ++r4) x[64 * r4] = f32x4{s[4 * r4], s[4 * r4 + 1], s[4 * r4 + 2], s[4 * r4 + 3]};
+          u32x4 pk[2];
+          pack_tile<T>(s, pk);
+          __builtin_amdgcn_s_setprio(1);
+#pragma unroll
+          for (int d = 0; d < ND; ++d) acc[d] = TL::cols(smem, sd(buf) + cb, n, d, pk, s, acc[d]);
+          __builtin_amdgcn_s_setprio(0);
+        }
       }
-      if (tn >= 0) put(buf ^ 1, fulln);
+      const int qn = q3 == 2 ? 0 : q3 + 1;
+      if (tn >= 0) put(buf ^ 1, qn, fulln);
       __syncthreads();
       buf ^= 1;
+      qprev = q3;
+      q3 = qn;
       tq = tn;
+      gcur = gn;
       full = fulln;
     }
+  };
+  if (tq >= 0) {
+    if (keys) walk(std::true_type{});
+    else walk(std::false_type{});
   }
   if (lane == 0) sbad[wave] = dirty;
   __syncthreads();
   if (any_flag<NT / 64>(sbad)) {                                      // as in the forward kernel, over both sides' rows
     for (int g = 0; g < p.G; ++g) {
       const int h = hk * p.G + g;
-      Tiles<RG / QT> it;
-      it.init(rq, first, (p.Sq + QT - 1) / QT, kr.x, kr.y, p.nsplit, split);
+      start();
       for (int tq = it.next(); tq >= 0; tq = it.next()) {
         if (whole(tq)) continue;
         __syncthreads();
