@@ -848,7 +848,6 @@ __global__ __launch_bounds__(NT, NT / 256) void attn_masked_dkv_kernel(MaskP p) 
     auto finish = [&]() {                                        // dk of the tile before: its probabilities, its rows of Q
 #pragma unroll
       for (int n = 0; n < NS; ++n) {
-        __builtin_amdgcn_sched_barrier(0);                     // (one half tile at a time: both at once do not fit the registers)
         const f32x4* x = exchange(buf ^ 1, n);
 #pragma unroll
         for (int r4 = 0; r4 < 4; ++r4) {
@@ -886,7 +885,6 @@ __global__ __launch_bounds__(NT, NT / 256) void attn_masked_dkv_kernel(MaskP p) 
         for (int n = 0; n < NS; ++n) {
 #pragma unroll
           for (int r = 0; r < 16; ++r) dp[n][r] = 0.f;
-          __builtin_amdgcn_sched_barrier(0);
           __builtin_amdgcn_s_setprio(1);
 #pragma unroll
           for (int c = 0; c < NP; ++c) dp[n] = mfma32<T>(TL::rows(smem, sd(buf) + rb, n, c), wf[c], dp[n]);
@@ -904,7 +902,6 @@ __global__ __launch_bounds__(NT, NT / 256) void attn_masked_dkv_kernel(MaskP p) 
           f32x16 s, dcap;
 #pragma unroll
           for (int r = 0; r < 16; ++r) s[r] = 0.f;
-          __builtin_amdgcn_sched_barrier(0);
           __builtin_amdgcn_s_setprio(1);
 #pragma unroll
           for (int c = 0; c < NP; ++c) s = mfma32<T>(TL::rows(smem, sq(q3) + rb, n, c), wf[c], s);
