@@ -303,7 +303,7 @@ template <class TL, int R, int ND, class F> __device__ __forceinline__ void add_
 
 // ---- forward -------------------------------------------------------------------------------------------------------------------
 template <class T, int DP, int KT>
-__global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void attn_masked_fwd_kernel(MaskP p) {
+__global__ __launch_bounds__(256, sizeof(T) == 2 ? (DP == 64 ? 3 : 2) : 1) void attn_masked_fwd_kernel(MaskP p) {
   using TL = Tile<T, DP, KT, 256>;
   constexpr int NP = TL::NCH / 2, ND = DP / 32, NS = KT / 32;
   __shared__ __align__(16) char smem[4 * TL::BYTES + 2 * KT * 4 + 32];      // K, V of two tiles; ids; flags of the waves
