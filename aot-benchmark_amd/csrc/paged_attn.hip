@@ -27,7 +27,7 @@ struct PagedP {
   float *weights, *part, *ml, *scores;
   long qs[2], os[2], ks[3], vs[3], t_s, ws[2], ps[2];
   long num_pages, S;
-  int B, H, Hk, G, D, cap_len, page_shift, chunk, nsplit;
+  int B, H, Hk, G, D, cap_len, page_shift, chunk, nsplit, osplit;
   float scale, softcap;
 };
 
@@ -178,15 +178,11 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? (DP == 128 ? 3 : DP == 256 ? 
       x[j] = blk.ok >> j & 1 ? y : NEG_INF;
       mx = fmaxf(mx, x[j]);
     }
-    if (p.weights) {
-      if (live) {
-        float* sc = p.scores + ((long)b * p.H + h) * p.S;
+    if (p.weights && live) {                                     // (a row of scores is whole groups of four)
+      float* sc = p.scores + ((long)b * p.H + h) * p.S + t0 + kg * 4;
 #pragma unroll
-        for (int j = 0; j < 8; ++j) {
-          const int t = t0 + (j >> 2) * 16 + kg * 4 + (j & 3);
-          if (t < t_end) sc[t] = x[j];
-        }
-      }
+      for (int T2 = 0; T2 < 2; ++T2)
+        if (t0 + T2 * 16 + kg * 4 < t_end) *(f32x4*)(sc + T2 * 16) = f32x4{x[4 * T2], x[4 * T2 + 1], x[4 * T2 + 2], x[4 * T2 + 3]};
     }
     mx = fmaxf(mx, __shfl_xor(mx, 16));
     mx = fmaxf(mx, __shfl_xor(mx, 32));
@@ -277,7 +273,7 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? (DP == 128 ? 3 : DP == 256 ? 
   }
 }
 
-// First B * H workgroups: out = sum over the splits; thread groups of D / 4 take every so-many-th split, their sums are added in a fixed
+// First B * H (* osplit) workgroups: out = sum over the splits; thread groups of D / 4 take every so-many-th split, their sums are added in a fixed
 // order.  The others: weights += group sum of exp2(s - M) / L for 1024 entries of one key head, four a thread; every one forms (M, L) of its
 // heads from the splits' pairs, a wave a head.
 static constexpr int JOIN_KEYS = 1024;
@@ -289,8 +285,8 @@ __global__ __launch_bounds__(256) void paged_join_kernel(PagedP p) {
   const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63;
   const long nout = (long)p.B * p.H;
   auto live_sum = [](float l) { return l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l); };      // no entry: zero; a NaN stays one
-  if (blockIdx.x < nout) {
-    const int b = blockIdx.x / p.H, h = blockIdx.x - b * p.H;
+  if (blockIdx.x < nout * p.osplit) {
+    const int bh0 = blockIdx.x / p.osplit, cut = blockIdx.x - bh0 * p.osplit, b = bh0 / p.H, h = bh0 - b * p.H;
     const int len = max(0, min(p.lengths[b], p.cap_len)), ns = (len + p.chunk - 1) / p.chunk;
     const long at = ((long)b * p.H + h) * p.nsplit;
     const float* ml = p.ml + at * 2;
@@ -311,7 +307,7 @@ __global__ __launch_bounds__(256) void paged_join_kernel(PagedP p) {
     if (lane == 0) red[4 + wave] = l;
     __syncthreads();
     const float inv = live_sum(red[4] + red[5] + red[6] + red[7]);
-    const int nd = p.D / 4, groups = 256 / nd, g = tid / nd, d = (tid - g * nd) * 4;       // D is a multiple of 4, at most 256
+    const int nd = p.D / p.osplit / 4, groups = 256 / nd, g = tid / nd, d = cut * nd * 4 + (tid - g * nd) * 4;   // D is a multiple of 4, at most 256
     f32x4 a{0.f, 0.f, 0.f, 0.f};
     if (g < groups) {
 #pragma unroll 4
@@ -327,7 +323,7 @@ __global__ __launch_bounds__(256) void paged_join_kernel(PagedP p) {
     }
     return;
   }
-  const long w = blockIdx.x - nout;
+  const long w = blockIdx.x - nout * p.osplit;
   const int tiles = (p.cap_len + JOIN_KEYS - 1) / JOIN_KEYS;
   const int tile = (int)(w % tiles), bh = (int)(w / tiles), b = bh / p.Hk, hk = bh - b * p.Hk;
   const int len = max(0, min(p.lengths[b], p.cap_len)), ns = (len + p.chunk - 1) / p.chunk;
@@ -383,12 +379,15 @@ static int paged_chunk(long rows, long cap) {
   return std::max(128, pow2_at_least(chunk));
 }
 
+// workspace: sums [B * H][nsplit][D], their (m, l), scores [B * H][capacity in whole groups of four]
+static long score_row(long cap) { return (cap + 3) / 4 * 4; }
+static long part_floats(int B, int H, int D, int nsplit) { return ((long)B * H * nsplit * (D + 2) + 3) / 4 * 4; }
 static long paged_work(int B, int H, int Hk, int D, long cap, int with_weights, int* chunk, int* nsplit) {
   const int G = H / Hk, qt = (G + 15) / 16;
   *chunk = paged_chunk((long)B * Hk * qt, cap);
   *nsplit = (int)std::max(1L, (cap + *chunk - 1) / *chunk);
   if (*nsplit == 1 && !with_weights) return 0;
-  return (long)B * H * *nsplit * (D + 2) + (with_weights ? (long)B * H * cap : 0);
+  return part_floats(B, H, D, *nsplit) + (with_weights ? (long)B * H * score_row(cap) : 0);
 }
 
 extern "C" int aot_paged_attn_work_floats(int B, int H, int Hk, int D, int page, int max_pages, int with_weights, long* floats) {
@@ -419,14 +418,14 @@ extern "C" int aot_paged_attn(const void* q, const void* k_pages, const void* v_
   if (!aligned16(q) || !aligned16(k_pages) || !aligned16(v_pages) || p.qs[0] % a16 || p.qs[1] % a16) return AOT_ERR_BADARG;
   for (int i = 0; i < 3; ++i) if (p.ks[i] % a16 || p.vs[i] % a16) return AOT_ERR_BADARG;
   p.num_pages = num_pages;
-  p.B = B; p.H = H; p.Hk = Hk; p.G = G; p.D = D; p.cap_len = (int)cap; p.S = cap;
+  p.B = B; p.H = H; p.Hk = Hk; p.G = G; p.D = D; p.cap_len = (int)cap; p.S = score_row(cap);
   while ((1 << p.page_shift) < page) ++p.page_shift;
   p.scale = scale; p.softcap = softcap;
   const long need = paged_work(B, H, Hk, D, cap, weights != nullptr, &p.chunk, &p.nsplit);
-  if (need && (!work || work_floats < need)) return AOT_ERR_BADARG;
+  if (need && (!work || !aligned16(work) || work_floats < need)) return AOT_ERR_BADARG;
   p.part = work;
   p.ml = work + (long)B * H * p.nsplit * D;
-  p.scores = p.ml + (long)B * H * p.nsplit * 2;
+  p.scores = work + part_floats(B, H, D, p.nsplit);
   const bool split = need > 0;
   const dim3 grid(p.nsplit, Hk * qt, B);
   hipStream_t st = (hipStream_t)stream;
@@ -444,7 +443,8 @@ extern "C" int aot_paged_attn(const void* q, const void* k_pages, const void* v_
   hipError_t e = hipGetLastError();
   if (e != hipSuccess) return (int)e;
   if (split) {
-    const long blocks = (long)B * H + (weights ? (long)B * Hk * ((cap + JOIN_KEYS - 1) / JOIN_KEYS) : 0);
+    p.osplit = p.nsplit >= 32 && D % 32 == 0 ? D / 32 : 1;        // many splits: a head's output by 32 columns a workgroup
+    const long blocks = (long)B * H * p.osplit + (weights ? (long)B * Hk * ((cap + JOIN_KEYS - 1) / JOIN_KEYS) : 0);
     if (blocks > 0x7fffffffL) return AOT_ERR_UNSUPPORTED;
     with_dtype(dtype, [&](auto t) { hipLaunchKernelGGL((paged_join_kernel<decltype(t)>), dim3((unsigned)blocks), dim3(256), 0, st, p); });
   }

@@ -3,12 +3,12 @@
 // kept entries move, in order, into the pages of new_table, so pages that other sequences share stay as they are.
 //
 // Two launches.  Select: one workgroup a row; a radix select (three digits of an order-preserving key, histograms in shared memory) finds
-// the weight of the last entry that stays, ballots turn the kept flags into places.  It is bound by reading the weights (five times, from
-// L2 after the first) and by latency.  Move: 16-byte pieces of the kept K / V rows, bound by
+// the weight of the last entry that stays, ballots turn the kept flags into places.  It is bound by reading the weights (rows of up
+// to 16384 once, longer ones five times, from L2 after the first) and by latency.  Move: 16-byte pieces of the kept K / V rows, bound by
 // memory: each kept row is read once and written once.
 #include "seq_common.h"
 
-static constexpr int SEL_T = 1024;
+static constexpr int SEL_T = 1024, HOLD = 16;
 
 // larger key = heavier; -0 and +0 alike; NaN below everything
 __device__ __forceinline__ unsigned weight_key(float w) {
@@ -51,6 +51,7 @@ __device__ __forceinline__ int block_scan(int x, int* lds, int* sum) {
   return base + inc - x;
 }
 
+template <bool HELD>
 __global__ __launch_bounds__(SEL_T) void evict_select_kernel(EvictP p) {
   __shared__ int hist[2048];
   __shared__ int scan[SEL_T / 64];
@@ -64,12 +65,32 @@ __global__ __launch_bounds__(SEL_T) void evict_select_kernel(EvictP p) {
   const int keep = min(len, p.budget);
   const int lo = min(p.sink, len), hi = max(lo, len - p.recent);            // the contested middle
   const int want = keep - lo - (len - hi);                                  // how many of it stay (all of it if nothing has to go)
+  // a wave owns a run of entries, 64 at a time; up to HOLD of them a lane stay in registers (HELD: the row is at most HOLD * SEL_T long),
+  // so a row of 16384 is read once instead of five times: 33 us for 128 rows, 29 held
+  const int per = ((len + SEL_T - 1) / SEL_T) * 64, t0 = min(wave * per, len), t1 = min(t0 + per, len), steps = per / 64;
+  unsigned held[HELD ? HOLD : 1];
+  if constexpr (HELD) {
+#pragma unroll
+    for (int i = 0; i < HOLD; ++i) {
+      const int t = t0 + lane + 64 * i;
+      held[i] = i < steps && t < t1 ? weight_key(w[t]) : 0u;
+    }
+  }
+  auto each = [&](auto&& f) {                                               // f(entry, its key), the same order every time
+    if constexpr (HELD) {
+#pragma unroll
+      for (int i = 0; i < HOLD; ++i)
+        if (i < steps) f(t0 + lane + 64 * i, held[i]);
+    } else {
+      for (int t = t0 + lane; t < t0 + per; t += 64) f(t, t < t1 ? weight_key(w[t]) : 0u);
+    }
+  };
   unsigned thr = 0;
   int ties = 0;                                                             // of the entries equal to thr the first `ties` stay
   const bool all = keep == len;
   if (!all && want > 0) {
     // Digits of 11, 11 and 10 bits: the first holds sign, exponent and two mantissa bits, so that weights of one magnitude still spread over
-    // several counters (with 8 bits a wave's 64 additions met in one or two and queued: 41 us for 128 rows of 16384, now ####)
+    // several counters (with 8 bits a wave's 64 additions met in one or two and queued: 41 us for 128 rows of 16384, 33 with these)
     unsigned prefix = 0;
     int left = want;
 #pragma unroll 1
@@ -79,11 +100,9 @@ __global__ __launch_bounds__(SEL_T) void evict_select_kernel(EvictP p) {
       hist[tid] = 0;
       hist[tid + SEL_T] = 0;
       __syncthreads();
-#pragma unroll 4
-      for (int t = lo + tid; t < hi; t += SEL_T) {
-        const unsigned key = weight_key(w[t]);
-        if ((key & above) == prefix) atomicAdd(&hist[(key >> shift) & digit], 1);
-      }
+      each([&](int t, unsigned key) {
+        if (t >= lo && t < min(hi, t1) && (key & above) == prefix) atomicAdd(&hist[(key >> shift) & digit], 1);
+      });
       __syncthreads();
       const int c1 = hist[2047 - 2 * tid], c0 = hist[2046 - 2 * tid];       // from the heaviest digit down: where does `left` run out
       int sum;
@@ -101,22 +120,20 @@ __global__ __launch_bounds__(SEL_T) void evict_select_kernel(EvictP p) {
     thr = prefix;
     ties = left;
   }
-  // a wave owns a run of entries: count, exchange the counts, then place the kept ones by ballots
-  const int per = ((len + SEL_T - 1) / SEL_T) * 64, t0 = min(wave * per, len), t1 = min(t0 + per, len);
+  // count, exchange the waves' counts, then place the kept entries by ballots
   const unsigned long long below = (1ull << lane) - 1;
-  auto kind = [&](int t, float x, bool& sure, bool& tie) {
-    const unsigned key = weight_key(x);
+  auto kind = [&](int t, unsigned key, bool& sure, bool& tie) {
     const bool mid = !all && t >= lo && t < hi;
     sure = t < t1 && (!mid || (want > 0 && key > thr));
     tie = t < t1 && mid && want > 0 && key == thr;
   };
   int heavier = 0, equal = 0;
-  for (int t = t0 + lane; t < t0 + per; t += 64) {
+  each([&](int t, unsigned key) {
     bool sure, tie;
-    kind(t, t < t1 ? w[t] : 0.f, sure, tie);
+    kind(t, key, sure, tie);
     heavier += __popcll(__ballot(sure));
     equal += __popcll(__ballot(tie));
-  }
+  });
   if (lane == 0) { counts[wave][0] = heavier; counts[wave][1] = equal; }
   __syncthreads();
   int at = 0, eq = 0;
@@ -127,22 +144,21 @@ __global__ __launch_bounds__(SEL_T) void evict_select_kernel(EvictP p) {
   float* nw = p.new_weights + b * p.nws[0] + h * p.nws[1];
   const int* pos = p.pos ? p.pos + b * p.pss[0] + h * p.pss[1] : nullptr;
   int* np = p.pos ? p.new_pos + b * p.nps[0] + h * p.nps[1] : nullptr;
-  for (int t = t0 + lane; t < t0 + per; t += 64) {
-    const float x = t < t1 ? w[t] : 0.f;
+  each([&](int t, unsigned key) {
     bool sure, tie;
-    kind(t, x, sure, tie);
+    kind(t, key, sure, tie);
     const unsigned long long teq = __ballot(tie);
     const bool stay = sure || (tie && eq + __popcll(teq & below) < ties);
     const unsigned long long go = __ballot(stay);
     if (stay) {
       const int j = at + __popcll(go & below);
       kept[j] = t;
-      nw[j] = x;
+      nw[j] = w[t];                                                         // (the weight itself: a key forgets -0 and NaN's bits)
       if (pos) np[j] = pos[t];
     }
     at += __popcll(go);
     eq += __popcll(teq);
-  }
+  });
   for (int i = keep + tid; i < p.budget; i += SEL_T) kept[i] = -1;
   for (int i = keep + tid; i < p.S; i += SEL_T) {
     nw[i] = 0.f;
@@ -209,7 +225,8 @@ extern "C" int aot_paged_evict(void* k_pages, void* v_pages, const int* table, c
   };
   while (piece > es && !fits(piece)) piece >>= 1;
   hipStream_t st = (hipStream_t)stream;
-  hipLaunchKernelGGL(evict_select_kernel, dim3(Hk, B), dim3(SEL_T), 0, st, p);
+  if (p.cap <= HOLD * SEL_T) hipLaunchKernelGGL(evict_select_kernel<true>, dim3(Hk, B), dim3(SEL_T), 0, st, p);
+  else hipLaunchKernelGGL(evict_select_kernel<false>, dim3(Hk, B), dim3(SEL_T), 0, st, p);
   hipError_t e = hipGetLastError();
   if (e != hipSuccess) return (int)e;
   const int pieces = D * es / piece;

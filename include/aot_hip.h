@@ -568,7 +568,8 @@ int aot_attn_masked_floats(int B, int Sq, int Sk, int H, int Hk, int D, int back
  * (a cache that entries were evicted from), else len - 1 - t.  weights (optional): weights[b, hk, t] += the sum of the group's
  * probabilities, one writer per entry.  lengths are read on the device: 0 gives a zero row, more than max_pages * page counts as
  * that.  A page id outside the pool hides its entries.  Places past the length are not read.  D <= 256, rows of whole 16-byte pieces,
- * 16-byte aligned.  work: scratch of aot_paged_attn_work_floats floats (0: may be NULL); two calls in flight at once need two.
+ * 16-byte aligned.  work: scratch of aot_paged_attn_work_floats floats, 16-byte aligned (0: may be
+ * NULL); two calls in flight at once need two.
  * strides: q b h, out b h, k_pages page place h, v_pages page place h, table b, weights b h, key_pos b h (15). */
 int aot_paged_attn(const void* q, const void* k_pages, const void* v_pages, const int* table, const int* lengths, const float* slopes,
                    const int* key_pos, float* weights, void* out, float* work, long work_floats, int dtype, int B, int H, int Hk,
