@@ -1054,6 +1054,12 @@ def _device_of(first, *tensors):
     return dev
 
 
+def _elsewhere(dev, stream):
+    """Scope for a call whose tensors are on another device than the current one, or that names a stream (raw handle): copies and scratch
+    tensors are then made on that device and stream too."""
+    return torch.cuda.device(dev) if stream is None else torch.cuda.stream(torch.cuda.ExternalStream(stream, device=dev))
+
+
 _current_device = torch._C._cuda_getDevice if hasattr(torch._C, '_cuda_getDevice') else None
 _raw_stream = getattr(torch._C, '_cuda_getCurrentRawStream', None)
 _LONGS = [None] + [_L * n for n in range(1, 32)]
@@ -1118,9 +1124,9 @@ def rope(q, k, pos, freqs, interleaved=False, mscale=1.0, inverse=False, stream=
     if D > 1024 or (interleaved and D % 2):
         raise AotHipError('rope: head width %d not supported' % D)
     dev = _device_of(q, k, pos, freqs)
-    if _current_device() != dev:
-        with torch.cuda.device(dev):
-            return rope(q, k, pos, freqs, interleaved, mscale, inverse, stream)
+    if stream is not None or _current_device() != dev:
+        with _elsewhere(dev, stream):
+            return rope(q, k, pos, freqs, interleaved, mscale, inverse)
     q = _rows(q) if interleaved else _dense_last(q)
     qo = torch.empty((B, S, H, D), dtype=q.dtype, device=q.device)
     ko, Hk, more = None, 0, _NO3
@@ -1132,7 +1138,7 @@ def rope(q, k, pos, freqs, interleaved=False, mscale=1.0, inverse=False, stream=
     if H + Hk and B * S:
         st = _strides(q, 3) + more + (S * H * D, H * D, D) + (S * Hk * D, Hk * D, D) + _strides(pos, 2)
         _chk(load().aot_rope(q.data_ptr(), _ptr(k), qo.data_ptr(), _ptr(ko), pos.data_ptr(), freqs.data_ptr(), dtype, B, S, H, Hk, D, rot,
-                             1 if interleaved else 0, 1 if inverse else 0, mscale, _longs(st), _raw_stream(dev) if stream is None else stream),
+                             1 if interleaved else 0, 1 if inverse else 0, mscale, _longs(st), _raw_stream(dev)),
              'aot_rope')
     return qo, ko
 
@@ -1178,9 +1184,9 @@ def rope_append(q, k, v, pos, freqs, slots, k_pages, v_pages, interleaved=False,
     if interleaved and not (_whole_pieces(k_pages, 2 * k.element_size()) and _whole_pieces(v_pages, 2 * k.element_size())):
         raise AotHipError('rope_append: interleaved pairs need pages aligned to pairs')
     dev = _device_of(k, v, q, pos, freqs, slots, k_pages, v_pages)
-    if _current_device() != dev:
-        with torch.cuda.device(dev):
-            return rope_append(q, k, v, pos, freqs, slots, k_pages, v_pages, interleaved, mscale, stream)
+    if stream is not None or _current_device() != dev:
+        with _elsewhere(dev, stream):
+            return rope_append(q, k, v, pos, freqs, slots, k_pages, v_pages, interleaved, mscale)
     k, v, pos, slots = _dense_last(k), _dense_last(v), pos.contiguous(), slots.contiguous()
     if interleaved:
         k, v = _rows(k), _rows(v)
@@ -1196,7 +1202,7 @@ def rope_append(q, k, v, pos, freqs, slots, k_pages, v_pages, interleaved=False,
     if N and Hk:
         _chk(load().aot_rope_append(_ptr(q), k.data_ptr(), v.data_ptr(), _ptr(qo), k_pages.data_ptr(), v_pages.data_ptr(), pos.data_ptr(),
                                     slots.data_ptr(), freqs.data_ptr(), dtype, N, H, Hk, D, rot, 1 if interleaved else 0, mscale, page, P,
-                                    _longs(st + _strides(k_pages, 3) + _strides(v_pages, 3)), _raw_stream(dev) if stream is None else stream),
+                                    _longs(st + _strides(k_pages, 3) + _strides(v_pages, 3)), _raw_stream(dev)),
              'aot_rope_append')
     return qo
 
@@ -1209,7 +1215,8 @@ def _masked_args(name, q, k, v, scale, softcap, slopes, doc_q, doc_k, prefix):
     _need(k.shape[0] == B and k.shape[3] == D and Hk >= 1 and H >= Hk and H % Hk == 0, '%s: q %s and k %s do not fit', name, tuple(q.shape), tuple(k.shape))
     _need(1 <= D <= 128 and D * q.element_size() % 16 == 0, '%s: head width %d of %s not supported (whole 16-byte pieces, at most 128)', name, D, q.dtype)
     _need(max(Sq, Sk) <= 1 << 22 and B <= 65535, '%s: sizes beyond 2^22 tokens or 65535 sequences', name)
-    _need(softcap >= 0, '%s: softcap must not be negative', name)
+    _need(0 <= softcap < float('inf'), '%s: softcap must not be negative, nor infinite', name)
+    _need(scale is None or 0 < scale < float('inf'), '%s: scale must be positive', name)
     _need(slopes is None or (slopes.dtype == torch.float32 and tuple(slopes.shape) == (H,) and slopes.is_contiguous()), '%s: slopes must be dense float32 [H]', name)
     _need((doc_q is None) == (doc_k is None), '%s: doc_q and doc_k go together', name)
     if doc_q is not None:
@@ -1232,9 +1239,9 @@ def attn_masked(q, k, v, scale=None, causal=False, softcap=0.0, slopes=None, doc
     residual): residual=True asks for what rounding a 16-bit out left, which sharpens attn_masked_bwd; else (and for float32) it is None."""
     B, Sq, Sk, H, Hk, D, scale = _masked_args('attn_masked', q, k, v, scale, softcap, slopes, doc_q, doc_k, prefix)
     dev = _device_of(q, k, v, slopes, doc_q, doc_k, prefix)
-    if _current_device() != dev:
-        with torch.cuda.device(dev):
-            return attn_masked(q, k, v, scale, causal, softcap, slopes, doc_q, doc_k, prefix, residual, stream)
+    if stream is not None or _current_device() != dev:
+        with _elsewhere(dev, stream):
+            return attn_masked(q, k, v, scale, causal, softcap, slopes, doc_q, doc_k, prefix, residual)
     q, k, v = _rows(q), _rows(k), _rows(v)
     out = torch.empty((B, Sq, H, D), dtype=q.dtype, device=q.device)
     lse = torch.empty((B, H, Sq), dtype=torch.float32, device=q.device)
@@ -1250,7 +1257,7 @@ def attn_masked(q, k, v, scale=None, causal=False, softcap=0.0, slopes=None, doc
         _chk(load().aot_attn_masked(q.data_ptr(), _ptr(k), _ptr(v), out.data_ptr(), _ptr(res), lse.data_ptr(), _ptr(slopes), _ptr(doc_q),
                                     _ptr(doc_k) or _ptr(doc_q), _ptr(prefix), _ptr(ranges), _ptr(work), n, _DTYPE[q.dtype], B, Sq, Sk, H, Hk, D, 1 if causal else 0, scale, softcap,
                                     _longs(_strides(q, 3) + _strides(k, 3) + _strides(v, 3) + (Sq * H * D, H * D, D) + docs),
-                                    _raw_stream(dev) if stream is None else stream), 'aot_attn_masked')
+                                    _raw_stream(dev)), 'aot_attn_masked')
     return out, lse, res
 
 
@@ -1261,9 +1268,9 @@ def attn_masked_bwd(dout, q, k, v, out, lse, residual=None, scale=None, causal=F
     _need(lse.dtype == torch.float32 and tuple(lse.shape) == (B, H, Sq) and lse.is_contiguous(), 'attn_masked_bwd: lse must be dense float32 [B, H, Sq]')
     _need(residual is None or (residual.shape == q.shape and residual.dtype == q.dtype and residual.is_contiguous()), 'attn_masked_bwd: residual must be dense, like q')
     dev = _device_of(q, k, v, out, dout, lse, residual, slopes, doc_q, doc_k, prefix)
-    if _current_device() != dev:
-        with torch.cuda.device(dev):
-            return attn_masked_bwd(dout, q, k, v, out, lse, residual, scale, causal, softcap, slopes, doc_q, doc_k, prefix, stream)
+    if stream is not None or _current_device() != dev:
+        with _elsewhere(dev, stream):
+            return attn_masked_bwd(dout, q, k, v, out, lse, residual, scale, causal, softcap, slopes, doc_q, doc_k, prefix)
     q, k, v, out, dout = _rows(q), _rows(k), _rows(v), _rows(out), _rows(dout)
     where = dict(dtype=q.dtype, device=q.device)
     dq, dk, dv = torch.empty((B, Sq, H, D), **where), torch.empty((B, Sk, Hk, D), **where), torch.empty((B, Sk, Hk, D), **where)
@@ -1280,7 +1287,7 @@ def attn_masked_bwd(dout, q, k, v, out, lse, residual=None, scale=None, causal=F
                                         _ptr(doc_q) or _ptr(doc_k), _ptr(doc_k) or _ptr(doc_q), _ptr(prefix), _ptr(ranges), _ptr(work), n,
                                         _DTYPE[q.dtype], B, Sq, Sk, H, Hk, D, 1 if causal else 0, scale, softcap,
                                         _longs(_strides(q, 3) + _strides(k, 3) + _strides(v, 3) + _strides(out, 3) + _strides(dout, 3) + qs + ks + ks + docs),
-                                        _raw_stream(dev) if stream is None else stream), 'aot_attn_masked_bwd')
+                                        _raw_stream(dev)), 'aot_attn_masked_bwd')
     return dq, dk, dv
 
 
@@ -1302,11 +1309,11 @@ def paged_attn(q, k_pages, v_pages, table, lengths, scale=None, softcap=0.0, slo
         raise AotHipError('paged_attn: table must be int32 [B, max_pages]')
     mp = table.shape[1]
     cap = mp * page
-    if cap > _I32_MAX or B > 65535:
-        raise AotHipError('paged_attn: sizes beyond 2^31 entries or 65535 sequences')
+    if cap > 1 << 30 or B > 65535:
+        raise AotHipError('paged_attn: sizes beyond 2^30 entries or 65535 sequences')
     _check_int32('paged_attn: lengths', lengths, (B,))
-    if not softcap >= 0:
-        raise AotHipError('paged_attn: softcap must not be negative')
+    if not 0 <= softcap < float('inf'):
+        raise AotHipError('paged_attn: softcap must not be negative, nor infinite')
     if slopes is not None and (slopes.dtype != torch.float32 or tuple(slopes.shape) != (H,) or not slopes.is_contiguous()):
         raise AotHipError('paged_attn: slopes must be dense float32 [H]')
     for name, t, dt in (('weights', weights, torch.float32), ('key_pos', key_pos, torch.int32)):
@@ -1316,9 +1323,9 @@ def paged_attn(q, k_pages, v_pages, table, lengths, scale=None, softcap=0.0, slo
     if out is not None and (out.shape != q.shape or out.dtype != q.dtype or (out.stride(2) != 1 and D != 1)):
         raise AotHipError('paged_attn: out must be like q')
     dev = _device_of(q, k_pages, v_pages, table, lengths, slopes, weights, key_pos, out)
-    if _current_device() != dev:
-        with torch.cuda.device(dev):
-            return paged_attn(q, k_pages, v_pages, table, lengths, scale, softcap, slopes, weights, key_pos, out, stream)
+    if stream is not None or _current_device() != dev:
+        with _elsewhere(dev, stream):
+            return paged_attn(q, k_pages, v_pages, table, lengths, scale, softcap, slopes, weights, key_pos, out)
     lib = load()
     q, table, lengths = _rows(q), _dense_last(table), lengths.contiguous()
     if out is None:
@@ -1330,7 +1337,7 @@ def paged_attn(q, k_pages, v_pages, table, lengths, scale=None, softcap=0.0, slo
         (_NO2 if weights is None else _strides(weights, 2)) + (_NO2 if key_pos is None else _strides(key_pos, 2))
     _chk(lib.aot_paged_attn(_ptr(q), _ptr(k_pages), _ptr(v_pages), _ptr(table), _ptr(lengths), _ptr(slopes), _ptr(key_pos), _ptr(weights), _ptr(out),
                             _ptr(work), n.value, dtype, B, H, Hk, D, page, mp, P, D ** -0.5 if scale is None else scale, softcap, _longs(st),
-                            _raw_stream(dev) if stream is None else stream), 'aot_paged_attn')
+                            _raw_stream(dev)), 'aot_paged_attn')
     return out
 
 
@@ -1359,9 +1366,9 @@ def paged_evict(k_pages, v_pages, table, lengths, weights, new_table, budget, si
     if mp * page > _I32_MAX or npg * page > _I32_MAX or B > 65535 or Hk > 65535:
         raise AotHipError('paged_evict: sizes beyond 2^31 entries or 65535 rows')
     dev = _device_of(k_pages, v_pages, table, lengths, weights, new_table, key_pos)
-    if _current_device() != dev:
-        with torch.cuda.device(dev):
-            return paged_evict(k_pages, v_pages, table, lengths, weights, new_table, budget, sink, recent, key_pos, stream)
+    if stream is not None or _current_device() != dev:
+        with _elsewhere(dev, stream):
+            return paged_evict(k_pages, v_pages, table, lengths, weights, new_table, budget, sink, recent, key_pos)
     if mp and table.data_ptr() == new_table.data_ptr():
         raise AotHipError('paged_evict: new_table must not be table')
     S = weights.shape[2]
@@ -1377,5 +1384,5 @@ def paged_evict(k_pages, v_pages, table, lengths, weights, new_table, budget, si
         st += _NO2 + _NO2 if key_pos is None else _strides(key_pos, 2) + (Hk * S, S)
         _chk(load().aot_paged_evict(_ptr(k_pages), _ptr(v_pages), _ptr(table), _ptr(new_table), _ptr(lengths), _ptr(weights), _ptr(key_pos), _ptr(kept),
                                     _ptr(new_lengths), _ptr(new_weights), _ptr(new_pos), dtype, B, Hk, D, S, page, mp, npg, P, budget,
-                                    sink, recent, _longs(st), _raw_stream(dev) if stream is None else stream), 'aot_paged_evict')
+                                    sink, recent, _longs(st), _raw_stream(dev)), 'aot_paged_evict')
     return kept, new_lengths, new_weights, new_pos

@@ -322,7 +322,7 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? (DP == 64 ? 3 : 2) : 1) void 
   u32x4 qf[NP];
   own_row<T, NP>(qf, (const T*)p.q + hd.b * p.qs[0] + (long)i * p.qs[1] + hd.h * p.qs[2], iok, p.D);
   const Score sc(p, hd.h);
-  const int prefix = p.prefix ? p.prefix[hd.b] : 0;
+  const int prefix = p.prefix ? max(0, p.prefix[hd.b]) : 0;
   const int myid = p.doc_q ? (iok ? p.doc_q[hd.b * p.dcs[0] + i] : -1) : 0;
   const int qlast = min(q0 + 127, p.Sq - 1);
   const int4 *rk = nullptr;
@@ -578,7 +578,7 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void attn_masked_dq_ke
   if (lse == NEG_INF) { lse = __builtin_inff(); delta = 0.f; }   // sees nothing: every probability is zero
   if (iok && half == 0 && blockIdx.z == 0) p.delta[at] = delta;
   const Score sc(p, hd.h);
-  const int prefix = p.prefix ? p.prefix[hd.b] : 0;
+  const int prefix = p.prefix ? max(0, p.prefix[hd.b]) : 0;
   const int myid = p.doc_q ? (iok ? p.doc_q[hd.b * p.dcs[0] + i] : -1) : 0;
   const int qlast = min(q0 + 127, p.Sq - 1);
   const int4 *rk = nullptr;
@@ -759,7 +759,7 @@ __global__ __launch_bounds__(NT, NT / 256) void attn_masked_dkv_kernel(MaskP p) 
     own_row<T, NP>(wf, (const T*)(keys ? p.v : p.k) + b * st[0] + (long)t * st[1] + hk * st[2], tok, p.D);
   }
   auto exchange = [&](int buf, int n) { return (f32x4*)(smem + 5 * TL::BYTES + buf * XB + ((wave & (NW - 1)) * NS + n) * 4096) + lane; };
-  const int prefix = p.prefix ? p.prefix[b] : 0;
+  const int prefix = p.prefix ? max(0, p.prefix[b]) : 0;
   const int myid = p.doc_k ? (tok ? p.doc_k[b * p.dcs[1] + t] : -1) : 0;
   const int klast = min(k0 + KEYS - 1, p.Sk - 1);
   const int4 *rq = nullptr;
@@ -1021,10 +1021,10 @@ static void sum_join(const float* part, char* out, const long* st, long next, in
 }
 
 // ---- C entries -----------------------------------------------------------------------------------------------------------------------
-static int mask_args(int dtype, int B, int Sq, int Sk, int H, int Hk, int D, float softcap, const int* doc_q, const int* doc_k, const void* ranges,
+static int mask_args(int dtype, int B, int Sq, int Sk, int H, int Hk, int D, float scale, float softcap, const int* doc_q, const int* doc_k, const void* ranges,
                      const long* strides) {
   const int es = dtype_size(dtype);
-  if (!es || B < 0 || Sq < 0 || Sk < 0 || Hk < 1 || H < Hk || H % Hk || D < 1 || !strides || !(softcap >= 0.f)) return AOT_ERR_BADARG;
+  if (!es || B < 0 || Sq < 0 || Sk < 0 || Hk < 1 || H < Hk || H % Hk || D < 1 || !strides || !(softcap >= 0.f && softcap < __builtin_inff()) || !(scale > 0.f && scale < __builtin_inff())) return AOT_ERR_BADARG;   // (a running maximum of unscaled scores needs a positive scale)
   if ((doc_q == nullptr) != (doc_k == nullptr) || (doc_q && !ranges)) return AOT_ERR_BADARG;
   if (D > 128 || D * es % 16 || Sq > (1 << 22) || Sk > (1 << 22) || (long)B * H > 0x7fffffffL || B > 65535) return AOT_ERR_UNSUPPORTED;
   return AOT_OK;
@@ -1087,7 +1087,7 @@ extern "C" int aot_attn_masked_floats(int B, int Sq, int Sk, int H, int Hk, int 
 extern "C" int aot_attn_masked(const void* q, const void* k, const void* v, void* out, void* residual, float* lse, const float* slopes,
                                const int* doc_q, const int* doc_k, const int* prefix, void* ranges, float* work, long work_floats, int dtype, int B, int Sq, int Sk, int H, int Hk, int D,
                                int causal, float scale, float softcap, const long* strides, void* stream) {
-  int rc = mask_args(dtype, B, Sq, Sk, H, Hk, D, softcap, doc_q, doc_k, ranges, strides);
+  int rc = mask_args(dtype, B, Sq, Sk, H, Hk, D, scale, softcap, doc_q, doc_k, ranges, strides);
   if (rc) return rc;
   if (B == 0 || Sq == 0) return AOT_OK;
   if (!q || !out || !lse || (Sk && (!k || !v))) return AOT_ERR_BADARG;
@@ -1117,7 +1117,7 @@ extern "C" int aot_attn_masked_bwd(const void* q, const void* k, const void* v, 
                                    const void* dout, void* dq, void* dk, void* dv, const float* slopes, const int* doc_q, const int* doc_k, const int* prefix, void* ranges, float* work, long work_floats,
                                    int dtype, int B, int Sq, int Sk, int H, int Hk, int D, int causal, float scale, float softcap, const long* strides,
                                    void* stream) {
-  int rc = mask_args(dtype, B, Sq, Sk, H, Hk, D, softcap, doc_q, doc_k, ranges, strides);
+  int rc = mask_args(dtype, B, Sq, Sk, H, Hk, D, scale, softcap, doc_q, doc_k, ranges, strides);
   if (rc) return rc;
   if (B == 0 || (Sq == 0 && Sk == 0)) return AOT_OK;
   if ((Sq && (!q || !out || !lse || !dout || !dq)) || (Sk && (!k || !v || !dk || !dv))) return AOT_ERR_BADARG;

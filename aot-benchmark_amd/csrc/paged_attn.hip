@@ -363,8 +363,8 @@ __global__ __launch_bounds__(256) void paged_join_kernel(PagedP p) {
   }
 }
 
-static int pow2_at_least(long x) {
-  int r = 1;
+static long pow2_at_least(long x) {
+  long r = 1;
   while (r < x) r <<= 1;
   return r;
 }
@@ -376,7 +376,7 @@ static int paged_chunk(long rows, long cap) {
   const long want = std::max(1L, target / std::max(1L, rows));
   long chunk = (cap + want - 1) / want;
   chunk = std::max(chunk, (cap + 1023) / 1024);
-  return std::max(128, pow2_at_least(chunk));
+  return (int)std::max(128L, pow2_at_least(chunk));             // (a capacity is at most 2^30)
 }
 
 // workspace: sums [B * H][nsplit][D], their (m, l), scores [B * H][capacity in whole groups of four]
@@ -392,6 +392,7 @@ static long paged_work(int B, int H, int Hk, int D, long cap, int with_weights, 
 
 extern "C" int aot_paged_attn_work_floats(int B, int H, int Hk, int D, int page, int max_pages, int with_weights, long* floats) {
   if (!floats || B < 0 || Hk < 1 || H < Hk || H % Hk || D < 1 || page < 1 || max_pages < 0) return AOT_ERR_BADARG;
+  if ((long)page * max_pages > (1L << 30)) return AOT_ERR_UNSUPPORTED;
   int c, n;
   *floats = paged_work(B, H, Hk, D, (long)page * max_pages, with_weights, &c, &n);
   return AOT_OK;
@@ -402,10 +403,10 @@ extern "C" int aot_paged_attn(const void* q, const void* k_pages, const void* v_
                               int D, int page, int max_pages, long num_pages, float scale, float softcap, const long* strides, void* stream) {
   const int es = dtype_size(dtype);
   if (!es || B < 0 || Hk < 1 || H < Hk || H % Hk || D < 1 || page < 1 || (page & (page - 1)) || max_pages < 0 || num_pages < 0 || !strides ||
-      !(softcap >= 0.f)) return AOT_ERR_BADARG;
+      !(softcap >= 0.f && softcap < __builtin_inff())) return AOT_ERR_BADARG;
   const long cap = (long)page * max_pages;
   const int G = H / Hk, qt = (G + 15) / 16;
-  if (D > 256 || D * es % 16 || cap > 0x7fffffffL || num_pages * page > 0x7fffffffL || B > 65535 || (long)Hk * qt > 65535) return AOT_ERR_UNSUPPORTED;
+  if (D > 256 || D * es % 16 || cap > (1L << 30) || num_pages * page > 0x7fffffffL || B > 65535 || (long)Hk * qt > 65535) return AOT_ERR_UNSUPPORTED;
   if (B == 0) return AOT_OK;
   if (!q || !lengths || !out || (cap && !table) || (num_pages && (!k_pages || !v_pages))) return AOT_ERR_BADARG;
   PagedP p{};

@@ -102,7 +102,7 @@ class _MaskedAttention(Function):
 def masked_attention(q, k, v, scale=None, causal=False, softcap=0.0, slopes=None, doc_q=None, doc_k=None, prefix=None):
     """Attention of q [B, Sq, H, D] over k / v [B, Sk, Hk, D] (H a multiple of Hk), differentiable in the three; out like q.
 
-    Query i stands at place i + Sk - Sq among the keys.  scale: 1 / sqrt(D) by default.  causal: keys up to the query's place.
+    Query i stands at place i + Sk - Sq among the keys.  scale (positive): 1 / sqrt(D) by default.  causal: keys up to the query's place.
     softcap: scores become softcap * tanh(score / softcap).  slopes float32 [H]: slopes[h] * |distance| is taken off the score (no gradient).
     doc_q int32 [B, Sq], doc_k int32 [B, Sk]: a query sees the keys of its own document; a negative id is padding and sees nothing.
     prefix int32 [B]: under `causal`, keys before prefix[b] are seen by every query.  A query that sees nothing gives zeros and takes no

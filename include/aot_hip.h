@@ -538,7 +538,7 @@ int aot_rope_append(const void* q, const void* k, const void* v, void* qo, void*
 
 /* Attention under masks, q [B, Sq, H, D], k / v [B, Sk, Hk, D] -> out [B, Sq, H, D] and lse [B, H, Sq] (log2 of the sum of exponentials;
  * -inf for a row that sees nothing, whose output is zero).  Query i stands at place i + Sk - Sq of the key sequence.
- *   s = softcap tanh(scale q.k / softcap) - slopes[h] |i + Sk - Sq - t|      (softcap = 0: no cap; slopes [H] or NULL)
+ *   s = softcap tanh(scale q.k / softcap) - slopes[h] |i + Sk - Sq - t|      (scale > 0; softcap = 0: no cap; slopes [H] or NULL)
  * Key t is seen if (not causal, or t <= i + Sk - Sq, or t < prefix[b]) and (no documents, or doc_q[b, i] == doc_k[b, t] >= 0).  A negative
  * document id marks padding.  What masked places hold (NaN, infinities) does not reach the result.  prefix [B] or NULL (read with causal
  * only); doc_q [B, Sq] / doc_k [B, Sk] both or neither, then `ranges` is scratch of 16 * B * (ceil(Sq / 64) + ceil(Sk / 64)) bytes, 16-byte
@@ -568,7 +568,7 @@ int aot_attn_masked_floats(int B, int Sq, int Sk, int H, int Hk, int D, int back
  * (a cache that entries were evicted from), else len - 1 - t.  weights (optional): weights[b, hk, t] += the sum of the group's
  * probabilities, one writer per entry.  lengths are read on the device: 0 gives a zero row, more than max_pages * page counts as
  * that.  A page id outside the pool hides its entries.  Places past the length are not read.  D <= 256, rows of whole 16-byte pieces,
- * 16-byte aligned.  work: scratch of aot_paged_attn_work_floats floats, 16-byte aligned (0: may be
+ * 16-byte aligned; max_pages * page <= 2^30.  work: scratch of aot_paged_attn_work_floats floats, 16-byte aligned (0: may be
  * NULL); two calls in flight at once need two.
  * strides: q b h, out b h, k_pages page place h, v_pages page place h, table b, weights b h, key_pos b h (15). */
 int aot_paged_attn(const void* q, const void* k_pages, const void* v_pages, const int* table, const int* lengths, const float* slopes,

@@ -163,6 +163,34 @@ def test_masked_attention_and_gradients(seq, dtype, shape):
         within(name, g, w, b)
 
 
+def test_prefix_outside_the_keys(seq):
+    q, k, v = (rand((3, 40, 2, 64), torch.float32, i) for i in range(3))
+    pre = torch.tensor([-2 ** 31, -1, 2 ** 31 - 1], dtype=torch.int32, device='cuda')
+    out = seq.masked_attention(q, k, v, causal=True, prefix=pre)
+    assert torch.equal(out[:2], seq.masked_attention(q[:2], k[:2], v[:2], causal=True))
+    want, bound = R.attention(q[2:], k[2:], v[2:])
+    within('all seen', out[2:], want, bound)
+
+
+def test_calls_on_a_named_stream(seq):
+    """stream=: the launch, its copies of odd inputs and its scratch belong to that stream."""
+    import aot_hip
+    x = rand((1, 700, 2, 3 * 64 + 1), torch.float16, 1)
+    q, k, v = x[..., :64], x[..., 64:128], x[..., 128:192]                  # rows off 16 bytes: dense copies are made
+    kp, vp, table, _ = cache(2, 4000, 16, 2, 64, torch.float16, 3)
+    n = torch.tensor([4000, 77], dtype=torch.int32, device='cuda')
+    want = aot_hip.attn_masked(q, k, v, causal=True)[0]
+    wp = aot_hip.paged_attn(q[0, :2], kp, vp, table, n)
+    torch.cuda.synchronize()
+    side = torch.cuda.Stream()
+    for _ in range(5):
+        a = aot_hip.attn_masked(q, k, v, causal=True, stream=side.cuda_stream)[0]
+        b = aot_hip.paged_attn(q[0, :2], kp, vp, table, n, stream=side.cuda_stream)
+        torch.empty(1 << 22, device='cuda').fill_(float('nan'))             # the current stream reuses what it may
+    side.synchronize()
+    assert torch.equal(a, want) and torch.equal(b, wp)
+
+
 def test_masked_attention_empty_sides(seq):
     q, k = rand((2, 5, 2, 64), torch.float16, 1).requires_grad_(), rand((2, 0, 1, 64), torch.float16, 2).requires_grad_()
     out = seq.masked_attention(q, k, k, causal=True)

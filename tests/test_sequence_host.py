@@ -34,9 +34,9 @@ def test_c_entries_refuse_before_any_launch():
         assert append(**bad) == -1, bad
     assert append(pages=1 << 28) == -2 and append(N=0) == 0
 
-    def masked(dtype=0, B=1, Sq=1, Sk=1, H=1, Hk=1, D=32, cap=0.0, q=P(16), k=P(16), dq=None, dk=None, rng=None, st=z14, lse=P(16), res=None):
-        return lib.aot_attn_masked(q, k, P(16), P(16), res, lse, None, dq, dk, None, rng, None, 0, dtype, B, Sq, Sk, H, Hk, D, 1, 1.0, cap, st, None)
-    for bad in (dict(dtype=7), dict(H=3, Hk=2), dict(Hk=0), dict(cap=-1.0), dict(cap=math.nan), dict(dq=P(16)), dict(dq=P(16), dk=P(16)), dict(q=P(24)), dict(q=None),
+    def masked(dtype=0, B=1, Sq=1, Sk=1, H=1, Hk=1, D=32, cap=0.0, q=P(16), k=P(16), dq=None, dk=None, rng=None, st=z14, lse=P(16), res=None, scale=1.0):
+        return lib.aot_attn_masked(q, k, P(16), P(16), res, lse, None, dq, dk, None, rng, None, 0, dtype, B, Sq, Sk, H, Hk, D, 1, scale, cap, st, None)
+    for bad in (dict(scale=0.0), dict(scale=-1.0), dict(scale=math.inf), dict(cap=math.inf), dict(dtype=7), dict(H=3, Hk=2), dict(Hk=0), dict(cap=-1.0), dict(cap=math.nan), dict(dq=P(16)), dict(dq=P(16), dk=P(16)), dict(q=P(24)), dict(q=None),
                 dict(k=None), dict(lse=None), dict(st=None), dict(res=P(24)), dict(Sk=4096), dict(st=L(0, 33, *[0] * 12)), dict(Sq=-1), dict(D=0)):
         assert masked(**bad) == -1, bad
     assert masked(D=132) == -2 and masked(D=33) == -2 and masked(dtype=1, D=36) == -2 and masked(Sk=(1 << 22) + 1) == -2
@@ -57,6 +57,8 @@ def test_c_entries_refuse_before_any_launch():
     n = ctypes.c_long(-1)
     assert lib.aot_paged_attn_work_floats(1, 8, 2, 64, 16, 4, 0, ctypes.addressof(n)) == 0 and n.value == 0
     assert lib.aot_paged_attn_work_floats(1, 8, 2, 64, 16, 4, 1, ctypes.addressof(n)) == 0 and n.value >= 8 * (64 + 66)
+    assert lib.aot_paged_attn_work_floats(4096, 64, 8, 64, 1 << 20, 1 << 12, 1, ctypes.addressof(n)) == -2
+    assert lib.aot_paged_attn_work_floats(4096, 64, 8, 64, 1 << 20, 1 << 10, 0, ctypes.addressof(n)) == 0 and n.value == 0      # one split of 2^30
     assert lib.aot_paged_attn_work_floats(1, 8, 3, 64, 16, 4, 1, ctypes.addressof(n)) == -1
     assert lib.aot_paged_attn_work_floats(1, 8, 2, 64, 16, 4, 1, None) == -1
 
@@ -103,6 +105,12 @@ def test_python_calls_refuse_what_the_kernels_do_not_take():
     refused('doc_k', S.masked_attention, q, k, k, doc_q=pos, doc_k=i32(1, 3))
     refused('prefix', S.masked_attention, q, k, k, prefix=i32(2))
     refused('softcap', S.masked_attention, q, k, k, softcap=-1.0)
+    refused('softcap', S.masked_attention, q, k, k, softcap=math.inf)
+    refused('scale', S.masked_attention, q, k, k, scale=0.0)
+    refused('scale', S.masked_attention, q, k, k, scale=-0.5)
+    refused('scale', S.masked_attention, q, k, k, scale=math.nan)
+    refused('softcap', S.paged_attention, f(2, 4, 32), kp, kp, table, n, softcap=math.nan)
+    refused('beyond', S.paged_attention, f(1, 4, 32), f(1, 1 << 10, 2, 32), f(1, 1 << 10, 2, 32), i32(1, (1 << 20) + 1), i32(1))
     refused('slopes', S.masked_attention, q, k, k, slopes=f(3))
     refused('no gradient', S.masked_attention, q, k, k, slopes=f(4, requires_grad=True))
     refused('of one of', S.masked_attention, q, k, k.half())
