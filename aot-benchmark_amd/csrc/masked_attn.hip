@@ -935,7 +935,7 @@ __global__ __launch_bounds__(NT, NT / 256) void attn_masked_dkv_kernel(MaskP p) 
               const i32x4 id = *(const i32x4*)(sid + buf * QT + j0);
 #pragma unroll
               for (int w = 0; w < 4; ++w)
-                if (j0 + w < lim - tq * QT || id[w] != myid) s[4 * r4 + w] = 0.f;
+                if (j0 + w < lim - tq * QT || id[w] != myid) { s[4 * r4 + w] = 0.f; dcap[4 * r4 + w] = 0.f; }   // (either may be NaN there)
             }
           }
           f32x4* x = exchange(buf, n);

@@ -205,12 +205,15 @@ def test_masked_attention_empty_sides(seq):
 
 @pytest.mark.parametrize('dtype', DT)
 @pytest.mark.parametrize('fill', [float('nan'), float('inf'), -float('inf')])
-def test_masked_places_may_hold_anything(seq, dtype, fill):
+@pytest.mark.parametrize('more', [{}, dict(softcap=6.0), dict(softcap=6.0, slopes=True)])
+def test_masked_places_may_hold_anything(seq, dtype, fill, more):
     """Results are those of the same call with zeros in the masked places, bit for bit."""
     dt = DT[dtype]
     S = 200
     ids = docs_of(1, S, 3, 5, 20)
     dead = ids[0] < 0
+    if 'slopes' in more:
+        more = dict(more, slopes=torch.tensor([0.02, 0.1], device='cuda'))
     late = torch.arange(S, device='cuda') >= 150                           # keys no query of a shorter query block sees
 
     def run(x):
@@ -218,14 +221,14 @@ def test_masked_places_may_hold_anything(seq, dtype, fill):
         for t in (q, k, v, do):
             t[:, dead] = x
         lead = [t.requires_grad_() for t in (q, k, v)]
-        a = seq.masked_attention(q, k, v, causal=True, doc_q=ids, doc_k=ids)
+        a = seq.masked_attention(q, k, v, causal=True, doc_q=ids, doc_k=ids, **more)
         ga = torch.autograd.grad(a, lead, do)
         k2, v2 = rand((1, S, 2, 64), dt, 31), rand((1, S, 2, 64), dt, 32)
         k2[:, late], v2[:, late] = x, x
         q2, do2 = rand((1, S, 2, 64), dt, 33), rand((1, S, 2, 64), dt, 34)
         q2[:, late], do2[:, late] = x, x                                   # causal: rows before 150 see no late key; the late rows' results go
         lead2 = [t.requires_grad_() for t in (q2, k2, v2)]
-        c = seq.masked_attention(q2, k2, v2, causal=True)
+        c = seq.masked_attention(q2, k2, v2, causal=True, **more)
         return [a] + list(ga), c[:, :150], torch.autograd.grad(c, lead2, do2)[0][:, :150]
 
     (a, c, dq), (a0, c0, dq0) = run(fill), run(0.0)
