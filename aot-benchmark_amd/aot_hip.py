@@ -1072,6 +1072,13 @@ def _strides(t, n):
     return st if 1 not in sh else tuple([0 if sh[i] == 1 else st[i] for i in range(n)])
 
 
+def _own_places(name, *tensors):
+    """Tensors that are written must not name a place twice (expanded views do)."""
+    for t in tensors:
+        if t is not None and 0 in t.stride() and any(s == 0 and d > 1 for s, d in zip(t.stride(), t.shape)):
+            raise AotHipError('%s: a tensor that is written must not be an expanded view' % name)
+
+
 def _longs(values):
     """Host array of strides."""
     return _LONGS[len(values)](*values)
@@ -1181,6 +1188,7 @@ def rope_append(q, k, v, pos, freqs, slots, k_pages, v_pages, interleaved=False,
     if D > 1024 or (interleaved and D % 2):
         raise AotHipError('rope_append: head width %d not supported' % D)
     P, page, _, _ = _check_pages('rope_append', k_pages, v_pages, k.dtype, D, Hk)
+    _own_places('rope_append', k_pages, v_pages)
     if interleaved and not (_whole_pieces(k_pages, 2 * k.element_size()) and _whole_pieces(v_pages, 2 * k.element_size())):
         raise AotHipError('rope_append: interleaved pairs need pages aligned to pairs')
     dev = _device_of(k, v, q, pos, freqs, slots, k_pages, v_pages)
@@ -1320,6 +1328,7 @@ def paged_attn(q, k_pages, v_pages, table, lengths, scale=None, softcap=0.0, slo
         if t is not None and (t.dtype != dt or t.dim() != 3 or t.shape[0] != B or t.shape[1] != Hk or t.shape[2] < cap or
                               (t.stride(2) != 1 and t.shape[2] > 1)):
             raise AotHipError('paged_attn: %s must be %s [B, Hk, at least %d], last dimension dense' % (name, dt, cap))
+    _own_places('paged_attn', weights, out)
     if out is not None and (out.shape != q.shape or out.dtype != q.dtype or (out.stride(2) != 1 and D != 1)):
         raise AotHipError('paged_attn: out must be like q')
     dev = _device_of(q, k_pages, v_pages, table, lengths, slopes, weights, key_pos, out)
@@ -1358,6 +1367,7 @@ def paged_evict(k_pages, v_pages, table, lengths, weights, new_table, budget, si
         raise AotHipError('paged_evict: weights must be float32 [B, Hk, at least %d]' % (mp * page))
     if key_pos is not None and (key_pos.dtype != torch.int32 or key_pos.shape != weights.shape):
         raise AotHipError('paged_evict: key_pos must be int32, shaped like weights')
+    _own_places('paged_evict', k_pages, v_pages)
     budget, sink, recent = int(budget), int(sink), int(recent)
     if budget < 1 or sink < 0 or recent < 0 or sink + recent > budget:
         raise AotHipError('paged_evict: sink %d + recent %d must fit the budget %d' % (sink, recent, budget))

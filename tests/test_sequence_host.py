@@ -122,6 +122,9 @@ def test_python_calls_refuse_what_the_kernels_do_not_take():
     refused('head width', S.paged_attention, f(2, 4, 264), f(6, 8, 2, 264), f(6, 8, 2, 264), table, n)
     refused('16-byte', S.paged_attention, f(2, 4, 32), f(6, 8, 2, 33)[..., :32], f(6, 8, 2, 33)[..., :32], table, n)
     refused('last dimension', S.paged_attention, f(2, 4, 32), f(6, 8, 32, 2).transpose(2, 3), f(6, 8, 32, 2).transpose(2, 3), table, n)
+    refused('expanded', S.paged_attention, f(2, 4, 32), kp, kp, table, n, weights=f(1, 2, 24).expand(2, 2, 24))
+    refused('expanded', S.rope_append, q[0], k[0], k[0], pos[0], freqs, pos[0], f(1, 8, 2, 32).expand(6, 8, 2, 32), kp)
+    refused('expanded', S.paged_evict, kp, f(1, 8, 2, 32).expand(6, 8, 2, 32), table, n, w, i32(2, 1), 8)
     refused('serving call', S.paged_attention, f(2, 4, 32, requires_grad=True), kp, kp, table, n)
     refused('serving call', S.rope_append, q[0], f(4, 2, 32, requires_grad=True), k[0], pos[0], freqs, pos[0], kp, kp)
     refused('fit the budget', S.paged_evict, kp, kp, table, n, w, i32(2, 1), 8, sink=5, recent=4)
