@@ -26,6 +26,7 @@
 // the value for bf16, 2^-12 for fp16, below which fp16 also loses what is under 6e-8), the sum that divides is not.
 #include "seq_common.h"
 
+static constexpr int AHEAD = 4;                               // fragments of a group that is read ahead of its products
 static constexpr int RG = 64;                                  // tokens a document range covers
 
 struct MaskP {
@@ -159,8 +160,12 @@ template <class T, int DP, int R, int NT> struct Tile {           // NT threads 
     }
   }
   // first operand of a product over the columns: lane = row 32 n + (lane & 31), piece 2 c + lane / 32.  o: the tile's offset + row_base()
-  static __device__ __forceinline__ u32x4 rows(const char* lds, int o, int n, int c) {
-    return *(const u32x4*)(lds + (o ^ (place(0, 2 * c) << 4)) + n * 32 * ROWB);
+  // (pinned: a volatile read, which stays where it is written -- see in_groups)
+  template <bool PINNED = false> static __device__ __forceinline__ u32x4 rows(const char* lds, int o, int n, int c) {
+    typedef __attribute__((address_space(3))) const volatile u32x4 lds_u32x4;
+    const char* x = lds + (o ^ (place(0, 2 * c) << 4)) + n * 32 * ROWB;
+    if constexpr (PINNED) return *(lds_u32x4*)x;
+    else return *(const u32x4*)x;
   }
   // 16-bit: first operand of a product over 16 rows (32 n + 16 kb ..) of the tile, in score-tile order: lane = column 32 db + (lane & 31).
   // o: the tile's offset + col_base()
@@ -278,6 +283,34 @@ template <class T> __device__ __forceinline__ void store_out(const MaskP& p, lon
       store4((T*)p.res_out + row * p.D + e, x[0] - (float)(T)x[0], x[1] - (float)(T)x[1], x[2] - (float)(T)x[2], x[3] - (float)(T)x[3]);
 }
 
+// N fragments read and used in groups of A, each group's reads issued before the products of the group ahead of it (pinned reads: left to
+// itself the compiler puts every read right before its use, and a wave waits out the latency of each).  Measured at 2 x 4096 x 16 x 128 plain
+// 437 -> 420 us forward, dk / dv under a cap with four heads a key head 446 -> 420; the dq kernel, whose registers are full, lost 4 % and does without.
+template <int N, int A, class L, class U> __device__ __forceinline__ void in_groups(L&& load, U&& use) {
+  u32x4 f[2][A];
+#pragma unroll
+  for (int i = 0; i < A; ++i) if (i < N) f[0][i] = load(i);
+#pragma unroll
+  for (int g = 0; g < N; g += A) {
+#pragma unroll
+    for (int i = 0; i < A; ++i) if (g + A + i < N) f[(g / A + 1) & 1][i] = load(g + A + i);
+    __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+    for (int i = 0; i < A; ++i) if (g + i < N) use(g + i, f[(g / A) & 1][i]);
+    __builtin_amdgcn_sched_barrier(0);
+  }
+}
+
+// acc[d] += the product over rows 32 n .. of the tile at o, all column blocks
+template <class TL, class T, int ND> __device__ __forceinline__ void cols_all(f32x16 (&acc)[ND], const char* lds, int o, int n, const u32x4 (&pk)[2], const f32x16& p) {
+  if constexpr (sizeof(T) == 2)
+    in_groups<2 * ND, AHEAD>([&](int i) { return TL::col16(lds, o, n, i / 2, i % 2); },
+                             [&](int i, const u32x4& a) { acc[i / 2] = mfma32<T>(a, pk[i % 2], acc[i / 2]); });
+  else
+#pragma unroll
+    for (int d = 0; d < ND; ++d) acc[d] = TL::cols(lds, o, n, d, pk, p, acc[d]);
+}
+
 // acc += what the encoded tile's rows that `seen` admits add to each column
 template <class TL, int R, int ND, class F> __device__ __forceinline__ void add_seen(f32x16 (&acc)[ND], const char* lds, F&& seen) {
   const int half = (threadIdx.x & 63) >> 5, cb = TL::col_base();
@@ -389,12 +422,11 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? (DP == 64 ? 3 : 2) : 1) void 
     f32x16 s[NS];
     __builtin_amdgcn_s_setprio(1);
 #pragma unroll
-    for (int n = 0; n < NS; ++n) {
+    for (int n = 0; n < NS; ++n)
 #pragma unroll
       for (int r = 0; r < 16; ++r) s[n][r] = 0.f;
-#pragma unroll
-      for (int c = 0; c < NP; ++c) s[n] = mfma32<T>(TL::rows(smem, sk(buf) + rb, n, c), qf[c], s[n]);
-    }
+    in_groups<NS * NP, AHEAD>([&](int i) { return TL::template rows<true>(smem, sk(buf) + rb, i / NP, i % NP); },
+                              [&](int i, const u32x4& a) { s[i / NP] = mfma32<T>(a, qf[i % NP], s[i / NP]); });
     __builtin_amdgcn_s_setprio(0);
     // in powers of two: s * m0 (plain scores are left as they are, the scale goes into the exponential's argument)
     float m0 = sc.mul;
@@ -450,8 +482,7 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? (DP == 64 ? 3 : 2) : 1) void 
       u32x4 pk[2];
       pack_tile<T>(s[n], pk);
       __builtin_amdgcn_s_setprio(1);
-#pragma unroll
-      for (int d = 0; d < ND; ++d) o[d] = TL::cols(smem, sv(buf) + cb, n, d, pk, s[n], o[d]);
+      cols_all<TL, T>(o, smem, sv(buf) + cb, n, pk, s[n]);
       __builtin_amdgcn_s_setprio(0);
     }
     if (tn >= 0) put(buf ^ 1, fulln);
@@ -858,8 +889,7 @@ __global__ __launch_bounds__(NT, NT / 256) void attn_masked_dkv_kernel(MaskP p) 
         u32x4 pk[2];
         pack_tile<T>(dp[n], pk);
         __builtin_amdgcn_s_setprio(1);
-#pragma unroll
-        for (int d = 0; d < ND; ++d) acc[d] = TL::cols(smem, sq(qprev) + cb, n, d, pk, dp[n], acc[d]);
+        cols_all<TL, T>(acc, smem, sq(qprev) + cb, n, pk, dp[n]);
         __builtin_amdgcn_s_setprio(0);
       }
     };
@@ -886,8 +916,7 @@ __global__ __launch_bounds__(NT, NT / 256) void attn_masked_dkv_kernel(MaskP p) 
 #pragma unroll
           for (int r = 0; r < 16; ++r) dp[n][r] = 0.f;
           __builtin_amdgcn_s_setprio(1);
-#pragma unroll
-          for (int c = 0; c < NP; ++c) dp[n] = mfma32<T>(TL::rows(smem, sd(buf) + rb, n, c), wf[c], dp[n]);
+          in_groups<NP, AHEAD>([&](int i) { return TL::template rows<true>(smem, sd(buf) + rb, n, i); }, [&](int i, const u32x4& a) { dp[n] = mfma32<T>(a, wf[i], dp[n]); });
           __builtin_amdgcn_s_setprio(0);
 #pragma unroll
           for (int r4 = 0; r4 < 4; ++r4) {
@@ -903,8 +932,7 @@ __global__ __launch_bounds__(NT, NT / 256) void attn_masked_dkv_kernel(MaskP p) 
 #pragma unroll
           for (int r = 0; r < 16; ++r) s[r] = 0.f;
           __builtin_amdgcn_s_setprio(1);
-#pragma unroll
-          for (int c = 0; c < NP; ++c) s = mfma32<T>(TL::rows(smem, sq(q3) + rb, n, c), wf[c], s);
+          in_groups<NP, AHEAD>([&](int i) { return TL::template rows<true>(smem, sq(q3) + rb, n, i); }, [&](int i, const u32x4& a) { s = mfma32<T>(a, wf[i], s); });
           __builtin_amdgcn_s_setprio(0);
           float m0 = sc.mul;
           if (sc.capped) {
@@ -949,8 +977,7 @@ __global__ __launch_bounds__(NT, NT / 256) void attn_masked_dkv_kernel(MaskP p) 
           u32x4 pk[2];
           pack_tile<T>(s, pk);
           __builtin_amdgcn_s_setprio(1);
-#pragma unroll
-          for (int d = 0; d < ND; ++d) acc[d] = TL::cols(smem, sd(buf) + cb, n, d, pk, s, acc[d]);
+          cols_all<TL, T>(acc, smem, sd(buf) + cb, n, pk, s);
           __builtin_amdgcn_s_setprio(0);
         }
       }
