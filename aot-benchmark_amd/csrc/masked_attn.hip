@@ -285,7 +285,7 @@ template <class T> __device__ __forceinline__ void store_out(const MaskP& p, lon
 
 // N fragments read and used in groups of A, each group's reads issued before the products of the group ahead of it (pinned reads: left to
 // itself the compiler puts every read right before its use, and a wave waits out the latency of each).  Measured at 2 x 4096 x 16 x 128 plain
-// 437 -> 420 us forward, dk / dv under a cap with four heads a key head 446 -> 420; the dq kernel, whose registers are full, lost 4 % and does without.
+// 437 -> 407 us forward, 837 -> 807 dk / dv; the dq kernel, whose registers are full, lost 4 % and does without.
 template <int N, int A, class L, class U> __device__ __forceinline__ void in_groups(L&& load, U&& use) {
   u32x4 f[2][A];
 #pragma unroll
@@ -762,7 +762,7 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void attn_masked_dq_ke
 // instead of 128 and two waves fit a SIMD, one's exponentials under the other's matrix work.  The probabilities (times the cap's derivative)
 // go through shared memory in 32 bits, lane to lane, and the second wave uses them one tile later, so the tile's one barrier suffices: the
 // tile of Q is kept a turn longer (three buffers).  One wave with both sums took 978 us for 2 x 4096 tokens and 16 heads of 128, two waves
-// that both formed S 984, this takes 837.  Where the key blocks are few, `nsplit` workgroups share the query tiles of one (every
+// that both formed S 984, this 837 and 807 with the shared-memory reads a group ahead.  Where the key blocks are few, `nsplit` workgroups share the query tiles of one (every
 // nsplit-th tile, so the split is even under a causal mask too); their 32-bit sums are added in order by sum_join_kernel.
 template <class T, int DP, int QT, int NT>
 __global__ __launch_bounds__(NT, NT / 256) void attn_masked_dkv_kernel(MaskP p) {
