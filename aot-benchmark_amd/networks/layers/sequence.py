@@ -118,9 +118,15 @@ def _no_grad(name, *tensors):
 
 
 def cache_slots(table, seq, pos, page):
-    """Places of tokens in the pool: entry pos[n] of sequence seq[n] lies at table[seq, pos // page] * page + pos % page (int32)."""
-    pos = pos.long()
-    return (table[seq.long(), pos // page].long() * page + pos % page).to(torch.int32)
+    """Places of tokens in the pool: entry pos[n] of sequence seq[n] lies at table[seq, pos // page] * page + pos % page (int32).  -1 (rope_append
+    writes nothing) for a padded token (pos or seq negative), for one outside the table, and for a page id that no int32 place can name."""
+    B, n = table.shape
+    if not table.numel():
+        return torch.full(pos.shape, -1, dtype=torch.int32, device=pos.device)
+    pos, seq = pos.long(), seq.long()
+    ok = (pos >= 0) & (pos < n * page) & (seq >= 0) & (seq < B)
+    slot = table[seq.clamp(0, B - 1), (pos // page).clamp(0, n - 1)].long() * page + pos.remainder(page)
+    return torch.where(ok & (slot >= 0) & (slot <= 0x7fffffff), slot, -1).to(torch.int32)
 
 
 def rope_append(q, k, v, pos, freqs, slots, k_pages, v_pages, interleaved=False, mscale=1.0):

@@ -166,3 +166,13 @@ def test_the_references_agree_with_torch():
     a = R.paged(q[:, 8], kp, vp, table, n)[0]
     assert torch.allclose(a, R.attention(q, k, v, causal=True)[0][:, 8], atol=1e-13)
     assert R.evict(torch.tensor([[[1., 5., 5., 0., 7., float('nan')]]]), torch.tensor([6]), 4, 1, 1, 6) == [[0, 1, 4, 5]]
+
+
+def test_cache_slots_of_padded_and_foreign_tokens():
+    from networks.layers import sequence as S
+    table = torch.tensor([[3, 0, 5], [1, -1, 1 << 28]], dtype=torch.int32)
+    seq = torch.tensor([0, 0, 1, 0, -1, 2, 0, 1, 1])
+    pos = torch.tensor([0, 47, 5, -1, 4, 4, 48, 17, 33], dtype=torch.int32)
+    got = S.cache_slots(table, seq, pos, 16)
+    assert got.dtype == torch.int32 and got.tolist() == [48, 95, 21, -1, -1, -1, -1, -1, -1]
+    assert S.cache_slots(table[:, :0], seq, pos, 16).tolist() == [-1] * 9
