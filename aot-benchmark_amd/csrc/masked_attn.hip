@@ -439,10 +439,19 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? (DP == 64 ? 3 : 2) : 1) void 
     }
     if (p.slopes) {
       const float far = (float)(i + p.off - t * KT - 4 * half);
+      const int first = q0 + wave * 32 + p.off - t * KT;         // the wave's first query, from the tile's first key
+      if (first >= KT - 1 || first <= -31) {                     // every key on one side of every query: two operations a pair, not three
+        const float sl = first > 0 ? sc.slope : -sc.slope, c = -sl * far;
 #pragma unroll
-      for (int n = 0; n < NS; ++n)
+        for (int n = 0; n < NS; ++n)
 #pragma unroll
-        for (int r = 0; r < 16; ++r) s[n][r] = s[n][r] * m0 - sc.slope * fabsf(far - (float)(n * 32 + mfma32_row(r, 0)));
+          for (int r = 0; r < 16; ++r) s[n][r] = __builtin_fmaf(s[n][r], m0, __builtin_fmaf(sl, (float)(n * 32 + mfma32_row(r, 0)), c));
+      } else {
+#pragma unroll
+        for (int n = 0; n < NS; ++n)
+#pragma unroll
+          for (int r = 0; r < 16; ++r) s[n][r] = __builtin_fmaf(s[n][r], m0, -sc.slope * fabsf(far - (float)(n * 32 + mfma32_row(r, 0))));
+      }
       m0 = 1.f;
     }
     if (!full) {
@@ -695,7 +704,7 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void attn_masked_dq_ke
       if (p.slopes) {
         const float far = (float)(i + p.off - t * KT - n * 32 - 4 * half);
 #pragma unroll
-        for (int r = 0; r < 16; ++r) s[r] = s[r] * m0 - sc.slope * fabsf(far - (float)mfma32_row(r, 0));
+        for (int r = 0; r < 16; ++r) s[r] = __builtin_fmaf(s[r], m0, -sc.slope * fabsf(far - (float)mfma32_row(r, 0)));
         m0 = 1.f;
       }
 #pragma unroll
@@ -947,7 +956,7 @@ __global__ __launch_bounds__(NT, NT / 256) void attn_masked_dkv_kernel(MaskP p) 
           if (p.slopes) {
             const float slope = p.slopes[hk * p.G + gcur] * LOG2E, far = (float)(tq * QT + n * 32 + 4 * half + p.off - t);
 #pragma unroll
-            for (int r = 0; r < 16; ++r) s[r] = s[r] * m0 - slope * fabsf(far + (float)mfma32_row(r, 0));
+            for (int r = 0; r < 16; ++r) s[r] = __builtin_fmaf(s[r], m0, -slope * fabsf(far + (float)mfma32_row(r, 0)));
             m0 = 1.f;
           }
 #pragma unroll
