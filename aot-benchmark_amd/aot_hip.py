@@ -1322,6 +1322,8 @@ def paged_attn(q, k_pages, v_pages, table, lengths, scale=None, softcap=0.0, slo
     _check_int32('paged_attn: lengths', lengths, (B,))
     if not 0 <= softcap < float('inf'):
         raise AotHipError('paged_attn: softcap must not be negative, nor infinite')
+    if scale is not None and not 0 < scale < float('inf'):
+        raise AotHipError('paged_attn: scale must be positive')
     if slopes is not None and (slopes.dtype != torch.float32 or tuple(slopes.shape) != (H,) or not slopes.is_contiguous()):
         raise AotHipError('paged_attn: slopes must be dense float32 [H]')
     for name, t, dt in (('weights', weights, torch.float32), ('key_pos', key_pos, torch.int32)):

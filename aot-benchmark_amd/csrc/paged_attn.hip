@@ -403,7 +403,7 @@ extern "C" int aot_paged_attn(const void* q, const void* k_pages, const void* v_
                               int D, int page, int max_pages, long num_pages, float scale, float softcap, const long* strides, void* stream) {
   const int es = dtype_size(dtype);
   if (!es || B < 0 || Hk < 1 || H < Hk || H % Hk || D < 1 || page < 1 || (page & (page - 1)) || max_pages < 0 || num_pages < 0 || !strides ||
-      !(softcap >= 0.f && softcap < __builtin_inff())) return AOT_ERR_BADARG;
+      !(softcap >= 0.f && softcap < __builtin_inff()) || !(scale > 0.f && scale < __builtin_inff())) return AOT_ERR_BADARG;
   const long cap = (long)page * max_pages;
   const int G = H / Hk, qt = (G + 15) / 16;
   if (D > 256 || D * es % 16 || cap > (1L << 30) || num_pages * page > 0x7fffffffL || B > 65535 || (long)Hk * qt > 65535) return AOT_ERR_UNSUPPORTED;

@@ -176,3 +176,16 @@ def test_cache_slots_of_padded_and_foreign_tokens():
     got = S.cache_slots(table, seq, pos, 16)
     assert got.dtype == torch.int32 and got.tolist() == [48, 95, 21, -1, -1, -1, -1, -1, -1]
     assert S.cache_slots(table[:, :0], seq, pos, 16).tolist() == [-1] * 9
+
+
+@pytest.mark.parametrize('scale', [0.0, -0.5, math.inf, math.nan])
+def test_one_token_attention_refuses_a_scale_that_is_not_positive(scale):
+    import aot_hip
+    from networks.layers import sequence as S
+    P, i32 = ctypes.c_void_p, lambda *s: torch.zeros(s, dtype=torch.int32)
+    strides = (ctypes.c_long * 15)()
+    assert aot_hip.load().aot_paged_attn(P(16), P(16), P(16), P(16), P(16), None, None, None, P(16), None, 0, 0, 1, 1, 1, 32, 16, 1, 4, scale, 0.0,
+                                         strides, None) == -1
+    pages = torch.zeros(6, 8, 2, 32)
+    with pytest.raises(aot_hip.AotHipError, match='scale must be positive'):
+        S.paged_attention(torch.zeros(2, 4, 32), pages, pages, i32(2, 3), i32(2), scale=scale)
