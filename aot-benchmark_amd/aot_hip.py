@@ -1161,6 +1161,8 @@ def _check_pages(name, k_pages, v_pages, dtype, D=None, Hk=None):
         raise AotHipError('%s: the page size must be a power of two (got %d)' % (name, page))
     if P * page > _I32_MAX:
         raise AotHipError('%s: a pool of %d places is too large' % (name, P * page))
+    if h < 1:
+        raise AotHipError('%s: pages need at least one key head' % name)
     if (k_pages.stride(3) != 1 or v_pages.stride(3) != 1) and d != 1:
         raise AotHipError('%s: the last dimension of the pages must be dense' % name)
     return P, page, h, d
@@ -1207,7 +1209,7 @@ def rope_append(q, k, v, pos, freqs, slots, k_pages, v_pages, interleaved=False,
         st = _strides(q, 2) + st + (H * D, D)
     else:
         st = _NO2 + st + _NO2
-    if N and Hk:
+    if N:
         _chk(load().aot_rope_append(_ptr(q), k.data_ptr(), v.data_ptr(), _ptr(qo), k_pages.data_ptr(), v_pages.data_ptr(), pos.data_ptr(),
                                     slots.data_ptr(), freqs.data_ptr(), dtype, N, H, Hk, D, rot, 1 if interleaved else 0, mscale, page, P,
                                     _longs(st + _strides(k_pages, 3) + _strides(v_pages, 3)), _raw_stream(dev)),
@@ -1307,7 +1309,7 @@ def paged_attn(q, k_pages, v_pages, table, lengths, scale=None, softcap=0.0, slo
         raise AotHipError('paged_attn: q must be [B, H, D] of float32 / float16 / bfloat16')
     B, H, D = q.shape
     P, page, Hk, _ = _check_pages('paged_attn', k_pages, v_pages, q.dtype, D)
-    if Hk < 1 or H < Hk or H % Hk:
+    if H < Hk or H % Hk:
         raise AotHipError('paged_attn: %d query heads on %d key heads' % (H, Hk))
     if D < 1 or D > 256 or D * q.element_size() % 16:
         raise AotHipError('paged_attn: head width %d of %s not supported (whole 16-byte pieces, at most 256)' % (D, q.dtype))
@@ -1389,7 +1391,7 @@ def paged_evict(k_pages, v_pages, table, lengths, weights, new_table, budget, si
     new_lengths = torch.empty(B, dtype=torch.int32, device=k_pages.device)
     new_weights = torch.empty((B, Hk, S), dtype=torch.float32, device=k_pages.device)
     new_pos = torch.empty((B, Hk, S), dtype=torch.int32, device=k_pages.device) if key_pos is not None else None
-    if B and Hk:
+    if B:
         if not mp:
             raise AotHipError('paged_evict: table has no pages')
         st = _strides(k_pages, 3) + _strides(v_pages, 3) + _strides(table, 1) + _strides(new_table, 1) + _strides(weights, 2) + (Hk * S, S)
