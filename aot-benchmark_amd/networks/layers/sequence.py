@@ -62,7 +62,9 @@ class _Rope(Function):
 def rope(q, k, pos, freqs, interleaved=False, mscale=1.0):
     """Rotary positions, differentiable in q and k.  q [B, S, H, D], k [B, S, Hk, D] or None (then one tensor is returned); pos int32 [B, S] or
     [S]; freqs float64 [rot / 2] (rope_freqs): the first rot elements of every head turn by pos * freqs, in pairs (j, j + rot / 2), or
-    (2j, 2j + 1) if interleaved, and are multiplied by mscale; the others pass."""
+    (2j, 2j + 1) if interleaved, and are multiplied by mscale; the others pass.  freqs has no gradient."""
+    if freqs.requires_grad and torch.is_grad_enabled():
+        raise AotHipError('rope: freqs have no gradient; pass freqs.detach()')
     if pos.dim() == 1:
         pos = pos.expand(q.shape[0], -1)
     if k is None:
@@ -132,7 +134,7 @@ def cache_slots(table, seq, pos, page):
 def rope_append(q, k, v, pos, freqs, slots, k_pages, v_pages, interleaved=False, mscale=1.0):
     """Turns the new tokens' q [N, H, D] (or None) and k [N, Hk, D] by pos int32 [N], writes the turned keys and v [N, Hk, D] to the places slots
     int32 [N] (cache_slots; negative: a padded token, nothing is written) of k_pages / v_pages [pages, page, Hk, D], returns the turned q."""
-    _no_grad('rope_append', q, k, v, k_pages, v_pages)
+    _no_grad('rope_append', q, k, v, freqs, k_pages, v_pages)
     return aot_hip.rope_append(q, k, v, pos, freqs, slots, k_pages, v_pages, bool(interleaved), float(mscale))
 
 
