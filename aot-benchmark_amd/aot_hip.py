@@ -1377,8 +1377,8 @@ def paged_evict(k_pages, v_pages, table, lengths, weights, new_table, budget, si
         raise AotHipError('paged_evict: sink %d + recent %d must fit the budget %d' % (sink, recent, budget))
     if npg * page < budget:
         raise AotHipError('paged_evict: new_table holds %d entries, the budget is %d' % (npg * page, budget))
-    if mp * page > _I32_MAX or npg * page > _I32_MAX or B > 65535 or Hk > 65535:
-        raise AotHipError('paged_evict: sizes beyond 2^31 entries or 65535 rows')
+    if mp * page > 1 << 30 or npg * page > 1 << 30 or budget >= 1 << 29 or B > 65535 or Hk > 65535:
+        raise AotHipError('paged_evict: sizes beyond 2^30 entries, a budget of 2^29 or 65535 rows')
     dev = _device_of(k_pages, v_pages, table, lengths, weights, new_table, key_pos)
     if stream is not None or _current_device() != dev:
         with _elsewhere(dev, stream):

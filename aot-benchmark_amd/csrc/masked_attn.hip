@@ -1062,7 +1062,7 @@ static int mask_args(int dtype, int B, int Sq, int Sk, int H, int Hk, int D, flo
   const int es = dtype_size(dtype);
   if (!es || B < 0 || Sq < 0 || Sk < 0 || Hk < 1 || H < Hk || H % Hk || D < 1 || !strides || !(softcap >= 0.f && softcap < __builtin_inff()) || !(scale > 0.f && scale < __builtin_inff())) return AOT_ERR_BADARG;   // (a running maximum of unscaled scores needs a positive scale)
   if ((doc_q == nullptr) != (doc_k == nullptr) || (doc_q && !ranges)) return AOT_ERR_BADARG;
-  if (D > 128 || D * es % 16 || Sq > (1 << 22) || Sk > (1 << 22) || (long)B * H > 0x7fffffffL || B > 65535) return AOT_ERR_UNSUPPORTED;
+  if (D > 128 || D * es % 16 || Sq > (1 << 22) || Sk > (1 << 22) || (long)B * H * 512 > 0xffffffffL || B > 65535) return AOT_ERR_UNSUPPORTED;
   return AOT_OK;
 }
 static bool rows_aligned(const void* x, const long* st, int es) {

@@ -428,6 +428,9 @@ extern "C" int aot_paged_attn(const void* q, const void* k_pages, const void* v_
   p.ml = work + (long)B * H * p.nsplit * D;
   p.scores = work + part_floats(B, H, D, p.nsplit);
   const bool split = need > 0;
+  p.osplit = p.nsplit >= 32 && D % 32 == 0 ? D / 32 : 1;          // many splits: a head's output by 32 columns a workgroup
+  const long joins = (long)B * H * p.osplit + (weights ? (long)B * Hk * ((cap + JOIN_KEYS - 1) / JOIN_KEYS) : 0);
+  if (split && joins >= 1L << 24) return AOT_ERR_UNSUPPORTED;     // (a launch's work items are below 2^32)
   const dim3 grid(p.nsplit, Hk * qt, B);
   hipStream_t st = (hipStream_t)stream;
   with_dtype(dtype, [&](auto t) {
@@ -444,10 +447,7 @@ extern "C" int aot_paged_attn(const void* q, const void* k_pages, const void* v_
   hipError_t e = hipGetLastError();
   if (e != hipSuccess) return (int)e;
   if (split) {
-    p.osplit = p.nsplit >= 32 && D % 32 == 0 ? D / 32 : 1;        // many splits: a head's output by 32 columns a workgroup
-    const long blocks = (long)B * H * p.osplit + (weights ? (long)B * Hk * ((cap + JOIN_KEYS - 1) / JOIN_KEYS) : 0);
-    if (blocks > 0x7fffffffL) return AOT_ERR_UNSUPPORTED;
-    with_dtype(dtype, [&](auto t) { hipLaunchKernelGGL((paged_join_kernel<decltype(t)>), dim3((unsigned)blocks), dim3(256), 0, st, p); });
+    with_dtype(dtype, [&](auto t) { hipLaunchKernelGGL((paged_join_kernel<decltype(t)>), dim3((unsigned)joins), dim3(256), 0, st, p); });
   }
   AOT_LAUNCH_CHECK();
 }

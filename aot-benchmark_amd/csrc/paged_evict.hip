@@ -201,7 +201,9 @@ extern "C" int aot_paged_evict(void* k_pages, void* v_pages, const int* table, c
   const int es = dtype_size(dtype);
   if (!es || B < 0 || Hk < 1 || D < 1 || S < 0 || page < 1 || (page & (page - 1)) || max_pages < 0 || new_pages < 0 || num_pages < 0 || !strides ||
       budget < 1 || sink < 0 || recent < 0 || (long)sink + recent > budget || (long)new_pages * page < budget) return AOT_ERR_BADARG;
-  if (num_pages * page > 0x7fffffffL || (long)max_pages * page > 0x7fffffffL || B > 65535 || Hk > 65535) return AOT_ERR_UNSUPPORTED;
+  // (a row's entries, and the runs of them that the waves take, are counted in 32 bits; a launch's work items are below 2^32)
+  if (num_pages * page > 0x7fffffffL || (long)max_pages * page > (1L << 30) || (long)new_pages * page > (1L << 30) || budget >= 1 << 29 || B > 65535 ||
+      Hk > 65535) return AOT_ERR_UNSUPPORTED;
   if (B == 0) return AOT_OK;
   if (!k_pages || !v_pages || !table || !new_table || table == new_table || !lengths || !weights || !kept || !new_lengths || !new_weights ||
       new_weights == weights || lengths == new_lengths || (key_pos && (!new_key_pos || new_key_pos == key_pos))) return AOT_ERR_BADARG;

@@ -123,7 +123,7 @@ static int rope_launch(RopeP& p, int dtype, hipStream_t stream) {
   p.R = p.rows >= 8192 ? 4 : 1;
   const size_t lds = (size_t)p.R * (p.rot / 2) * sizeof(float2);
   const long blocks = (p.rows + p.R - 1) / p.R;
-  if (blocks > 0x7fffffffL) return AOT_ERR_UNSUPPORTED;
+  if (blocks >= 1L << 24) return AOT_ERR_UNSUPPORTED;          // (a launch's work items are below 2^32)
   auto go = [&](auto t, auto w) {
     using T = decltype(t);
     if constexpr (decltype(w)::value * sizeof(T) <= 16) hipLaunchKernelGGL((rope_kernel<T, decltype(w)::value, APPEND>), dim3((unsigned)blocks), dim3(256), lds, stream, p);

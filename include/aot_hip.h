@@ -525,6 +525,7 @@ int aot_window_scatter_f32(const float* win, float* dense, int G, int h, int w, 
  * else (j, j + rot / 2); the rest of the head is copied.  inverse: the negated angle -- with the same mscale the gradient of the forward
  * turn.  H or Hk may be 0 (its pointers NULL); qo == q / ko == k (same strides) turns in place.  Any strides and alignment for
  * half-split pairs; interleaved ones need D even, pairs aligned to their size and even strides.
+ * B * S < 2^26.
  * strides: q b s h, k b s h, qo b s h, ko b s h, pos b s (14).  Beside the sine positions of networks/layers/position.py:33-74. */
 int aot_rope(const void* q, const void* k, void* qo, void* ko, const int* pos, const double* freqs, int dtype, int B, int S,
              int H, int Hk, int D, int rot, int interleaved, int inverse, float mscale, const long* strides, void* stream);
@@ -544,7 +545,7 @@ int aot_rope_append(const void* q, const void* k, const void* v, void* qo, void*
  * only); doc_q [B, Sq] / doc_k [B, Sk] both or neither, then `ranges` is scratch of 16 * B * (ceil(Sq / 64) + ceil(Sk / 64)) bytes, 16-byte
  * aligned.  residual (16-bit types, dense [B, Sq, H, D], or NULL): what rounding out left, for the backward call.  work: scratch of
  * aot_attn_masked_floats(.., 0, ..) floats (0: may be NULL), 16-byte aligned.  D <= 128, rows of whole 16-byte pieces, 16-byte aligned, outputs
- * too.  Sq, Sk <= 2^22.
+ * too.  Sq, Sk <= 2^22; B * H < 2^23.
  * strides: q b s h, k b s h, v b s h, out b s h, doc_q b, doc_k b (14).  Beside aot_attn_f32 (attention.py:82-117). */
 int aot_attn_masked(const void* q, const void* k, const void* v, void* out, void* residual, float* lse, const float* slopes,
                     const int* doc_q, const int* doc_k, const int* prefix, void* ranges, float* work, long work_floats, int dtype, int B, int Sq, int Sk, int H, int Hk, int D,
@@ -578,7 +579,7 @@ int aot_paged_attn_work_floats(int B, int H, int Hk, int D, int page, int max_pa
 
 /* Eviction by collected weight: of the lengths[b] entries of every (sequence, key head) the first `sink`, the last `recent` and the
  * heaviest others stay, `budget` in all (all of them if there are no more), ties to the lower index, NaN lightest.  The kept entries' K / V
- * rows are copied in order to the pages of new_table [B, new_pages] (new_pages * page >= budget; pages of the pool that no live sequence
+ * rows are copied in order to the pages of new_table [B, new_pages] (max_pages * page, new_pages * page <= 2^30; new_pages * page >= budget < 2^29; pages of the pool that no live sequence
  * reads -- the old pages are left as they are and may be shared).  kept [B, Hk, budget]: their old indices, -1 behind the last;
  * new_lengths [B]; new_weights / new_key_pos [B, Hk, S]: moved along, zero behind the last (key_pos optional, both or neither).  A page id
  * outside the pool moves nothing; a negative id in new_table keeps a sequence where it is (its indices are still reported).

@@ -31,3 +31,26 @@ def test_frequencies_that_want_a_gradient_are_refused():
             S.rope(q, other, pos, f)
     with pytest.raises(AotHipError, match='serving call'):
         S.rope_append(q[0], k[0], k[0], pos[0], f, pos[0], kp, kp)
+
+
+def test_sizes_past_the_kernels_index_range_are_refused():
+    """Eviction counts a row's entries and the waves' runs of them in 32 bits: 2^30 entries a row, as in paged attention.  A launch's work
+    items are below 2^32 a dimension, which is looked at before anything is launched."""
+    import ctypes
+    import aot_hip
+    from networks.layers import sequence as S
+    lib, P = aot_hip.load(), ctypes.c_void_p
+    z14, z16 = (ctypes.c_long * 14)(), (ctypes.c_long * 16)()
+
+    def evict(page=1 << 16, mp=1, npg=1, budget=16):
+        return lib.aot_paged_evict(P(16), P(16), P(16), P(32), P(16), P(16), None, P(16), P(32), P(32), None, 1, 1, 1, 32, mp * page, page, mp, npg, 9, budget,
+                                   1, 1, z16, None)
+    assert evict(mp=(1 << 14) + 1) == -2 and evict(npg=(1 << 14) + 1) == -2 and evict(npg=1 << 14, budget=1 << 29) == -2
+    page, i = torch.zeros(1, 1 << 10, 2, 32), i32(1)
+    with pytest.raises(aot_hip.AotHipError, match='beyond'):
+        S.paged_evict(page, page, i32(1, (1 << 20) + 1), i, torch.zeros(1).expand(1, 2, (1 << 30) + (1 << 10)), i32(1, 1), 8)
+    with pytest.raises(aot_hip.AotHipError, match='beyond'):
+        S.paged_evict(page, page, i32(1, 1), i, torch.zeros(1, 2, 1 << 10), i32(1, (1 << 20) + 1), 8)
+    assert lib.aot_rope(P(16), None, P(16), None, P(16), P(16), 0, 1 << 13, 1 << 13, 1, 0, 32, 32, 0, 0, 1.0, z14, None) == -2      # 2^26 tokens, four a workgroup
+    assert lib.aot_attn_masked(P(16), P(16), P(16), P(16), None, P(16), None, None, None, None, None, None, 0, 0, 1 << 12, 1, 1, 1 << 12, 1, 32, 0, 1.0, 0.0,
+                               z14, None) == -2
