@@ -41,6 +41,7 @@ struct MaskP {
   float *qpart, *ml;                                           // split keys: sums [qsplit][B][Sq][H][D], (m, l) [qsplit][B][Sq][H][2]
   int B, Sq, Sk, H, Hk, G, D, causal, off, nsplit, qsplit;
   float scale, softcap;
+  Cap cap;
 };
 
 __global__ __launch_bounds__(256) void doc_range_kernel(const int* dq, const int* dk, int4* rq, int4* rk, int Sq, int Sk, long qs, long ks) {
@@ -265,14 +266,10 @@ __device__ __forceinline__ Head head_of(int x, const MaskP& p) {
 }
 
 struct Score {
-  float mul, cap2, slope;
+  float mul, slope;
   bool capped;
-  __device__ __forceinline__ Score(const MaskP& p, int h) {
-    capped = p.softcap > 0.f;
-    mul = capped ? p.scale * 2.f * LOG2E / p.softcap : p.scale * LOG2E;
-    cap2 = p.softcap * LOG2E;
-    slope = p.slopes ? p.slopes[h] * LOG2E : 0.f;
-  }
+  Cap cap;
+  __device__ __forceinline__ Score(const MaskP& p, int h) : mul(p.cap.lin), slope(p.slopes ? p.slopes[h] * LOG2E : 0.f), capped(p.softcap > 0.f), cap(p.cap) {}
 };
 
 // four elements e .. of an output row, and what their rounding left (for the backward pass' do.o) where it is asked for
@@ -432,10 +429,7 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? (DP == 64 ? 3 : 2) : 1) void 
     float m0 = sc.mul;
     if (sc.capped) {
       m0 = 1.f;
-#pragma unroll
-      for (int n = 0; n < NS; ++n)
-#pragma unroll
-        for (int r = 0; r < 16; ++r) s[n][r] = sc.cap2 * tanh_from_exp2(s[n][r] * sc.mul);
+      sc.cap.tiles(s);
     }
     if (p.slopes) {
       const float far = (float)(i + p.off - t * KT - 4 * half);
@@ -567,7 +561,7 @@ __global__ __launch_bounds__(256) void attn_masked_join_kernel(MaskP p) {
 
 // ---- gradient of the queries -----------------------------------------------------------------------------------------------------
 template <class T, int DP, int KT>
-__global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void attn_masked_dq_kernel(MaskP p) {
+__global__ __launch_bounds__(256, (sizeof(T) == 2 ? 2 : 1) + (DP == 32)) void attn_masked_dq_kernel(MaskP p) {
   using TL = Tile<T, DP, KT, 256>;
   constexpr int NP = TL::NCH / 2, ND = DP / 32, NS = KT / 32;
   __shared__ __align__(16) char smem[4 * TL::BYTES + 2 * KT * 4 + 32];
@@ -680,7 +674,8 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void attn_masked_dq_ke
     if (tn >= 0) fetch(tn);
 #pragma unroll
     for (int n = 0; n < NS; ++n) {
-      f32x16 s, dp;
+      f32x16 st[1], dp;
+      f32x16& s = st[0];
 #pragma unroll
       for (int r = 0; r < 16; ++r) { s[r] = 0.f; dp[r] = 0.f; }
       __builtin_amdgcn_s_setprio(1);
@@ -694,12 +689,7 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void attn_masked_dq_ke
       float m0 = sc.mul;
       if (sc.capped) {
         m0 = 1.f;
-#pragma unroll
-        for (int r = 0; r < 16; ++r) {
-          const float th = tanh_from_exp2(s[r] * sc.mul);
-          s[r] = sc.cap2 * th;
-          dp[r] *= 1.f - th * th;
-        }
+        sc.cap.tile(st, [&](int r, float d) { dp[r] *= d; });
       }
       if (p.slopes) {
         const float far = (float)(i + p.off - t * KT - n * 32 - 4 * half);
@@ -937,7 +927,8 @@ __global__ __launch_bounds__(NT, NT / 256) void attn_masked_dkv_kernel(MaskP p) 
       } else {
 #pragma unroll
         for (int n = 0; n < NS; ++n) {
-          f32x16 s, dcap;
+          f32x16 st[1], dcap;
+          f32x16& s = st[0];
 #pragma unroll
           for (int r = 0; r < 16; ++r) s[r] = 0.f;
           __builtin_amdgcn_s_setprio(1);
@@ -946,12 +937,7 @@ __global__ __launch_bounds__(NT, NT / 256) void attn_masked_dkv_kernel(MaskP p) 
           float m0 = sc.mul;
           if (sc.capped) {
             m0 = 1.f;
-#pragma unroll
-            for (int r = 0; r < 16; ++r) {
-              const float th = tanh_from_exp2(s[r] * sc.mul);
-              s[r] = sc.cap2 * th;
-              dcap[r] = 1.f - th * th;
-            }
+            sc.cap.tile(st, [&](int r, float d) { dcap[r] = d; });
           }
           if (p.slopes) {
             const float slope = p.slopes[hk * p.G + gcur] * LOG2E, far = (float)(tq * QT + n * 32 + 4 * half + p.off - t);
@@ -1072,7 +1058,7 @@ static bool rows_aligned(const void* x, const long* st, int es) {
 static void mask_common(MaskP& p, int B, int Sq, int Sk, int H, int Hk, int D, int causal, float scale, float softcap, const float* slopes,
                         const int* doc_q, const int* doc_k, const int* prefix, void* ranges) {
   p.B = B; p.Sq = Sq; p.Sk = Sk; p.H = H; p.Hk = Hk; p.G = H / Hk; p.D = D; p.causal = causal != 0; p.off = Sk - Sq;
-  p.scale = scale; p.softcap = softcap; p.slopes = slopes; p.doc_q = doc_q; p.doc_k = doc_k; p.prefix = causal ? prefix : nullptr;
+  p.scale = scale; p.softcap = softcap; p.cap = Cap::of(scale, softcap); p.slopes = slopes; p.doc_q = doc_q; p.doc_k = doc_k; p.prefix = causal ? prefix : nullptr;
   p.rq = (const int4*)ranges;
   p.rk = p.rq + (long)B * ((Sq + RG - 1) / RG);
 }

@@ -29,6 +29,7 @@ struct PagedP {
   long num_pages, S;
   int B, H, Hk, G, D, cap_len, page_shift, chunk, nsplit, osplit;
   float scale, softcap;
+  Cap cap;
 };
 
 template <class T> __device__ __forceinline__ f32x4 mfma16(const u32x4& a, const u32x4& b, f32x4 c) {
@@ -75,7 +76,7 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? (DP == 128 ? 3 : DP == 256 ? 
     }
   }
   const bool capped = p.softcap > 0.f;
-  const float mul = capped ? p.scale * 2.f * LOG2E / p.softcap : p.scale * LOG2E, cap2 = p.softcap * LOG2E;
+  const Cap cap = p.cap;
   const float slope = p.slopes ? p.slopes[h] * LOG2E : 0.f;
   const int* kpos = p.key_pos ? p.key_pos + b * p.ps[0] + hk * p.ps[1] : nullptr;
   const int qpos = len > 0 ? (kpos ? kpos[len - 1] : len - 1) : 0;
@@ -172,8 +173,8 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? (DP == 128 ? 3 : DP == 256 ? 
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
       const int t = t0 + (j >> 2) * 16 + kg * 4 + (j & 3);
-      float y = s[j >> 2][j & 3] * mul;
-      if (capped) y = cap2 * tanh_from_exp2(y);
+      const float raw = s[j >> 2][j & 3];
+      float y = capped ? cap(raw) : raw * cap.lin;
       if (p.slopes) y -= slope * fabsf((float)(qpos - (kpos ? (blk.ok >> j & 1 ? kpos[t] : 0) : t)));
       x[j] = blk.ok >> j & 1 ? y : NEG_INF;
       mx = fmaxf(mx, x[j]);
@@ -421,7 +422,7 @@ extern "C" int aot_paged_attn(const void* q, const void* k_pages, const void* v_
   p.num_pages = num_pages;
   p.B = B; p.H = H; p.Hk = Hk; p.G = G; p.D = D; p.cap_len = (int)cap; p.S = score_row(cap);
   while ((1 << p.page_shift) < page) ++p.page_shift;
-  p.scale = scale; p.softcap = softcap;
+  p.scale = scale; p.softcap = softcap; p.cap = Cap::of(scale, softcap);
   const long need = paged_work(B, H, Hk, D, cap, weights != nullptr, &p.chunk, &p.nsplit);
   if (need && (!work || !aligned16(work) || work_floats < need)) return AOT_ERR_BADARG;
   p.part = work;

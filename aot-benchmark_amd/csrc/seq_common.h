@@ -51,9 +51,82 @@ template <class T> __device__ __forceinline__ unsigned word_finite(unsigned x) {
   }
 }
 
-// s -> cap * tanh(s / cap) as 1 - 2 / (1 + exp(2 x)): absolute error a few 2^-24 of cap, exact limits at both ends
-// (x = s * 2 log2(e) / cap on entry).  Returns the tanh.
-__device__ __forceinline__ float tanh_from_exp2(float x) { return 1.f - 2.f * rcp_hw(1.f + exp2_hw(x)); }
+// The cap on a score, in powers of two: s -> cap log2(e) tanh(y), y = s scale / cap, from x = 2 log2(e) y, and the cap's derivative
+// 1 - tanh^2.  With E = exp(-2 |y|) = exp2(-|x|):
+//   |x| >= 1   tanh = +-(1 - E) / (1 + E) and 1 - tanh^2 = 4 E / (1 + E)^2: no cancellation that counts (1 - E is exact and at least 1/2),
+//              infinities give +-1 and 0
+//   |x| < 1    tanh = y (1 + z P(z)), z = x^2, P a minimax fit of (tanh(y) / y - 1) / z on [0, 1] (least squares on Chebyshev nodes, reweighted
+//              until level): 0.6 2^-24 of the value.  As s log2(e) scale (1 + z P) the score's error is relative to the score whatever the cap
+//              (1 - 2 / (1 + exp(2 y)) leaves a few 2^-24 of the cap: noise of the size of the scores where the cap is 1e6).
+// A tile all of whose scores are small, which is the rule under the caps in use, takes the polynomial alone: 7 plain operations a
+// score instead of 6 with two of quarter rate.
+struct Cap {
+  float mul, lin, top;                                          // s -> x; scale log2(e); cap log2(e)
+  static Cap of(float scale, float cap) { return Cap{std::min(scale * 2.f * LOG2E / cap, 3.0e38f), scale * LOG2E, cap * LOG2E}; }
+  __device__ __forceinline__ float bend(float x) const {        // tanh(y) / y, |x| < 1
+    const float z = x * x;
+    return __builtin_fmaf(z, __builtin_fmaf(z, __builtin_fmaf(z, -8.533986692782491e-05f, 0.0019189956365153193f), -0.04003699868917465f), 1.f);
+  }
+  __device__ __forceinline__ float far(float s, float E, float r) const { return __builtin_copysignf(top * ((1.f - E) * r), s); }
+  __device__ __forceinline__ float operator()(float s) const {
+    const float x = s * mul, E = exp2_hw(-fabsf(x)), near = s * lin * bend(x), away = far(s, E, rcp_hw(1.f + E));
+    return fabsf(x) < 1.f ? near : away;                        // (both formed first: a selection, not a branch a lane)
+  }
+  template <int N> __device__ __forceinline__ bool small(const f32x16 (&s)[N]) const {     // of the whole wave (NaN aside)
+    float a = 0.f;
+#pragma unroll
+    for (int n = 0; n < N; ++n)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) a = fmaxf(a, fabsf(s[n][r]));
+    return !__any(a * mul >= 1.f);
+  }
+  template <int N> __device__ __forceinline__ void tiles(f32x16 (&s)[N]) const {
+    if (small(s)) {
+#pragma unroll
+      for (int n = 0; n < N; ++n)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) s[n][r] = s[n][r] * lin * bend(s[n][r] * mul);
+    } else {
+      Cap c = *this;
+      asm("" : "+s"(c.mul), "+s"(c.lin));                        // (as below)
+#pragma unroll
+      for (int n = 0; n < N; ++n)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+          s[n][r] = c(s[n][r]);
+          if (r % 2) __builtin_amdgcn_sched_barrier(0);
+        }
+      asm volatile("");
+    }
+  }
+  // a tile's scores, and slope(r, the derivative) for each
+  template <class F> __device__ __forceinline__ void tile(f32x16 (&s)[1], F&& slope) const {
+    constexpr float HALF_LN2 = 0.34657359027997265f;
+    if (small(s)) {
+#pragma unroll
+      for (int r = 0; r < 16; ++r) {
+        const float x = s[0][r] * mul, w = bend(x), th = x * HALF_LN2 * w;
+        s[0][r] = s[0][r] * lin * w;
+        slope(r, __builtin_fmaf(-th, th, 1.f));
+        if (r % 4 == 3) __builtin_amdgcn_sched_barrier(0);
+      }
+    } else {
+      // Registers decide here.  Without the empty statements the compiler forms what both branches begin with ahead of them and what they end
+      // with behind them, for all sixteen scores, and without the fences it works on all of them side by side: 40 and more registers, spilled.
+      Cap c = *this;
+      asm("" : "+s"(c.mul), "+s"(c.lin));
+#pragma unroll
+      for (int r = 0; r < 16; ++r) {
+        const float x = s[0][r] * c.mul, E = exp2_hw(-fabsf(x)), q = rcp_hw(1.f + E), w = bend(x), th = x * HALF_LN2 * w, two = q + q;
+        const float near = s[0][r] * c.lin * w, away = c.far(s[0][r], E, q), dn = __builtin_fmaf(-th, th, 1.f), da = E * two * two;
+        s[0][r] = fabsf(x) < 1.f ? near : away;
+        slope(r, fabsf(x) < 1.f ? dn : da);
+        if (r % 2) __builtin_amdgcn_sched_barrier(0);
+      }
+      asm volatile("");
+    }
+  }
+};
 
 // dtype code of the C ABI -> f(type tag); false for an unknown code
 template <class F> static inline bool with_dtype(int dtype, F&& f) {

@@ -1,0 +1,99 @@
+"""Edges of the token-sequence operators on the MI355X, against their definitions in 64 bits (tests/sequence_refs.py, sequence_edge_refs.py)."""
+import pytest
+import torch
+
+import sequence_edge_refs as X
+import sequence_refs as R
+from test_sequence_gpu import DT, cache, docs_of, rand, seq, within         # noqa: F401  (seq: the fixture)
+
+pytestmark = pytest.mark.gpu
+
+
+def results(seq, q, k, v, do, **o):                                        # noqa: F811
+    lead = [x.detach().requires_grad_() for x in (q, k, v)]
+    out = seq.masked_attention(*lead, **o)
+    return [out.detach()] + list(torch.autograd.grad(out, lead, do))
+
+
+# ---- eviction: rows longer than the registers hold, read again in every pass ------------------------------------------------------
+@pytest.mark.parametrize('lens,page,K,budget,sink,recent,kind', [
+    ([16384, 16383, 16321], 64, 2, 4096, 4, 128, 'random'), ([16385, 900, 1, 0], 64, 2, 4097, 0, 0, 'ties'), ([16385], 1, 1, 16384, 3, 5, 'random'),
+    ([70000, 33333, 700, 65536], 16, 2, 5000, 7, 1000, 'random'), ([70001, 1023], 16, 1, 1000, 0, 0, 'ties'), ([40000], 256, 1, 640, 64, 0, 'same'),
+    ([50000, 20001], 64, 1, 8191, 1, 1, 'nan'), ([131072, 130000], 64, 1, 4096, 4, 1024, 'nan')])
+def test_paged_evict_of_long_rows(seq, lens, page, K, budget, sink, recent, kind):      # noqa: F811
+    B, D, dt = len(lens), 8, torch.float16
+    kp, vp, table, _ = cache(B, max(lens), page, K, D, dt, 1)
+    more = -(-budget // page)
+    kp, vp = (torch.cat([x, rand((B * more, page, K, D), dt, 5)]) for x in (kp, vp))
+    new = (torch.arange(B * more, device='cuda') + kp.shape[0] - B * more).to(torch.int32).view(B, more)
+    S = table.shape[1] * page
+    w = torch.rand(B, K, S, device='cuda', generator=torch.Generator(device='cuda').manual_seed(3))
+    if kind == 'ties':
+        w = (w * 4).floor()
+    elif kind == 'same':
+        w.fill_(0.5)
+    elif kind == 'nan':
+        w[..., ::3] = float('nan')
+        w[..., 1::500] = float('inf')
+    lengths = torch.tensor(lens, dtype=torch.int32, device='cuda')
+    pos = torch.arange(S, dtype=torch.int32, device='cuda').expand(B, K, S) * 3 + 1
+    k0, v0 = kp.clone(), vp.clone()
+    kept, n, nw, npos = seq.paged_evict(kp, vp, table, lengths, w, new, budget, sink, recent, key_pos=pos)
+    rows = R.evict(w.cpu(), lengths.cpu(), budget, sink, recent, S)
+    assert n.tolist() == [min(x, budget) for x in lens]
+    j = torch.arange(budget, device='cuda')
+    for b in range(B):
+        for h in range(K):
+            want = torch.tensor(rows[b * K + h], dtype=torch.long, device='cuda')
+            m = len(want)
+            assert torch.equal(kept[b, h, :m].long(), want) and bool((kept[b, h, m:] == -1).all())
+            assert torch.equal(nw[b, h, :m].view(torch.int32), w[b, h, want].view(torch.int32)) and not nw[b, h, m:].any()
+            assert torch.equal(npos[b, h, :m], pos[b, h, want]) and not npos[b, h, m:].any()
+            src, at = table[b].long()[want // page], new[b].long()[j[:m] // page]
+            for x0 in (k0, v0):
+                x0[at, j[:m] % page, h] = x0[src, want % page, h]
+    assert torch.equal(kp, k0) and torch.equal(vp, v0)
+
+
+# ---- the cap, large and small ------------------------------------------------------------------------------------------------------
+@pytest.mark.parametrize('softcap', [1e-3, 0.5, 4.0, 20.0, 50.0, 1e3, 1e6, 1e8, 3e38])
+@pytest.mark.parametrize('D,H,K,causal', [(64, 4, 2, True), (128, 2, 2, False), (32, 2, 1, True)])
+def test_cap_of_any_size(seq, softcap, D, H, K, causal):                   # noqa: F811
+    """In 32 bits, errors relative to the capped score and not to the cap; a cap far past the scores is no cap."""
+    q, k, v, do = rand((1, 150, H, D), torch.float32, 1, 2.0), rand((1, 170, K, D), torch.float32, 2), rand((1, 170, K, D), torch.float32, 3), rand((1, 150, H, D), torch.float32, 4)
+    got = results(seq, q, k, v, do, causal=causal, softcap=softcap)
+    for name, g, (want, bound) in zip(('out', 'dq', 'dk', 'dv'), got, X.attention(q, k, v, do, causal=causal, softcap=softcap)):
+        within(name, g, want, bound)
+    if softcap >= 1e6:                                                      # (1 - (s / cap)^2 / 3 rounds to one)
+        for name, g, (want, bound) in zip(('out', 'dq', 'dk', 'dv'), got, X.attention(q, k, v, do, causal=causal)):
+            within(name, g, want, 2 * bound)
+
+
+@pytest.mark.parametrize('dtype', ['f32', 'bf16'])
+def test_gradients_of_scores_near_the_cap(seq, dtype):                      # noqa: F811
+    """Every score three to eight times the cap: the cap's derivative is 1e-2 to 1e-6 and keeps its relative accuracy, on both sides of zero."""
+    dt = DT[dtype]
+    q, k, v, do = (rand((1, 70, 2, 64), dt, i) for i in range(4))
+    side = torch.where(torch.arange(70, device='cuda') % 2 == 0, 1.0, -1.0)
+    q, k = (0.02 * q.float() + 1.0).to(dt), ((0.02 * k.float() + 1.0) * side[None, :, None, None]).to(dt)      # scores near +-8
+    for softcap in (1.0, 2.5):
+        got = results(seq, q, k, v, do, softcap=softcap)
+        for name, g, (want, bound) in zip(('out', 'dq', 'dk', 'dv'), got, X.attention(q, k, v, do, softcap=softcap)):
+            within(name, g, want, bound)
+
+
+@pytest.mark.parametrize('softcap', [1e-3, 20.0, 1e3, 1e6, 3e38])
+@pytest.mark.parametrize('D', [32, 128, 256])
+def test_cap_of_any_size_over_pages(seq, softcap, D):                       # noqa: F811
+    kp, vp, table, _ = cache(2, 700, 16, 2, D, torch.float32, 1)
+    q, lengths = rand((2, 4, D), torch.float32, 7, 2.0), torch.tensor([700, 333], dtype=torch.int32, device='cuda')
+    w = torch.zeros(2, 2, table.shape[1] * 16, device='cuda')
+    out = seq.paged_attention(q, kp, vp, table, lengths, softcap=softcap, weights=w)
+    for b, n in enumerate(lengths.tolist()):
+        t = torch.arange(n, device='cuda')
+        k, v = (x[table[b].long()[t // 16], t % 16][None] for x in (kp, vp))
+        want, bound = X.attention(q[b][None, None], k, v, torch.zeros_like(q[b])[None, None], softcap=softcap)[0]
+        within('out', out[b][None, None], want, bound + 16 * R.E32 * want.abs())      # (the join over splits)
+        unit = torch.eye(n, device='cuda')[None, :, None].expand(1, n, 2, n)             # values of unit vectors: the probabilities themselves
+        p, bound = X.attention(q[b][None, None], k, unit, torch.zeros(1, 1, 4, n, device='cuda'), softcap=softcap)[0]
+        within('weights', w[b, :, :n], p[0, 0].unflatten(0, (2, 2)).sum(1), (bound + 16 * R.E32 * p)[0, 0].unflatten(0, (2, 2)).sum(1))
