@@ -805,8 +805,9 @@ __global__ __launch_bounds__(NT, NT / 256) void attn_masked_dkv_kernel(MaskP p) 
     rq = p.rq + (long)b * ((p.Sq + RG - 1) / RG);
   }
   const int first = p.causal && k0 >= prefix ? max(0, k0 - p.off) / QT : 0;
-  auto whole = [&](int tq) {                                     // every pair of the tile is seen (rows past Sq have probability zero)
+  auto whole = [&](int tq) {                                     // every pair of the tile is seen (a row past Sq is not: 0 of its own meets the keys' infinities)
     const int a = tq * QT;
+    if (a + QT > p.Sq) return false;
     if (p.causal && klast > a + p.off && klast >= prefix) return false;
     if (rq) {
       const int4 x = rq[a / RG];
@@ -849,7 +850,7 @@ __global__ __launch_bounds__(NT, NT / 256) void attn_masked_dkv_kernel(MaskP p) 
       glse = i < p.Sq ? p.lse[at] : __builtin_inff();
       if (glse == NEG_INF) glse = __builtin_inff();              // sees nothing: every probability is zero
       gdel = i < p.Sq ? p.delta[at] : 0.f;
-      gid = p.doc_q ? (i < p.Sq ? p.doc_q[b * p.dcs[0] + i] : -1) : 0;
+      gid = i < p.Sq ? (p.doc_q ? p.doc_q[b * p.dcs[0] + i] : 0) : -1;
     }
   };
   auto put = [&](int buf, int q3, bool full) {

@@ -97,3 +97,23 @@ def test_cap_of_any_size_over_pages(seq, softcap, D):                       # no
         unit = torch.eye(n, device='cuda')[None, :, None].expand(1, n, 2, n)             # values of unit vectors: the probabilities themselves
         p, bound = X.attention(q[b][None, None], k, unit, torch.zeros(1, 1, 4, n, device='cuda'), softcap=softcap)[0]
         within('weights', w[b, :, :n], p[0, 0].unflatten(0, (2, 2)).sum(1), (bound + 16 * R.E32 * p)[0, 0].unflatten(0, (2, 2)).sum(1))
+
+
+# ---- infinities and NaN in places that are seen -------------------------------------------------------------------------------------
+@pytest.mark.parametrize('dtype', DT)
+@pytest.mark.parametrize('Sq,D', [(70, 64), (130, 128), (1, 32), (65, 32)])
+def test_a_key_of_weight_zero_takes_no_gradient(seq, dtype, Sq, D):         # noqa: F811
+    """A seen key whose infinite element makes every score -inf: weight zero, gradients zero, whether or not the queries fill their tiles."""
+    dt, t = DT[dtype], 40
+    q, k, v, do = rand((1, Sq, 2, D), dt, 1), rand((1, 100, 1, D), dt, 2), rand((1, 100, 1, D), dt, 3), rand((1, Sq, 2, D), dt, 4)
+    q[..., 5] = -q[..., 5].abs() - 0.01
+    k[0, t, 0, 5] = float('inf')
+    rest = torch.arange(100, device='cuda') != t
+    out, dq, dk, dv = results(seq, q, k, v, do)
+    ref = X.attention(q, k[:, rest], v[:, rest], do)
+    within('out', out, *ref[0])
+    cols = torch.arange(D, device='cuda') != 5                                 # (dq's own column is 0 * inf)
+    within('dq', dq[..., cols], *(x[..., cols] for x in ref[1]))
+    for name, g, r in (('dk', dk, ref[2]), ('dv', dv, ref[3])):
+        assert not g[:, t].any(), name
+        within(name, g[:, rest], *r)
