@@ -19,8 +19,9 @@
 // largest document id (doc_range_kernel), tested 64 tiles at a time by one ballot.
 //
 // Masked places may hold anything.  A masked score is replaced, never multiplied; where a masked row would enter a product with
-// weight zero (0 * inf is NaN), tiles with a mask are staged with infinities and NaN replaced by zero; if there were any, a second walk
-// over those tiles counts the seen ones (the same product, of 0 / 1 weights and small codes) and adds what they make of the sums.
+// weight zero (0 * inf is NaN), infinities and NaN of a tile with a mask are replaced by zero -- forward as V is staged, backward in shared
+// memory once the tile's scores, which see them, are formed; if there were any, a second walk over those tiles counts the seen ones (the
+// same product, of 0 / 1 weights and small codes) and adds what they make of the sums.
 //
 // Scores, statistics and sums are 32-bit.  p and ds are rounded to the inputs' type for the following product (nearest even: 2^-9 of
 // the value for bf16, 2^-12 for fp16, below which fp16 also loses what is under 6e-8), the sum that divides is not.
@@ -116,13 +117,16 @@ template <class T, int DP, int R, int NT> struct Tile {           // NT threads 
       g.r[i] = row < nrow && d < D && (EVEN || n < R * NCH) ? *(const u32x4*)(x + (long)row * rs + d) : u32x4{0, 0, 0, 0};
     }
   }
-  static __device__ __forceinline__ bool clean(Regs& g) {        // infinities and NaN to zero; whether the wave had any
+  static __device__ __forceinline__ bool nonfinite(const Regs& g) {     // whether the wave has an infinity or a NaN
     bool bad = false;
 #pragma unroll
     for (int i = 0; i < N; ++i)
 #pragma unroll
       for (int w = 0; w < 4; ++w) bad |= word_nonfinite<T>(g.r[i][w]);
-    if (!__any(bad)) return false;
+    return __any(bad);
+  }
+  static __device__ __forceinline__ bool clean(Regs& g) {        // infinities and NaN to zero; whether the wave had any
+    if (!nonfinite(g)) return false;
 #pragma unroll
     for (int i = 0; i < N; ++i)
 #pragma unroll
@@ -152,6 +156,16 @@ template <class T, int DP, int R, int NT> struct Tile {           // NT threads 
     if (n == 0) return 0.f;
     const bool pos = n & 255, neg = n & 0x7f00;
     return n >= 32768 || (pos && neg) ? __builtin_nanf("") : pos ? __builtin_inff() : -__builtin_inff();
+  }
+  // rows 32 n .. of the tile (whole lines): infinities and NaN to zero in place
+  static __device__ __forceinline__ void mend(char* lds, int n) {
+    for (int i = threadIdx.x; i < 32 * ROWB / 16; i += NT) {
+      u32x4* x = (u32x4*)(lds + n * 32 * ROWB) + i;
+      u32x4 v = *x;
+#pragma unroll
+      for (int w = 0; w < 4; ++w) v[w] = word_finite<T>(v[w]);
+      *x = v;
+    }
   }
   static __device__ __forceinline__ void store(char* lds, const Regs& g) {
 #pragma unroll
@@ -251,7 +265,7 @@ template <int N> __device__ __forceinline__ bool any_flag(const int* f) {
   int x = 0;
 #pragma unroll
   for (int i = 0; i < N; ++i) x |= f[i];
-  return x != 0;
+  return __builtin_amdgcn_readfirstlane(x) != 0;
 }
 
 struct Head { int b, h, hk; };
@@ -276,8 +290,10 @@ struct Score {
 template <class T> __device__ __forceinline__ void store_out(const MaskP& p, long at, long row, int e, const f32x4& x) {
   store4((T*)p.out + at + e, x[0], x[1], x[2], x[3]);
   if constexpr (sizeof(T) == 2)
-    if (p.res_out)
-      store4((T*)p.res_out + row * p.D + e, x[0] - (float)(T)x[0], x[1] - (float)(T)x[1], x[2] - (float)(T)x[2], x[3] - (float)(T)x[3]);
+    if (p.res_out) {
+      auto left = [](float y) { return fabsf(y) < __builtin_inff() ? y - (float)(T)y : 0.f; };       // (inf - inf would be NaN)
+      store4((T*)p.res_out + row * p.D + e, left(x[0]), left(x[1]), left(x[2]), left(x[3]));
+    }
 }
 
 // N fragments read and used in groups of A, each group's reads issued before the products of the group ahead of it (pinned reads: left to
@@ -308,8 +324,9 @@ template <class TL, class T, int ND> __device__ __forceinline__ void cols_all(f3
     for (int d = 0; d < ND; ++d) acc[d] = TL::cols(lds, o, n, d, pk, p, acc[d]);
 }
 
-// acc += what the encoded tile's rows that `seen` admits add to each column
-template <class TL, int R, int ND, class F> __device__ __forceinline__ void add_seen(f32x16 (&acc)[ND], const char* lds, F&& seen) {
+// acc += what the encoded tile's rows that `seen` admits add to each column; weighted: by a score gradient, which is 0 or NaN where its own row
+// of q or k is not finite (a score of +-inf has weight 0, NaN, or a cap's derivative of 0), so each gives NaN
+template <class TL, int R, int ND, class F> __device__ __forceinline__ void add_seen(f32x16 (&acc)[ND], const char* lds, F&& seen, bool weighted) {
   const int half = (threadIdx.x & 63) >> 5, cb = TL::col_base();
 #pragma unroll 1
   for (int n = 0; n < R / 32; ++n) {
@@ -326,7 +343,7 @@ template <class TL, int R, int ND, class F> __device__ __forceinline__ void add_
       for (int r = 0; r < 16; ++r) z[r] = 0.f;
       z = TL::cols(lds, cb, n, d, pk, one, z);
 #pragma unroll
-      for (int r = 0; r < 16; ++r) acc[d][r] += TL::decode(z[r]);
+      for (int r = 0; r < 16; ++r) acc[d][r] += weighted && z[r] != 0.f ? __builtin_nanf("") : TL::decode(z[r]);
     }
   }
 }
@@ -505,7 +522,7 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? (DP == 64 ? 3 : 2) : 1) void 
       TL::encode(smem, V, p.vs[1], t * KT, p.Sk, p.D);
       if (threadIdx.x < KT) sid[threadIdx.x] = t * KT + (int)threadIdx.x < p.Sk && p.doc_k ? p.doc_k[hd.b * p.dcs[1] + t * KT + threadIdx.x] : 0;
       __syncthreads();
-      add_seen<TL, KT>(o, smem, [&](int j) { return seen(t * KT + j, sid[j]); });
+      add_seen<TL, KT>(o, smem, [&](int j) { return seen(t * KT + j, sid[j]); }, false);
     }
   }
   l += __shfl_xor(l, 32);
@@ -564,12 +581,12 @@ template <class T, int DP, int KT>
 __global__ __launch_bounds__(256, (sizeof(T) == 2 ? 2 : 1) + (DP == 32)) void attn_masked_dq_kernel(MaskP p) {
   using TL = Tile<T, DP, KT, 256>;
   constexpr int NP = TL::NCH / 2, ND = DP / 32, NS = KT / 32;
-  __shared__ __align__(16) char smem[4 * TL::BYTES + 2 * KT * 4 + 32];
+  __shared__ __align__(16) char smem[4 * TL::BYTES + 2 * KT * 4 + 64];
   const int rb = TL::row_base(), cb = TL::col_base();
   auto sk = [&](int buf) { return buf * TL::BYTES; };          // offsets of the tiles
   auto sv = [&](int buf) { return (2 + buf) * TL::BYTES; };
   int* const sid = (int*)(smem + 4 * TL::BYTES);
-  int* const sbad = sid + 2 * KT;
+  int* const sbad = sid + 2 * KT;                               // [4]; of the two tiles [2][4]
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, half = lane >> 5;
   const Head hd = head_of(blockIdx.x, p);
   const int q0 = (p.causal ? gridDim.y - 1 - blockIdx.y : blockIdx.y) * 128;
@@ -583,28 +600,19 @@ __global__ __launch_bounds__(256, (sizeof(T) == 2 ? 2 : 1) + (DP == 32)) void at
   const long at = ((long)hd.b * p.H + hd.h) * p.Sq + i;
   float delta = 0.f;
   {
-    u32x4 of[NP];
+    u32x4 of[NP], rf[NP];                                        // the output and what its rounding left
     own_row<T, NP>(of, (const T*)p.o + hd.b * p.os[0] + (long)i * p.os[1] + hd.h * p.os[2], iok, p.D);
+    own_row<T, NP>(rf, (const T*)p.res + (((long)hd.b * p.Sq + i) * p.H + hd.h) * p.D, iok && p.res, p.D);
 #pragma unroll
     for (int c = 0; c < NP; ++c)
 #pragma unroll
       for (int w = 0; w < 4; ++w) {
         if constexpr (sizeof(T) == 4) delta += __uint_as_float(of[c][w]) * __uint_as_float(df[c][w]);
-        else {
-          delta += half_to_float<T>((u16)of[c][w]) * half_to_float<T>((u16)df[c][w]);
-          delta += half_to_float<T>((u16)(of[c][w] >> 16)) * half_to_float<T>((u16)(df[c][w] >> 16));
+        else {                                                   // (their sum first: a remainder of 0 times an infinite do is NaN)
+          const unsigned o = of[c][w], x = rf[c][w], y = df[c][w];
+          delta += (half_to_float<T>((u16)o) + half_to_float<T>((u16)x)) * half_to_float<T>((u16)y);
+          delta += (half_to_float<T>((u16)(o >> 16)) + half_to_float<T>((u16)(x >> 16))) * half_to_float<T>((u16)(y >> 16));
         }
-      }
-    if constexpr (sizeof(T) == 2)
-      if (p.res) {                                               // what the output's rounding left
-        own_row<T, NP>(of, (const T*)p.res + (((long)hd.b * p.Sq + i) * p.H + hd.h) * p.D, iok, p.D);
-#pragma unroll
-        for (int c = 0; c < NP; ++c)
-#pragma unroll
-          for (int w = 0; w < 4; ++w) {
-            delta += half_to_float<T>((u16)of[c][w]) * half_to_float<T>((u16)df[c][w]);
-            delta += half_to_float<T>((u16)(of[c][w] >> 16)) * half_to_float<T>((u16)(df[c][w] >> 16));
-          }
       }
     delta += __shfl_xor(delta, 32);
   }
@@ -652,7 +660,11 @@ __global__ __launch_bounds__(256, (sizeof(T) == 2 ? 2 : 1) + (DP == 32)) void at
     if (p.doc_k && threadIdx.x < KT) gid = t * KT + (int)threadIdx.x < p.Sk ? p.doc_k[hd.b * p.dcs[1] + t * KT + threadIdx.x] : -1;
   };
   auto put = [&](int buf, bool full) {
-    if (!full) dirty |= TL::clean(gk);
+    if (!full) {
+      const bool bad = TL::nonfinite(gk);
+      dirty |= bad;
+      if (lane == 0) sbad[4 + 4 * buf + wave] = bad;
+    }
     TL::store(smem + sk(buf), gk);
     TL::store(smem + sv(buf), gv);
     if (threadIdx.x < KT) sid[buf * KT + threadIdx.x] = gid;
@@ -672,6 +684,7 @@ __global__ __launch_bounds__(256, (sizeof(T) == 2 ? 2 : 1) + (DP == 32)) void at
     const int tn = it.next();
     const bool fulln = tn >= 0 && whole(tn);
     if (tn >= 0) fetch(tn);
+    const bool holes = !full && any_flag<4>(sbad + 4 + 4 * buf);   // scores from the tile as it is, the product without its infinities
 #pragma unroll
     for (int n = 0; n < NS; ++n) {
       f32x16 st[1], dp;
@@ -684,6 +697,11 @@ __global__ __launch_bounds__(256, (sizeof(T) == 2 ? 2 : 1) + (DP == 32)) void at
 #pragma unroll
       for (int c = 0; c < NP; ++c) dp = mfma32<T>(TL::rows(smem, sv(buf) + rb, n, c), df[c], dp);
       __builtin_amdgcn_s_setprio(0);
+      if (holes) {                                               // (the whole workgroup; S is formed, K is next read for its columns)
+        __syncthreads();
+        TL::mend(smem + sk(buf), n);
+        __syncthreads();
+      }
 #pragma unroll
       for (int r = 0; r < 16; ++r) dp[r] -= delta;
       float m0 = sc.mul;
@@ -738,7 +756,7 @@ __global__ __launch_bounds__(256, (sizeof(T) == 2 ? 2 : 1) + (DP == 32)) void at
       TL::encode(smem, K, p.ks[1], t * KT, p.Sk, p.D);
       if (threadIdx.x < KT) sid[threadIdx.x] = t * KT + (int)threadIdx.x < p.Sk && p.doc_k ? p.doc_k[hd.b * p.dcs[1] + t * KT + threadIdx.x] : 0;
       __syncthreads();
-      add_seen<TL, KT>(dq, smem, [&](int j) { return seen(t * KT + j, sid[j]); });
+      add_seen<TL, KT>(dq, smem, [&](int j) { return seen(t * KT + j, sid[j]); }, true);
     }
   }
   if (!iok) return;
@@ -769,14 +787,14 @@ __global__ __launch_bounds__(NT, NT / 256) void attn_masked_dkv_kernel(MaskP p) 
   constexpr int NW = NT / 128, KEYS = 32 * NW;                  // waves of either kind; keys of the workgroup
   constexpr int NP = TL::NCH / 2, ND = DP / 32, NS = QT / 32;
   constexpr int XB = NW * NS * 4096;                            // probabilities of a tile: [pair][half tile][4][lane][4] floats
-  __shared__ __align__(16) char smem[5 * TL::BYTES + 2 * XB + 6 * QT * 4 + 64];   // dO of two tiles, Q of three; probabilities; lse, delta, ids; flags
+  __shared__ __align__(16) char smem[5 * TL::BYTES + 2 * XB + 6 * QT * 4 + 128];   // dO of two tiles, Q of three; probabilities; lse, delta, ids; flags
   const int rb = TL::row_base(), cb = TL::col_base();
   auto sd = [&](int buf) { return buf * TL::BYTES; };          // offsets of the tiles
   auto sq = [&](int q3) { return (2 + q3) * TL::BYTES; };
   float* const slse = (float*)(smem + 5 * TL::BYTES + 2 * XB);  // [2][QT]
   float* const sdel = slse + 2 * QT;
   int* const sid = (int*)(sdel + 2 * QT);
-  int* const sbad = sid + 2 * QT;                               // [8]
+  int* const sbad = sid + 2 * QT;                               // [8]; of the three tiles [3][8]
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, half = lane >> 5;
   const bool keys = wave >= NW;                                 // this wave forms dk, else dv
   const int b = blockIdx.x / p.Hk, hk = blockIdx.x - b * p.Hk, split = blockIdx.z;
@@ -855,8 +873,9 @@ __global__ __launch_bounds__(NT, NT / 256) void attn_masked_dkv_kernel(MaskP p) 
   };
   auto put = [&](int buf, int q3, bool full) {
     if (!full) {
-      dirty |= TL::clean(gq);
-      dirty |= TL::clean(gd);
+      const bool badq = TL::nonfinite(gq), badd = TL::nonfinite(gd);
+      dirty |= badq || badd;
+      if (lane == 0) sbad[8 + 8 * q3 + wave] = badq || badd;
     }
     TL::store(smem + sq(q3), gq);
     TL::store(smem + sd(buf), gd);
@@ -867,12 +886,13 @@ __global__ __launch_bounds__(NT, NT / 256) void attn_masked_dkv_kernel(MaskP p) 
     }
   };
   start();
-  int tq = next(), gcur = g, buf = 0, q3 = 0, qprev = 0;
+  int tq = next(), gcur = g, buf = 0, q3 = 0, qprev = 2;
   bool full = tq >= 0 && whole(tq);
   if (tq >= 0) {
     fetch(tq, gcur);
     put(0, 0, full);
   }
+  for (int i = threadIdx.x; i < TL::BYTES / 16; i += NT) ((u32x4*)(smem + sq(2)))[i] = u32x4{0, 0, 0, 0};
   __syncthreads();
   auto walk = [&](auto role) {                                 // (a loop of its own for either kind of wave: same tiles, same barriers)
     f32x16 dp[NS];                                               // dk's waves: do.v - D of the tile, until its probabilities are there
@@ -884,7 +904,8 @@ __global__ __launch_bounds__(NT, NT / 256) void attn_masked_dkv_kernel(MaskP p) 
         for (int r4 = 0; r4 < 4; ++r4) {
           const f32x4 pr = x[64 * r4];
 #pragma unroll
-          for (int w = 0; w < 4; ++w) dp[n][4 * r4 + w] = pr[w] == 0.f ? 0.f : pr[w] * dp[n][4 * r4 + w];     // (a masked pair's do.v may be anything)
+          for (int w = 0; w < 4; ++w)                            // (-0: a masked pair, whose do.v may be anything)
+            dp[n][4 * r4 + w] = __float_as_uint(pr[w]) == 0x80000000u ? 0.f : pr[w] * dp[n][4 * r4 + w];
         }
         u32x4 pk[2];
         pack_tile<T>(dp[n], pk);
@@ -893,7 +914,13 @@ __global__ __launch_bounds__(NT, NT / 256) void attn_masked_dkv_kernel(MaskP p) 
         __builtin_amdgcn_s_setprio(0);
       }
     };
-    if constexpr (decltype(role)::value) {                     // nothing before the first tile: probabilities of zero
+    auto mend = [&](int n) {                                     // both kinds of wave: S and do.v of these rows are formed, next come their columns
+      __syncthreads();
+      TL::mend(smem + sq(q3), n);
+      TL::mend(smem + sd(buf), n);
+      __syncthreads();
+    };
+    if constexpr (decltype(role)::value) {                     // nothing before the first tile: probabilities of zero, rows of zero
 #pragma unroll
       for (int n = 0; n < NS; ++n)
 #pragma unroll
@@ -910,6 +937,7 @@ __global__ __launch_bounds__(NT, NT / 256) void attn_masked_dkv_kernel(MaskP p) 
       const int tn = next(), gn = g;
       const bool fulln = tn >= 0 && whole(tn);
       if (tn >= 0) fetch(tn, gn);
+      const bool holes = !full && any_flag<NT / 64>(sbad + 8 + 8 * q3);   // scores from the tiles as they are, the products without their infinities
       if constexpr (decltype(role)::value) {
 #pragma unroll
         for (int n = 0; n < NS; ++n) {
@@ -918,6 +946,7 @@ __global__ __launch_bounds__(NT, NT / 256) void attn_masked_dkv_kernel(MaskP p) 
           __builtin_amdgcn_s_setprio(1);
           in_groups<NP, AHEAD>([&](int i) { return TL::template rows<true>(smem, sd(buf) + rb, n, i); }, [&](int i, const u32x4& a) { dp[n] = mfma32<T>(a, wf[i], dp[n]); });
           __builtin_amdgcn_s_setprio(0);
+          if (holes) mend(n);
 #pragma unroll
           for (int r4 = 0; r4 < 4; ++r4) {
             const f32x4 de = *(const f32x4*)(sdel + buf * QT + n * 32 + 8 * r4 + 4 * half);
@@ -935,6 +964,7 @@ __global__ __launch_bounds__(NT, NT / 256) void attn_masked_dkv_kernel(MaskP p) 
           __builtin_amdgcn_s_setprio(1);
           in_groups<NP, AHEAD>([&](int i) { return TL::template rows<true>(smem, sq(q3) + rb, n, i); }, [&](int i, const u32x4& a) { s = mfma32<T>(a, wf[i], s); });
           __builtin_amdgcn_s_setprio(0);
+          if (holes) mend(n);
           float m0 = sc.mul;
           if (sc.capped) {
             m0 = 1.f;
@@ -959,7 +989,7 @@ __global__ __launch_bounds__(NT, NT / 256) void attn_masked_dkv_kernel(MaskP p) 
               const i32x4 id = *(const i32x4*)(sid + buf * QT + j0);
 #pragma unroll
               for (int w = 0; w < 4; ++w)
-                if (j0 + w < lim - tq * QT || id[w] != myid) { s[4 * r4 + w] = 0.f; dcap[4 * r4 + w] = 0.f; }   // (either may be NaN there)
+                if (j0 + w < lim - tq * QT || id[w] != myid) { s[4 * r4 + w] = -0.f; dcap[4 * r4 + w] = 1.f; }   // (either may be NaN there)
             }
           }
           f32x4* x = exchange(buf, n);
@@ -1005,7 +1035,7 @@ __global__ __launch_bounds__(NT, NT / 256) void attn_masked_dkv_kernel(MaskP p) 
         TL::encode(smem + sd(0), (const T*)p.d_o + b * p.dos[0] + h * p.dos[2], p.dos[1], tq * QT, p.Sq, p.D);
         if (threadIdx.x < QT) sid[threadIdx.x] = tq * QT + (int)threadIdx.x < p.Sq && p.doc_q ? p.doc_q[b * p.dcs[0] + tq * QT + threadIdx.x] : 0;
         __syncthreads();
-        add_seen<TL, QT>(acc, smem + (keys ? sq(0) : sd(0)), [&](int j) { return seen(tq * QT + j, sid[j]); });
+        add_seen<TL, QT>(acc, smem + (keys ? sq(0) : sd(0)), [&](int j) { return seen(tq * QT + j, sid[j]); }, keys);
       }
     }
   }

@@ -117,3 +117,43 @@ def test_a_key_of_weight_zero_takes_no_gradient(seq, dtype, Sq, D):         # no
     for name, g, r in (('dk', dk, ref[2]), ('dv', dv, ref[3])):
         assert not g[:, t].any(), name
         within(name, g[:, rest], *r)
+
+
+def same_kind(name, got, want, bound):
+    """NaN and infinities at the same places, finite values within their bound."""
+    assert torch.equal(torch.isnan(got), torch.isnan(want)), '%s: NaN at %d places for %d' % (name, int(torch.isnan(got).sum()), int(torch.isnan(want).sum()))
+    inf = torch.isinf(want)
+    assert torch.equal(torch.isinf(got), inf) and torch.equal(got.double()[inf], want[inf]), '%s: infinities' % name
+    ok = torch.isfinite(want)
+    within(name, got[ok], want[ok], bound[ok])
+
+
+@pytest.mark.parametrize('dtype', DT)
+@pytest.mark.parametrize('fill', [float('nan'), float('inf'), -float('inf')])
+@pytest.mark.parametrize('which', ['q', 'k', 'v', 'do'])
+@pytest.mark.parametrize('softcap', [0.0, 5.0])
+@pytest.mark.parametrize('causal,D', [(True, 64), (True, 128), (False, 32)])
+def test_seen_infinities_and_nan_in_the_gradients(seq, dtype, fill, which, softcap, causal, D):      # noqa: F811
+    """One non-finite element that some queries see: the same results as the definition's, in a tile with a mask and in one without.  (Scores of
+    order 1, so no probability that counts is too small for 32 bits.)"""
+    dt = DT[dtype]
+    for place in (3, 75, 139):                                             # whole tiles above it; inside a masked one; the last row of all
+        x = dict(q=rand((1, 140, 2, D), dt, 1, 0.7), k=rand((1, 140, 1, D), dt, 2, 0.7), v=rand((1, 140, 1, D), dt, 3), do=rand((1, 140, 2, D), dt, 4))
+        x[which][0, place, 0, 6] = fill
+        got = results(seq, x['q'], x['k'], x['v'], x['do'], causal=causal, softcap=softcap)
+        for name, g, (want, bound) in zip(('out', 'dq', 'dk', 'dv'), got, X.attention(x['q'], x['k'], x['v'], x['do'], causal=causal, softcap=softcap)):
+            same_kind('%s, %s at %d' % (name, which, place), g, want, bound)
+
+
+@pytest.mark.parametrize('dtype', DT)
+def test_seen_infinities_within_documents(seq, dtype):                      # noqa: F811
+    dt, D = DT[dtype], 64
+    ids = docs_of(1, 200, 4, 5, 13)
+    for which in range(4):
+        x = [rand((1, 200, 2, D), dt, 1, 0.7), rand((1, 200, 2, D), dt, 2, 0.7), rand((1, 200, 2, D), dt, 3), rand((1, 200, 2, D), dt, 4)]
+        x[which][0, 100, 1, 9] = float('inf')
+        for t in x:
+            t[0, 190] = float('nan')                                        # padding
+        got = results(seq, *x, causal=True, softcap=4.0, doc_q=ids, doc_k=ids)
+        for name, g, (want, bound) in zip(('out', 'dq', 'dk', 'dv'), got, X.attention(*x, causal=True, softcap=4.0, doc_q=ids, doc_k=ids)):
+            same_kind('%s of %d' % (name, which), g, want, bound)
