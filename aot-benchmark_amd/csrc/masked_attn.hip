@@ -24,7 +24,8 @@
 // same product, of 0 / 1 weights and small codes) and adds what they make of the sums.
 //
 // Scores, statistics and sums are 32-bit.  p and ds are rounded to the inputs' type for the following product (nearest even: 2^-9 of
-// the value for bf16, 2^-12 for fp16, below which fp16 also loses what is under 6e-8), the sum that divides is not.
+// the value for bf16, 2^-12 for fp16), the sum that divides is not.  fp16 ends at 6e-8, so there p is held 2^15 times as large and ds by the
+// power of two that its column's largest so far allows: what is lost is 2^-39 of the largest.
 #include "seq_common.h"
 
 static constexpr int AHEAD = 4;                               // fragments of a group that is read ahead of its products
@@ -489,7 +490,7 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? (DP == 64 ? 3 : 2) : 1) void 
       for (int r = 0; r < 16; ++r) mx = fmaxf(mx, s[n][r]);
     mx = fmaxf(mx, __shfl_xor(mx, 32)) * m0;
     const float m2 = fmaxf(m, mx), base = m2 == NEG_INF ? 0.f : m2;
-    const float f = exp2_hw(m - base);
+    const float f = exp2_hw(m - base), low = base - LIFT<T>;
     m = m2;
     l *= f;
     if (__any(f != 1.f))
@@ -498,7 +499,7 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? (DP == 64 ? 3 : 2) : 1) void 
 #pragma unroll
     for (int n = 0; n < NS; ++n) {
 #pragma unroll
-      for (int r = 0; r < 16; ++r) { s[n][r] = exp2_hw(__builtin_fmaf(s[n][r], m0, -base)); l += s[n][r]; }
+      for (int r = 0; r < 16; ++r) { s[n][r] = exp2_hw(__builtin_fmaf(s[n][r], m0, -low)); l += s[n][r]; }
       u32x4 pk[2];
       pack_tile<T>(s[n], pk);
       __builtin_amdgcn_s_setprio(1);
@@ -550,7 +551,7 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? (DP == 64 ? 3 : 2) : 1) void 
       const int e = d * 32 + mfma32_row(r, half);
       if (e < p.D) store_out<T>(p, at, row, e, f32x4{o[d][r] * inv, o[d][r + 1] * inv, o[d][r + 2] * inv, o[d][r + 3] * inv});
     }
-  if (half == 0) p.lse[((long)hd.b * p.H + hd.h) * p.Sq + i] = l == 0.f ? NEG_INF : m + log2f(l);
+  if (half == 0) p.lse[((long)hd.b * p.H + hd.h) * p.Sq + i] = l == 0.f ? NEG_INF : m + (log2f(l) - LIFT<T>);
 }
 
 // Split keys joined: four elements of a row a thread, the splits in order
@@ -573,7 +574,24 @@ __global__ __launch_bounds__(256) void attn_masked_join_kernel(MaskP p) {
   const float inv = l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l);
   const long bi = row / p.H, h = row - bi * p.H, b = bi / p.Sq, i = bi - b * p.Sq;
   store_out<T>(p, b * p.os[0] + i * p.os[1] + h * p.os[2], row, d, a * inv);
-  if (d == 0) p.lse[(b * p.H + h) * p.Sq + i] = l == 0.f ? NEG_INF : m + log2f(l);
+  if (d == 0) p.lse[(b * p.H + h) * p.Sq + i] = l == 0.f ? NEG_INF : m + (log2f(l) - LIFT<T>);
+}
+
+// The largest magnitude (NaN aside) of a lane's half of its column of a score tile, and the power of two, at most `up`, by which it comes to lie in
+// [2^14, 2^15); an infinity: so low that nothing finite beside it overflows
+static constexpr int TOP = 60;
+__device__ __forceinline__ float column_max(const f32x16& s) {
+  float a = 0.f;
+#pragma unroll
+  for (int r = 0; r < 16; ++r) a = fmaxf(a, fabsf(s[r]));
+  return a;
+}
+// x = the magnitude times 2^up.  By the whole wave, so that both halves of a column agree (an exchange for every tile would cost more than this
+// does where it is rare: in a column's first tiles)
+__device__ __forceinline__ int fitting(float x, int up) {
+  x = fmaxf(x, __shfl_xor(x, 32));
+  if (x <= 32768.f) return up;
+  return x < __builtin_inff() ? min(up, up + 15 - __builtin_amdgcn_frexp_expf(x)) : min(up, -TOP);
 }
 
 // ---- gradient of the queries -----------------------------------------------------------------------------------------------------
@@ -669,6 +687,12 @@ __global__ __launch_bounds__(256, (sizeof(T) == 2 ? 2 : 1) + (DP == 32)) void at
     TL::store(smem + sv(buf), gv);
     if (threadIdx.x < KT) sid[buf * KT + threadIdx.x] = gid;
   };
+  // fp16: score gradients are small multiples of 1 / Sk of dout's and would be subnormal or lost; each query's are held 2^up times as large,
+  // up such that its largest so far lies below 2^15 (lowered, with the sums, when a larger one comes; part of the exponent otherwise).  With
+  // dout of 1e-3 at 4096 keys dq was off by 5e-3 of itself, eight times its own rounding.  2 x 4096 x 16 x 64: 254 -> 300 us, dk 507 -> 550.
+  constexpr bool LIFTED = std::is_same<T, f16>::value;
+  int up = LIFTED ? TOP : 0;
+  if constexpr (LIFTED) lse -= (float)up;
   f32x16 dq[ND];
 #pragma unroll
   for (int d = 0; d < ND; ++d)
@@ -697,11 +721,6 @@ __global__ __launch_bounds__(256, (sizeof(T) == 2 ? 2 : 1) + (DP == 32)) void at
 #pragma unroll
       for (int c = 0; c < NP; ++c) dp = mfma32<T>(TL::rows(smem, sv(buf) + rb, n, c), df[c], dp);
       __builtin_amdgcn_s_setprio(0);
-      if (holes) {                                               // (the whole workgroup; S is formed, K is next read for its columns)
-        __syncthreads();
-        TL::mend(smem + sk(buf), n);
-        __syncthreads();
-      }
 #pragma unroll
       for (int r = 0; r < 16; ++r) dp[r] -= delta;
       float m0 = sc.mul;
@@ -731,6 +750,24 @@ __global__ __launch_bounds__(256, (sizeof(T) == 2 ? 2 : 1) + (DP == 32)) void at
               if (id[w] != myid) s[4 * r4 + w] = 0.f;
           }
         }
+      }
+      if constexpr (LIFTED) {
+        const float mx = column_max(s);
+        if (__any(mx > 32768.f)) {
+          const int drop = up - fitting(mx, up);
+          const float f = __builtin_amdgcn_ldexpf(1.f, -drop);
+          up -= drop;
+          lse += (float)drop;
+#pragma unroll
+          for (int r = 0; r < 16; ++r) s[r] *= f;
+#pragma unroll
+          for (int d = 0; d < ND; ++d) dq[d] *= f;
+        }
+      }
+      if (holes) {                                               // (the whole workgroup; S is formed, K is next read for its columns)
+        __syncthreads();
+        TL::mend(smem + sk(buf), n);
+        __syncthreads();
       }
       u32x4 pk[2];
       pack_tile<T>(s, pk);
@@ -762,14 +799,16 @@ __global__ __launch_bounds__(256, (sizeof(T) == 2 ? 2 : 1) + (DP == 32)) void at
   if (!iok) return;
   T* out = (T*)p.dq + hd.b * p.dqs[0] + (long)i * p.dqs[1] + hd.h * p.dqs[2];
   float* part = p.qpart + (((long)blockIdx.z * p.B + hd.b) * p.Sq + i) * p.H * p.D + (long)hd.h * p.D;
+  const float mul = __builtin_amdgcn_ldexpf(p.qsplit == 1 ? p.scale : 1.f, -up);
 #pragma unroll
   for (int d = 0; d < ND; ++d)
 #pragma unroll
     for (int r = 0; r < 16; r += 4) {
       const int e = d * 32 + mfma32_row(r, half);
       if (e >= p.D) continue;
-      if (p.qsplit == 1) store4(out + e, dq[d][r] * p.scale, dq[d][r + 1] * p.scale, dq[d][r + 2] * p.scale, dq[d][r + 3] * p.scale);
-      else *(f32x4*)(part + e) = f32x4{dq[d][r], dq[d][r + 1], dq[d][r + 2], dq[d][r + 3]};
+      const f32x4 x{dq[d][r] * mul, dq[d][r + 1] * mul, dq[d][r + 2] * mul, dq[d][r + 3] * mul};
+      if (p.qsplit == 1) store4(out + e, x[0], x[1], x[2], x[3]);
+      else *(f32x4*)(part + e) = x;
     }
 }
 
@@ -867,6 +906,7 @@ __global__ __launch_bounds__(NT, NT / 256) void attn_masked_dkv_kernel(MaskP p) 
       const long at = ((long)b * p.H + h) * p.Sq + i;
       glse = i < p.Sq ? p.lse[at] : __builtin_inff();
       if (glse == NEG_INF) glse = __builtin_inff();              // sees nothing: every probability is zero
+      glse -= LIFT<T>;
       gdel = i < p.Sq ? p.delta[at] : 0.f;
       gid = i < p.Sq ? (p.doc_q ? p.doc_q[b * p.dcs[0] + i] : 0) : -1;
     }
@@ -894,6 +934,8 @@ __global__ __launch_bounds__(NT, NT / 256) void attn_masked_dkv_kernel(MaskP p) 
   }
   for (int i = threadIdx.x; i < TL::BYTES / 16; i += NT) ((u32x4*)(smem + sq(2)))[i] = u32x4{0, 0, 0, 0};
   __syncthreads();
+  constexpr bool LIFTED = std::is_same<T, f16>::value;
+  int up = LIFTED && keys ? TOP : 0;                            // fp16: dk's score gradients are held 2^up times as large
   auto walk = [&](auto role) {                                 // (a loop of its own for either kind of wave: same tiles, same barriers)
     f32x16 dp[NS];                                               // dk's waves: do.v - D of the tile, until its probabilities are there
     auto finish = [&]() {                                        // dk of the tile before: its probabilities, its rows of Q
@@ -906,6 +948,19 @@ __global__ __launch_bounds__(NT, NT / 256) void attn_masked_dkv_kernel(MaskP p) 
 #pragma unroll
           for (int w = 0; w < 4; ++w)                            // (-0: a masked pair, whose do.v may be anything)
             dp[n][4 * r4 + w] = __float_as_uint(pr[w]) == 0x80000000u ? 0.f : pr[w] * dp[n][4 * r4 + w];
+        }
+        if constexpr (LIFTED) {                                  // as in the queries' kernel, a key's column here
+          const float mx = column_max(dp[n]), top = __builtin_amdgcn_ldexpf(mx, up);
+          if (__any(top > 32768.f)) {
+            const int to = fitting(top, up);
+            const float f = __builtin_amdgcn_ldexpf(1.f, to - up);
+            up = to;
+#pragma unroll
+            for (int d = 0; d < ND; ++d) acc[d] *= f;
+          }
+          const float f = __builtin_amdgcn_ldexpf(1.f, up);
+#pragma unroll
+          for (int r = 0; r < 16; ++r) dp[n][r] *= f;
         }
         u32x4 pk[2];
         pack_tile<T>(dp[n], pk);
@@ -946,13 +1001,13 @@ __global__ __launch_bounds__(NT, NT / 256) void attn_masked_dkv_kernel(MaskP p) 
           __builtin_amdgcn_s_setprio(1);
           in_groups<NP, AHEAD>([&](int i) { return TL::template rows<true>(smem, sd(buf) + rb, n, i); }, [&](int i, const u32x4& a) { dp[n] = mfma32<T>(a, wf[i], dp[n]); });
           __builtin_amdgcn_s_setprio(0);
-          if (holes) mend(n);
 #pragma unroll
           for (int r4 = 0; r4 < 4; ++r4) {
             const f32x4 de = *(const f32x4*)(sdel + buf * QT + n * 32 + 8 * r4 + 4 * half);
 #pragma unroll
             for (int w = 0; w < 4; ++w) dp[n][4 * r4 + w] -= de[w];
           }
+          if (holes) mend(n);
         }
       } else {
 #pragma unroll
@@ -964,7 +1019,6 @@ __global__ __launch_bounds__(NT, NT / 256) void attn_masked_dkv_kernel(MaskP p) 
           __builtin_amdgcn_s_setprio(1);
           in_groups<NP, AHEAD>([&](int i) { return TL::template rows<true>(smem, sq(q3) + rb, n, i); }, [&](int i, const u32x4& a) { s = mfma32<T>(a, wf[i], s); });
           __builtin_amdgcn_s_setprio(0);
-          if (holes) mend(n);
           float m0 = sc.mul;
           if (sc.capped) {
             m0 = 1.f;
@@ -1002,6 +1056,7 @@ __global__ __launch_bounds__(NT, NT / 256) void attn_masked_dkv_kernel(MaskP p) 
             for (int r4 = 0; r4 < 4; ++r4) x[64 * r4] = f32x4{s[4 * r4], s[4 * r4 + 1], s[4 * r4 + 2], s[4 * r4 + 3]};
           u32x4 pk[2];
           pack_tile<T>(s, pk);
+          if (holes) mend(n);
           __builtin_amdgcn_s_setprio(1);
           cols_all<TL, T>(acc, smem, sd(buf) + cb, n, pk, s);
           __builtin_amdgcn_s_setprio(0);
@@ -1040,7 +1095,7 @@ __global__ __launch_bounds__(NT, NT / 256) void attn_masked_dkv_kernel(MaskP p) 
     }
   }
   if (!tok) return;
-  const float mul = keys ? p.scale : 1.f;
+  const float mul = __builtin_amdgcn_ldexpf(keys && p.nsplit == 1 ? p.scale : 1.f, -up) * LOWER<T>;
   const long* st = keys ? p.dks : p.dvs;
   T* out = (T*)(keys ? p.dk : p.dv) + b * st[0] + (long)t * st[1] + hk * st[2];
   float* part = p.part + ((((long)split * 2 + keys) * p.B + b) * p.Sk + t) * p.Hk * p.D + (long)hk * p.D;
@@ -1050,8 +1105,9 @@ __global__ __launch_bounds__(NT, NT / 256) void attn_masked_dkv_kernel(MaskP p) 
     for (int r = 0; r < 16; r += 4) {
       const int e = d * 32 + mfma32_row(r, half);
       if (e >= p.D) continue;
-      if (p.nsplit == 1) store4(out + e, acc[d][r] * mul, acc[d][r + 1] * mul, acc[d][r + 2] * mul, acc[d][r + 3] * mul);
-      else *(f32x4*)(part + e) = f32x4{acc[d][r], acc[d][r + 1], acc[d][r + 2], acc[d][r + 3]};
+      const f32x4 x{acc[d][r] * mul, acc[d][r + 1] * mul, acc[d][r + 2] * mul, acc[d][r + 3] * mul};
+      if (p.nsplit == 1) store4(out + e, x[0], x[1], x[2], x[3]);
+      else *(f32x4*)(part + e) = x;
     }
 }
 

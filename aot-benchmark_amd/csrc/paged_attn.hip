@@ -16,7 +16,8 @@
 // paged_join_kernel adds up in index order (no atomics: results repeat bit for bit).  Collected weights need the final maximum and
 // sum, so the scores (4 bytes a head and entry, 1/64 of the cache's bytes at D = 128 and 16 bits) are left in the workspace too.
 // Scores, probabilities, sums and outputs are 32-bit; a probability is rounded to the cache's type on its way into the P.V product
-// (at most 2^-9 of itself for bf16, unbiased), while the sum that divides uses the unrounded ones.
+// (at most 2^-9 of itself for bf16, unbiased; fp16's are held 2^15 times as large meanwhile), while the sum that divides uses the
+// unrounded ones.
 #include "seq_common.h"
 
 struct PagedP {
@@ -188,11 +189,11 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? (DP == 128 ? 3 : DP == 256 ? 
     mx = fmaxf(mx, __shfl_xor(mx, 16));
     mx = fmaxf(mx, __shfl_xor(mx, 32));
     const float m2 = fmaxf(m, mx), base = m2 == NEG_INF ? 0.f : m2;      // nothing seen yet: exp2(-inf - 0) = 0 everywhere
-    const float f = exp2_hw(m - base);
+    const float f = exp2_hw(m - base), low = base - LIFT<T>;
     m = m2;
     float pr[8], add = 0.f;
 #pragma unroll
-    for (int j = 0; j < 8; ++j) { pr[j] = exp2_hw(x[j] - base); add += pr[j]; }
+    for (int j = 0; j < 8; ++j) { pr[j] = exp2_hw(x[j] - low); add += pr[j]; }
     l = l * f + add;
 #pragma unroll
     for (int e = 0; e < E; ++e) o[e] *= f;
@@ -343,7 +344,7 @@ __global__ __launch_bounds__(256) void paged_join_kernel(PagedP p) {
       for (int i = lane; i < ns; i += 64) l += ml[2 * i + 1] * exp2_hw(ml[2 * i] - mb);
 #pragma unroll
       for (int d = 1; d < 64; d <<= 1) l += __shfl_xor(l, d);
-      if (lane == 0) { red[wave] = mb; red[4 + wave] = live_sum(l); }
+      if (lane == 0) { red[wave] = mb - LIFT<T>; red[4 + wave] = live_sum(l); }      // (the sums are of lifted probabilities)
     }
     __syncthreads();
     for (int i = 0; i < n; ++i) {

@@ -19,6 +19,11 @@ template <> struct Elem<float> { static constexpr int CE = 4; };        // eleme
 template <> struct Elem<f16> { static constexpr int CE = 8; };
 template <> struct Elem<bf16> { static constexpr int CE = 8; };
 
+// fp16 ends at 6e-8, above the share of a key in a long row: its probabilities are held 2^15 times as large (at most 2^15 of 65504) while they
+// are rounded for a product, in the exponent they are formed with, so that none above 2^-39 of the largest is lost.
+template <class T> static constexpr float LIFT = std::is_same<T, f16>::value ? 15.f : 0.f;
+template <class T> static constexpr float LOWER = std::is_same<T, f16>::value ? 0x1p-15f : 1.f;
+
 __device__ __forceinline__ float exp2_hw(float x) { return __builtin_amdgcn_exp2f(x); }
 __device__ __forceinline__ float rcp_hw(float x) { return __builtin_amdgcn_rcpf(x); }
 

@@ -554,7 +554,8 @@ int aot_attn_masked(const void* q, const void* k, const void* v, void* out, void
  * that share them); residual as written by the forward call, or NULL
  * (do.o is then formed from the rounded output: for 16-bit types its error adds about a third to dq's and dk's); work: scratch of
  * aot_attn_masked_floats(.., 1, ..) floats, 16-byte aligned.  Probabilities and score gradients are rounded to `dtype` for the products they
- * enter (fp16: what is below 6e-8 is lost, as in any fp16 gradient -- scale the loss).  No atomics: results repeat bit for bit.
+ * enter; in fp16 they are held larger there by powers of two, so that only what is below 2^-39 of a row's largest is lost -- the gradients
+ * themselves are fp16 numbers, which end at 6e-8.  No atomics: results repeat bit for bit.
  * strides: q k v out dout dq dk dv (b s h each), doc_q b, doc_k b (26). */
 int aot_attn_masked_bwd(const void* q, const void* k, const void* v, const void* out, const void* residual, const float* lse,
                         const void* dout, void* dq, void* dk, void* dv, const float* slopes, const int* doc_q, const int* doc_k, const int* prefix, void* ranges, float* work, long work_floats,

@@ -69,7 +69,7 @@ def test_cap_of_any_size(seq, softcap, D, H, K, causal):                   # noq
             within(name, g, want, 2 * bound)
 
 
-@pytest.mark.parametrize('dtype', ['f32', 'bf16'])
+@pytest.mark.parametrize('dtype', DT)
 def test_gradients_of_scores_near_the_cap(seq, dtype):                      # noqa: F811
     """Every score three to eight times the cap: the cap's derivative is 1e-2 to 1e-6 and keeps its relative accuracy, on both sides of zero."""
     dt = DT[dtype]
@@ -157,3 +157,78 @@ def test_seen_infinities_within_documents(seq, dtype):                      # no
         got = results(seq, *x, causal=True, softcap=4.0, doc_q=ids, doc_k=ids)
         for name, g, (want, bound) in zip(('out', 'dq', 'dk', 'dv'), got, X.attention(*x, causal=True, softcap=4.0, doc_q=ids, doc_k=ids)):
             same_kind('%s of %d' % (name, which), g, want, bound)
+
+
+# ---- fp16: small gradients, small probabilities ---------------------------------------------------------------------------------------
+def rounded_once(got, want, bound, name):
+    """Elementwise within the bound, which an answer of zeros is not; and over all not twice as far off as the definition rounded once (the
+    score gradient's or the probability's own rounding adds an independent error of the same relative size: 1.4)."""
+    within(name, got, want, bound)
+    assert float((want.abs() > bound).double().mean()) > 0.5, name + ': the bound is too wide to say anything'
+    once = (want.half().double() - want).norm()
+    assert float((got.double() - want).norm()) <= 2 * float(once), name
+
+
+@pytest.mark.parametrize('size', [1.0, 1e-3, 1e-4])
+@pytest.mark.parametrize('Sq,Sk,H,K,D,o', [(256, 4096, 2, 1, 64, {}), (300, 2500, 2, 2, 128, dict(causal=True)), (200, 3000, 2, 2, 32, dict(softcap=5.0)),
+                                           (512, 6000, 4, 2, 64, dict(causal=True))])
+def test_small_gradients_in_fp16(seq, size, Sq, Sk, H, K, D, o):            # noqa: F811
+    dt = torch.float16
+    q, k, v, do = rand((1, Sq, H, D), dt, 1), rand((1, Sk, K, D), dt, 2), rand((1, Sk, K, D), dt, 3), rand((1, Sq, H, D), dt, 4, size)
+    got = results(seq, q, k, v, do, **o)
+    ref = X.attention(q, k, v, do, **o)
+    within('out', got[0], *ref[0])
+    for name, g, (want, bound) in zip(('dq', 'dk', 'dv'), got[1:], ref[1:]):
+        rounded_once(g, want, bound, name)
+
+
+def test_gradients_of_rows_far_apart_in_fp16(seq):                          # noqa: F811
+    """Documents whose gradients differ by 1e6, and rows of one document by 1e3: every row of dq and every document's dk keeps its digits."""
+    dt, S = torch.float16, 700
+    ids = docs_of(1, S, 3, 5)
+    q, k, v = (rand((1, S, 2, 64), dt, i) for i in range(3))
+    size = torch.where(ids[0] == 1, 1e-4, 100.0) * torch.where(torch.arange(S, device='cuda') % 3 == 0, 1.0, 1e-3 ** 0.5)
+    do = (rand((1, S, 2, 64), torch.float32, 4) * size[None, :, None, None]).to(dt)
+    got = results(seq, q, k, v, do, causal=True, doc_q=ids, doc_k=ids)
+    for name, g, (want, bound) in zip(('out', 'dq', 'dk', 'dv'), got, X.attention(q, k, v, do, causal=True, doc_q=ids, doc_k=ids)):
+        within(name, g, want, bound)
+        for d in range(3):
+            r = ids[0] == d
+            assert float((g[0, r].double() - want[0, r]).norm()) <= 2 * float((want[0, r].half().double() - want[0, r]).norm()), (name, d)
+
+
+def test_values_gradient_over_a_long_row_in_fp16(seq):                      # noqa: F811
+    """Probabilities of 2^-17: normal numbers of their product, not subnormal ones of seven bits."""
+    dt = torch.float16
+    q, k, v, do = rand((1, 64, 1, 32), dt, 1, 0.5), rand((1, 1 << 17, 1, 32), dt, 2, 0.5), rand((1, 1 << 17, 1, 32), dt, 3), rand((1, 64, 1, 32), dt, 4, 100.0)
+    got, ref = results(seq, q, k, v, do), X.attention(q, k, v, do)
+    rounded_once(got[3], *ref[3], 'dv')
+
+
+def spread(Sk, D, every):
+    """Queries of 1 and keys whose scores are 25.5 ln 2 at every so-many-th place and 0 elsewhere; values there 0, elsewhere about 1000."""
+    top = 25.5 * 0.6931471805599453 / D ** 0.5
+    k = torch.zeros(1, Sk, 1, D, device='cuda')
+    k[:, ::every] = top
+    v = rand((1, Sk, 1, D), torch.float32, 3) * 100 + 1000
+    v[:, ::every] = 0
+    return torch.ones(1, 3, 1, D, device='cuda').half(), k.half(), v.half()
+
+
+def test_many_small_probabilities_in_fp16(seq):                             # noqa: F811
+    """A few keys take nearly all the weight; what the thousands of others share, 2^-25 of theirs each, is the whole result."""
+    q, k, v = spread(8192, 64, 64)
+    ref = X.attention(q, k, v, torch.zeros_like(q))[0]
+    out = seq.masked_attention(q, k, v)
+    within('out', out, *ref)
+    assert float((ref[0].abs() > 4 * ref[1]).double().mean()) > 0.9
+    q, k, v = spread(8192, 64, 32)
+    ref = X.attention(q[:, :1], k, v, torch.zeros_like(q[:, :1]))[0]
+    table = torch.arange(128, dtype=torch.int32, device='cuda').view(1, 128)
+    w = torch.zeros(1, 1, 8192, device='cuda')
+    n = torch.tensor([8192], dtype=torch.int32, device='cuda')
+    for weights in (None, w):
+        out = seq.paged_attention(q[0, :1], k.view(128, 64, 1, 64), v.view(128, 64, 1, 64), table, n, weights=weights)
+        within('paged', out[None], *ref)
+    want, bound = R.paged(q[0, :1], k.view(128, 64, 1, 64), v.view(128, 64, 1, 64), table, n)[2:]
+    within('weights', w, want, bound)
