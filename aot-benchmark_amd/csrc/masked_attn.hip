@@ -1165,7 +1165,10 @@ template <class F> static void with_tile(int dtype, int D, F&& f) {
 
 // Where the blocks of 128 queries (or of keys) are too few for the chip's 256 CUs twice over, several workgroups share the tiles of one
 // block, every n-th tile each (even under a causal mask), a power of two of them (split keys: with at least four tiles each).  Their 32-bit sums go
-// through a workspace: 8 bytes an element and split more.  2047 queries on 8191 keys, 16 heads of 64: 188 us in one piece, 140 in two.
+// through a workspace: 8 bytes an element and split more.  Forward / backward, us, where the aim is no split, 256, 512 (taken) and 1024 workgroups,
+// causal: 16 queries on 8192 keys, 8 heads of 128 225 / 340, 31 / 65, 31 / 65, 31 / 65; 2047 on 8191, 16 / 8 of 64 174 / 540, 174 / 540, 133 / 468,
+// 127 / 487; 1024 on 4096, 16 of 128 124 / 270, 76 / 206, 65 / 191, 75 / 225; 2048, 16 of 128 66 / 177, 66 / 178, 63 / 148, 62 / 176; fp32 2 x 900, 8 of
+// 32 46 / 143, 32 / 90, 33 / 90, 33 / 96.
 static int mask_split(long blocks, int tiles) {
   int n = 1;
   while (n < 16 && blocks * n < 512 && 8 * n <= tiles) n *= 2;

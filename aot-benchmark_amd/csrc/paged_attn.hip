@@ -430,7 +430,9 @@ extern "C" int aot_paged_attn(const void* q, const void* k_pages, const void* v_
   p.ml = work + (long)B * H * p.nsplit * D;
   p.scores = work + part_floats(B, H, D, p.nsplit);
   const bool split = need > 0;
-  p.osplit = p.nsplit >= 32 && D % 32 == 0 ? D / 32 : 1;          // many splits: a head's output by 32 columns a workgroup
+  // A head's sums by 32 columns a workgroup where they are 64 KB and more: the reading of one workgroup outweighs that of the splits' (m, l) by each.
+  // Join with whole heads / by columns: D = 128, 64 splits 4.1 / 4.3 us, 128 5.4 / 4.6, 1024 8.8 / 6.0; D = 256, 64 splits 5.2 / 4.8, 1024 14.8 / 6.5.
+  p.osplit = (long)p.nsplit * D >= 16384 && D % 32 == 0 ? D / 32 : 1;
   const long joins = (long)B * H * p.osplit + (weights ? (long)B * Hk * ((cap + JOIN_KEYS - 1) / JOIN_KEYS) : 0);
   if (split && joins >= 1L << 24) return AOT_ERR_UNSUPPORTED;     // (a launch's work items are below 2^32)
   const dim3 grid(p.nsplit, Hk * qt, B);

@@ -120,7 +120,10 @@ static int rope_launch(RopeP& p, int dtype, hipStream_t stream) {
   const int n = std::max((p.inter ? p.rot : p.rot / 2) / ve + (p.D - p.rot) / ve, 1);
   p.up_shift = 0;
   while ((1 << p.up_shift) < n && p.up_shift < 8) ++p.up_shift;
-  p.R = p.rows >= 8192 ? 4 : 1;
+  // Rows a workgroup: one while that is what fills the 256 CUs, two as soon as eight workgroups a CU remain, four with sixteen a CU.  Kernel times
+  // with 1 / 2 / 4 rows, 20 heads of 128 turned: 2048 rows 7.1 / 6.6 / 8.1 us, 4096 11.5 / 9.9 / 11.2, 8192 18.0 / 16.4 / 16.4, 65536 159 / 137 / 134;
+  // three heads of 64: 4096 6.7 / 6.1 / 6.6, 16384 18.2 / 14.4 / 13.2; appended, 24 heads of 128: 2048 6.8 / 7.2 / 8.8, 8191 19.7 / 19.2 / 19.8.
+  p.R = p.rows >= 16384 ? 4 : p.rows >= 4096 ? 2 : 1;
   const size_t lds = (size_t)p.R * (p.rot / 2) * sizeof(float2);
   const long blocks = (p.rows + p.R - 1) / p.R;
   if (blocks >= 1L << 24) return AOT_ERR_UNSUPPORTED;          // (a launch's work items are below 2^32)

@@ -232,3 +232,21 @@ def test_many_small_probabilities_in_fp16(seq):                             # no
         within('paged', out[None], *ref)
     want, bound = R.paged(q[0, :1], k.view(128, 64, 1, 64), v.view(128, 64, 1, 64), table, n)[2:]
     within('weights', w, want, bound)
+
+
+# ---- rotary rows: one, two or four a workgroup -----------------------------------------------------------------------------------------
+@pytest.mark.parametrize('dtype', DT)
+@pytest.mark.parametrize('S,inter', [(4097, False), (16387, True), (16385, False)])
+def test_rotary_rows_a_workgroup(seq, dtype, S, inter):                     # noqa: F811
+    """Odd numbers of rows where a workgroup takes several: the same bits as the rows in short calls, appended too."""
+    dt = DT[dtype]
+    q, k = rand((S, 2, 32), dt, 1), rand((S, 1, 32), dt, 2)
+    pos, freqs = torch.arange(S, dtype=torch.int32, device='cuda') * 7, seq.rope_freqs(20, device='cuda')
+    a, b = seq.rope(q[None], k[None], pos, freqs, interleaved=inter)
+    short = [seq.rope(q[None, i:i + 1000], k[None, i:i + 1000], pos[i:i + 1000], freqs, interleaved=inter) for i in range(0, S, 1000)]
+    assert torch.equal(a, torch.cat([x for x, _ in short], 1)) and torch.equal(b, torch.cat([x for _, x in short], 1))
+    pages = [torch.zeros(S // 16 + 1, 16, 1, 32, dtype=dt, device='cuda') for _ in range(2)]
+    slots = torch.arange(S, dtype=torch.int32, device='cuda')
+    t = seq.rope_append(q, k, k, pos, freqs, slots, *pages, interleaved=inter)
+    assert torch.equal(t, a[0]) and torch.equal(pages[0].view(-1, 1, 32)[:S], b[0]) and torch.equal(pages[1].view(-1, 1, 32)[:S], k)
+    assert not pages[0].view(-1, 1, 32)[S:].any()
