@@ -2,7 +2,8 @@
 
 ``import aot_hip_ops`` defines one dispatcher op per fused stage, implemented for the ROCm ("CUDA") dispatch key only
 by the ctypes wrappers of ``aot_hip`` -- a CPU tensor therefore fails in the dispatcher ("no CPU fallback"), and the ops
-run on torch's current HIP stream.  All ops write into caller-provided outputs (``Tensor(a!)``), like the C ABI.
+run on torch's current HIP stream.  The frame engine's ops write into caller-provided outputs (``Tensor(a!)``), like the C ABI;
+those of token sequences return new tensors beside the caches that they update.
 
 The engine itself calls ``aot_hip.<fn>`` directly: a frame is ~200 launches and the dispatcher adds several microseconds
 to each, which matters once three clips share one GPU.  The ops are the integration surface for code

@@ -782,7 +782,7 @@ __global__ __launch_bounds__(256, (sizeof(T) == 2 ? 2 : 1) + (DP == 32)) void at
     t = tn;
     full = fulln;
   }
-  // The seen infinities and NaN that staging left out, if it met any (in a masked tile): once more over the masked tiles
+  // The seen infinities and NaN that the product left out, if it met any (in a masked tile): once more over the masked tiles
   if (lane == 0) sbad[wave] = dirty;
   __syncthreads();
   if (any_flag<4>(sbad)) {

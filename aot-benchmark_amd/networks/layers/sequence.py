@@ -105,7 +105,7 @@ def masked_attention(q, k, v, scale=None, causal=False, softcap=0.0, slopes=None
     """Attention of q [B, Sq, H, D] over k / v [B, Sk, Hk, D] (H a multiple of Hk), differentiable in the three; out like q.
 
     Query i stands at place i + Sk - Sq among the keys.  scale (positive): 1 / sqrt(D) by default.  causal: keys up to the query's place.
-    softcap: scores become softcap * tanh(score / softcap).  slopes float32 [H]: slopes[h] * |distance| is taken off the score (no gradient).
+    softcap: scores become softcap * tanh(score / softcap), 0: none.  slopes float32 [H]: slopes[h] * |distance| is taken off the score (no gradient).
     doc_q int32 [B, Sq], doc_k int32 [B, Sk]: a query sees the keys of its own document; a negative id is padding and sees nothing.
     prefix int32 [B]: under `causal`, keys before prefix[b] are seen by every query.  A query that sees nothing gives zeros and takes no
     gradient; what masked places hold never reaches a result."""
@@ -133,7 +133,8 @@ def cache_slots(table, seq, pos, page):
 
 def rope_append(q, k, v, pos, freqs, slots, k_pages, v_pages, interleaved=False, mscale=1.0):
     """Turns the new tokens' q [N, H, D] (or None) and k [N, Hk, D] by pos int32 [N], writes the turned keys and v [N, Hk, D] to the places slots
-    int32 [N] (cache_slots; negative: a padded token, nothing is written) of k_pages / v_pages [pages, page, Hk, D], returns the turned q."""
+    int32 [N] (cache_slots; negative: a padded token, nothing is written; a place named twice holds parts of either token) of k_pages / v_pages
+    [pages, page, Hk, D], returns the turned q."""
     _no_grad('rope_append', q, k, v, freqs, k_pages, v_pages)
     return aot_hip.rope_append(q, k, v, pos, freqs, slots, k_pages, v_pages, bool(interleaved), float(mscale))
 
@@ -152,6 +153,7 @@ def paged_evict(k_pages, v_pages, table, lengths, weights, new_table, budget, si
     """Thins every cache row to `budget` entries: the first `sink`, the last `recent`, and of the rest those that collected most weight
     (ties: the earlier).  The kept rows are copied, in order, into the pages of new_table int32 [B, new_pages] -- pages no sequence uses;
     the old ones stay as they are for whoever shares them.  Key heads choose for themselves.  Returns (kept int32 [B, Hk, budget]: old places,
-    -1 behind the last; new lengths; new weights and new key_pos, moved along)."""
+    -1 behind the last; new lengths; new weights and new key_pos, moved along).  Ids of -1 in new_table copy nothing: such a sequence goes on with
+    its old table row, length, weights and positions."""
     _no_grad('paged_evict', k_pages, v_pages, weights)
     return aot_hip.paged_evict(k_pages, v_pages, table, lengths, weights, new_table, budget, sink, recent, key_pos)

@@ -531,7 +531,7 @@ int aot_rope(const void* q, const void* k, void* qo, void* ko, const int* pos, c
              int H, int Hk, int D, int rot, int interleaved, int inverse, float mscale, const long* strides, void* stream);
 /* The same turn for N new tokens q [N, H, D], k [N, Hk, D] at pos [N], the turned keys and the values v [N, Hk, D] written to the cache
  * slots slots[n] = page_id * page + place of k_pages / v_pages (num_pages pages of `page` places, a power of two).  A negative slot, or one
- * outside the pool, writes nothing (padded tokens); two tokens with one slot leave either.  H = 0: keys and values only.
+ * outside the pool, writes nothing (padded tokens); two tokens of a call with one slot leave parts of either there.  H = 0: keys and values only.
  * strides: q n h, k n h, v n h, qo n h, k_pages page place h, v_pages page place h (14). */
 int aot_rope_append(const void* q, const void* k, const void* v, void* qo, void* k_pages, void* v_pages, const int* pos,
                     const int* slots, const double* freqs, int dtype, int N, int H, int Hk, int D, int rot, int interleaved,
@@ -541,7 +541,8 @@ int aot_rope_append(const void* q, const void* k, const void* v, void* qo, void*
  * -inf for a row that sees nothing, whose output is zero).  Query i stands at place i + Sk - Sq of the key sequence.
  *   s = softcap tanh(scale q.k / softcap) - slopes[h] |i + Sk - Sq - t|      (scale > 0; softcap = 0: no cap; slopes [H] or NULL)
  * Key t is seen if (not causal, or t <= i + Sk - Sq, or t < prefix[b]) and (no documents, or doc_q[b, i] == doc_k[b, t] >= 0).  A negative
- * document id marks padding.  What masked places hold (NaN, infinities) does not reach the result.  prefix [B] or NULL (read with causal
+ * document id marks padding.  What masked places hold (NaN, infinities) does not reach the result; what seen ones hold does, in the gradients
+ * too.  The cap may be of any size: errors are relative to the capped score.  prefix [B] or NULL (read with causal
  * only); doc_q [B, Sq] / doc_k [B, Sk] both or neither, then `ranges` is scratch of 16 * B * (ceil(Sq / 64) + ceil(Sk / 64)) bytes, 16-byte
  * aligned.  residual (16-bit types, dense [B, Sq, H, D], or NULL): what rounding out left, for the backward call.  work: scratch of
  * aot_attn_masked_floats(.., 0, ..) floats (0: may be NULL), 16-byte aligned.  D <= 128, rows of whole 16-byte pieces, 16-byte aligned, outputs
@@ -583,7 +584,8 @@ int aot_paged_attn_work_floats(int B, int H, int Hk, int D, int page, int max_pa
  * rows are copied in order to the pages of new_table [B, new_pages] (max_pages * page, new_pages * page <= 2^30; new_pages * page >= budget < 2^29; pages of the pool that no live sequence
  * reads -- the old pages are left as they are and may be shared).  kept [B, Hk, budget]: their old indices, -1 behind the last;
  * new_lengths [B]; new_weights / new_key_pos [B, Hk, S]: moved along, zero behind the last (key_pos optional, both or neither).  A page id
- * outside the pool moves nothing; a negative id in new_table keeps a sequence where it is (its indices are still reported).
+ * outside the pool moves nothing, in table or in new_table; what is returned for its sequence is that of the move all the same (to leave a sequence
+ * as it is, give it ids of -1 in new_table and go on with its old table row, length, weights and positions).
  * strides: k_pages page place h, v_pages page place h, table b, new_table b, weights b h, new_weights b h, key_pos b h,
  * new_key_pos b h (16).  Beside the first-and-latest rule of the bounded memory bank (aot_engine.py:307-338). */
 int aot_paged_evict(void* k_pages, void* v_pages, const int* table, const int* new_table, const int* lengths, const float* weights,
