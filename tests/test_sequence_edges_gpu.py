@@ -146,6 +146,20 @@ def test_seen_infinities_and_nan_in_the_gradients(seq, dtype, fill, which, softc
 
 
 @pytest.mark.parametrize('dtype', DT)
+@pytest.mark.parametrize('which', ['q', 'k', 'v', 'do'])
+def test_seen_infinities_where_the_sides_are_split(seq, dtype, which):      # noqa: F811
+    """Few queries over many keys: several workgroups share a block's tiles, one of them meets the element."""
+    dt = DT[dtype]
+    for place in (5, 130):
+        x = dict(q=rand((1, 140, 2, 32), dt, 1, 0.7), k=rand((1, 1100, 1, 32), dt, 2, 0.7), v=rand((1, 1100, 1, 32), dt, 3), do=rand((1, 140, 2, 32), dt, 4))
+        at = place if which in ('q', 'do') else 960 + place
+        x[which][0, at, 0, 6] = float('inf')
+        got = results(seq, x['q'], x['k'], x['v'], x['do'], causal=True, softcap=5.0)
+        for name, g, (want, bound) in zip(('out', 'dq', 'dk', 'dv'), got, X.attention(x['q'], x['k'], x['v'], x['do'], causal=True, softcap=5.0)):
+            same_kind('%s, %s at %d' % (name, which, at), g, want, bound)
+
+
+@pytest.mark.parametrize('dtype', DT)
 def test_seen_infinities_within_documents(seq, dtype):                      # noqa: F811
     dt, D = DT[dtype], 64
     ids = docs_of(1, 200, 4, 5, 13)
